@@ -249,6 +249,22 @@ int nml_l1_forward(const void* a, const void* b, size_t n, float denom, float* l
                    size_t workspace_bytes, void* stream);
 int nml_l1_backward(const void* a, const void* b, size_t n, const float* dloss, float denom, void* da, void* stream);
 
+/* Log probabilities of given tokens with the entropy of each row and its `top` most likely alternatives, from logits
+ * [rows][vocab] (`pitch` elements apart, dtype NML_F32 or NML_F16, any alignment of an element), in one launch and one pass:
+ *   log_probs[r] = log softmax(x_r)[targets[r]], entropy[r] = -sum p log p, stats[r] = (largest logit m, log sum e^(x - m)),
+ *   top_log_probs / top_indices [rows][top], the most likely first, equal ones by index.
+ * A negative target stands for padding: log probability 0, no gradient; one of vocab or more gives NaN.  A row whose logits are all
+ * -inf has log probabilities -inf, entropy 0, stats (-inf, 0) and the alternatives 0, 1, ...; a row with a NaN or +inf has NaN
+ * (and alternatives that are valid, otherwise unspecified, indices).  Sums are fp32, in a fixed order.
+ * top: 0 (both pointers may be NULL) to 32, at most vocab; with alternatives vocab is at most 2,000,000 / 1,000,000 (fp16 / fp32). */
+int nml_token_log_probs(const void* logits, int dtype, long long rows, int vocab, long long pitch, const long long* targets, int top,
+                        float* log_probs, float* entropy, float* stats, float* top_log_probs, long long* top_indices, void* stream);
+/* d_logits = d_log_probs (1[j = target] - p_j) - d_entropy p_j (log p_j + entropy), in the logits' type; d_entropy may be NULL (then
+ * entropy may be too).  Rows of -inf alone get zeros.  d_logits may be the logits' own memory (with their pitch). */
+int nml_token_log_probs_backward(const void* logits, int dtype, long long rows, int vocab, long long pitch, const long long* targets,
+                                 const float* stats, const float* entropy, const float* d_log_probs, const float* d_entropy, void* d_logits,
+                                 long long d_pitch, void* stream);
+
 /* Max pooling of an NHWC fp16 tensor (channels a multiple of 8), output size (h + 2 pad - k)/stride + 1.
  * The forward also writes one byte per output value naming the window tap that won (`index`,
  * batch * ho * wo * channels bytes); the backward gathers dy through it, writes every element of

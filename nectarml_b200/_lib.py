@@ -66,6 +66,8 @@ SYMBOLS = {
     "nml_l1_backward": (_I, [_VP, _VP, _SZ, _VP, C.c_float, _VP, _VP]),
     "nml_act_forward": (_I, [_VP, C.c_longlong, _I, _I, C.c_float, _VP, _VP, _I, _VP]),
     "nml_act_backward": (_I, [_VP, _I, _VP, _I, _VP, C.c_longlong, _I, _I, C.c_float, _VP, _VP]),
+    "nml_token_log_probs": (_I, [_VP, _I, C.c_longlong, _I, C.c_longlong, _VP, _I, _VP, _VP, _VP, _VP, _VP, _VP]),
+    "nml_token_log_probs_backward": (_I, [_VP, _I, C.c_longlong, _I, C.c_longlong, _VP, _VP, _VP, _VP, _VP, _VP, C.c_longlong, _VP]),
     "nml_maxpool_forward": (_I, [_VP, _I, _I, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
     "nml_maxpool_backward": (_I, [_VP, _VP, _I, _I, _I, _I, _I, _I, _I, _VP, _VP]),
     "nml_grads_check": (_I, [_VP, _SZ, C.c_float, _VP, _VP]),

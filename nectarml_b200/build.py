@@ -1,7 +1,8 @@
 """In-tree build of the CUDA library (nvcc, sm_100a only).
 
 ``python -m nectarml_b200.build`` compiles ``csrc/nml_api.cu`` (which includes the contraction
-kernels) and ``csrc/nml_layers.cu`` (normalisation / optimizer kernels of the training step) into ``nectarml_b200/libnectarml_b200.so``,
+kernels), ``csrc/nml_layers.cu`` (normalisation / optimizer kernels of the training step) and ``csrc/nml_logits.cu`` (token log
+probabilities) into ``nectarml_b200/libnectarml_b200.so``,
 ``csrc/nml_torch.cpp`` (the tensor-level host path on top of that library's C ABI) into ``nectarml_b200/_native.so``, and
 ``csrc/nml_dropin.cpp`` (the drop-in's calls of the same ABI) into ``nectarml_b200/_dropin.so``.
 nvcc cross-compiles without a GPU.
@@ -14,8 +15,8 @@ import sys
 import sysconfig
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = [os.path.join(_HERE, "csrc", "nml_api.cu"), os.path.join(_HERE, "csrc", "nml_layers.cu")]
-HEADERS = [os.path.join(_HERE, "csrc", n) for n in ("nml_launch.cuh", "nml_ptx.cuh", "nml_umma.cuh", "nml_prepass.cuh", "nml_gemm.cuh")] + [
+SOURCES = [os.path.join(_HERE, "csrc", n) for n in ("nml_api.cu", "nml_layers.cu", "nml_logits.cu")]
+HEADERS = [os.path.join(_HERE, "csrc", n) for n in ("nml_launch.cuh", "nml_host.cuh", "nml_ptx.cuh", "nml_umma.cuh", "nml_prepass.cuh", "nml_gemm.cuh")] + [
     os.path.join(os.path.dirname(_HERE), "include", "nectarml_b200.h")]
 OUTPUT = os.path.join(_HERE, "libnectarml_b200.so")
 NATIVE_SOURCE = os.path.join(_HERE, "csrc", "nml_torch.cpp")

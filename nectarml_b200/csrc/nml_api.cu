@@ -18,6 +18,7 @@
 #include "nml_prepass.cuh"
 #include "nml_umma.cuh"
 #include "nml_gemm.cuh"
+#include "nml_host.cuh"
 
 namespace nml {
 
@@ -297,6 +298,8 @@ static int device_state(DeviceState** out) {
         if (rc_attr) return rc_attr;
         rc_attr = load_helper_kernels();
         if (rc_attr) return rc_attr;
+        rc_attr = prepare_logits_kernels();
+        if (rc_attr) return rc_attr;
         s.err = static_cast<int*>(status);
         s.attr_set = true;
     }
@@ -324,6 +327,21 @@ static int planning_sms() {
     }
     cached.store(sms);
     return limited(sms);
+}
+
+int current_device(int** status_word, int* sms) {
+    DeviceState* ds = nullptr;
+    const int rc = device_state(&ds);
+    if (rc) return rc;
+    *status_word = ds->err;
+    *sms = limited(ds->sms);
+    return NML_OK;
+}
+int usable_sms() { return planning_sms(); }
+void count_launches(int n) { g_launches += n; }
+int cuda_failed(int error, const char* what) {
+    set_last_cuda_error(static_cast<cudaError_t>(error), what);
+    return NML_ERR_CUDA;
 }
 
 struct MathInfo {

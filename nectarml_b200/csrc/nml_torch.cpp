@@ -14,6 +14,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/engine.h>
@@ -978,8 +979,106 @@ PyObject* py_l1_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// ------------------------------------------------------------------ token log probabilities --
+// Rows of a tensor [..., vocab] without a copy: the last dimension is dense and the leading ones are steps of one pitch.
+struct Rows {
+    void* p;
+    int64_t rows, cols, pitch;
+};
+Rows rows_of(const at::Tensor& t, const char* what) {
+    if (!t.is_cuda()) fail("tensors must live on a CUDA device (there is no CPU path)");
+    if (t.dim() < 1) fail_assert(what);
+    Rows r{t.data_ptr(), 1, t.size(-1), t.size(-1)};
+    require(r.cols <= 1 || t.stride(-1) == 1, what);
+    bool first = true;
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (first) r.pitch = t.stride(d);
+        else require(t.numel() == 0 || t.stride(d) == r.pitch * r.rows, what);
+        first = false;
+        r.rows *= t.size(d);
+    }
+    require(t.numel() == 0 || r.pitch >= r.cols, what);
+    return r;
+}
+// A dense tensor of the device and type that a call needs.
+const at::Tensor& operand(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, int64_t count, const char* what) {
+    require(t.scalar_type() == type && t.numel() == count && t.device() == like.device(), what);
+    return t;
+}
+int vocab_of(const Rows& r) {
+    require(r.cols > 0 && r.cols <= 0x7fffffff, "logits [..., vocab] with 1 to 2^31 - 1 tokens");
+    return static_cast<int>(r.cols);
+}
+const char* const kLogits = "logits [..., vocab]: the last dimension dense, the leading ones steps of one pitch";
+const char* const kTargets = "targets: int64 on the logits' device, one per row";
+
+// token_log_probs(logits, targets, top) -> (log_probs, entropy, stats, top_log_probs, top_indices)
+PyObject* py_token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 3)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor &x = tensor(a[0], "logits"), &targets = tensor(a[1], "targets");
+        const int dtype = dtype_of(x);
+        const long top = as_int(a[2]);
+        const Rows r = rows_of(x, kLogits);
+        const int vocab = vocab_of(r);
+        require(targets.sizes() == x.sizes().slice(0, x.dim() - 1), "targets: the logits' shape without the last dimension");
+        void* const pt = ptr(operand(targets, x, at::kLong, r.rows, kTargets));
+        require(top >= 0 && top <= 32 && top <= vocab, "top: 0 to 32 alternatives, at most the vocabulary");
+        const c10::cuda::CUDAGuard device(x.device());
+        const auto f32 = at::TensorOptions().dtype(at::kFloat).device(x.device());
+        auto shape = targets.sizes().vec();
+        const at::Tensor lp = new_empty(shape, f32), entropy = new_empty(shape, f32);
+        shape.push_back(2);
+        const at::Tensor stats = new_empty(shape, f32);
+        shape.back() = top;
+        at::Tensor top_lp, top_index;
+        if (top) {
+            top_lp = new_empty(shape, f32);
+            top_index = new_empty(shape, f32.dtype(at::kLong));
+        }
+        if (r.rows > 0) {
+            float *const pl = floats(lp), *const pe = floats(entropy), *const ps = floats(stats), *const ptl = top ? floats(top_lp) : nullptr;
+            void* const pti = top ? ptr(top_index) : nullptr;
+            issue([&](void* st) {
+                return nml_token_log_probs(r.p, dtype, r.rows, vocab, r.pitch, static_cast<const long long*>(pt), static_cast<int>(top), pl, pe,
+                                           ps, ptl, static_cast<long long*>(pti), st);
+            });
+        }
+        return tuple_of(lp, entropy, stats, top_lp, top_index);
+    });
+}
+
+// token_log_probs_backward(logits, targets, stats, entropy, d_log_probs, d_entropy, out) -> d_logits
+PyObject* py_token_log_probs_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 7)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor &x = tensor(a[0], "logits"), &targets = tensor(a[1], "targets");
+        const int dtype = dtype_of(x);
+        const Rows r = rows_of(x, kLogits);
+        const int vocab = vocab_of(r);
+        void* const pt = ptr(operand(targets, x, at::kLong, r.rows, kTargets));
+        float* const ps = floats(operand(tensor(a[2], "stats"), x, at::kFloat, 2 * r.rows, "stats: as token_log_probs returned them"));
+        const at::Tensor *entropy = tensor_or_none(a[3], "entropy"), *d_entropy = tensor_or_none(a[5], "d_entropy");
+        require(!d_entropy || entropy, "the gradient of the entropy needs the entropy");
+        float* const pe = d_entropy ? floats(operand(*entropy, x, at::kFloat, r.rows, "entropy: as token_log_probs returned it")) : nullptr;
+        float* const pd = floats(operand(tensor(a[4], "d_log_probs"), x, at::kFloat, r.rows, "d_log_probs: float32, one per row"));
+        float* const ph = d_entropy ? floats(operand(*d_entropy, x, at::kFloat, r.rows, "d_entropy: float32, one per row")) : nullptr;
+        const c10::cuda::CUDAGuard device(x.device());
+        const at::Tensor out = a[6] != Py_None ? tensor(a[6], "out") : new_empty(x.sizes(), at::TensorOptions().dtype(x.scalar_type()).device(x.device()));
+        require(out.scalar_type() == x.scalar_type() && out.device() == x.device() && out.sizes() == x.sizes(), "out: shape, dtype and device of the logits");
+        const Rows o = rows_of(out, "out [..., vocab]: the last dimension dense, the leading ones steps of one pitch");
+        if (r.rows > 0)
+            issue([&](void* st) {
+                return nml_token_log_probs_backward(r.p, dtype, r.rows, vocab, r.pitch, static_cast<const long long*>(pt), ps, pe, pd, ph, o.p,
+                                                    o.pitch, st);
+            });
+        return THPVariable_Wrap(out);
+    });
+}
+
 #define NML_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {NML_FAST(geometry), NML_FAST(conv_forward), NML_FAST(conv_backward_data), NML_FAST(conv_backward_weight),
+PyMethodDef kMethods[] = {NML_FAST(token_log_probs), NML_FAST(token_log_probs_backward), NML_FAST(geometry), NML_FAST(conv_forward), NML_FAST(conv_backward_data), NML_FAST(conv_backward_weight),
                           NML_FAST(linear_forward), NML_FAST(linear_backward_data), NML_FAST(linear_backward_weight),
                           NML_FAST(bn_forward), NML_FAST(bn_backward), NML_FAST(act_forward), NML_FAST(act_backward),
                           NML_FAST(l1_forward), NML_FAST(l1_backward), NML_FAST(conv_layer), NML_FAST(bn_layer), {nullptr, nullptr, 0, nullptr}};

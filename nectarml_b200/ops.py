@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -210,6 +210,33 @@ def linear_backward_weight(x: torch.Tensor, dy: torch.Tensor, *, math: str = "f1
                            ws: Optional[Workspace] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """dw[out, in] = dy.T @ x (fp32), db[out] = dy.sum(0) (fp32)."""
     return _native.linear_backward_weight(x, dy, dw, db, _MATH[math], 1 if want_bias_grad else 0, ws or _default_ws)
+
+
+class TokenLogProbs(NamedTuple):
+    """What :func:`token_log_probs` returns; all float32 but ``top_indices`` (int64)."""
+    log_probs: torch.Tensor                   # [...]: of the targets
+    entropy: torch.Tensor                     # [...]
+    stats: torch.Tensor                       # [..., 2]: the largest logit m and log(sum(exp(logits - m)))
+    top_log_probs: Optional[torch.Tensor]     # [..., top], the most likely first
+    top_indices: Optional[torch.Tensor]       # [..., top]; equal ones by index
+
+
+def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0) -> TokenLogProbs:
+    """Log probabilities of the tokens ``targets`` [...] under ``logits`` [..., vocab] (float32 or float16), with the entropy of
+    every row and its ``top`` (0 to 32) most likely alternatives, in one pass over the logits.
+
+    The logits' last dimension is dense; the leading ones may be steps of any one pitch.  A negative target is padding: log
+    probability 0.  A target of ``vocab`` or more gives NaN, as does a row with NaN or +inf.  A row of -inf alone (a mask that leaves nothing)
+    has log probabilities -inf and entropy 0.  ``train.token_log_probs`` is the differentiable form."""
+    return TokenLogProbs(*_native.token_log_probs(logits, targets, top))
+
+
+def token_log_probs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, entropy: Optional[torch.Tensor],
+                             d_log_probs: torch.Tensor, d_entropy: Optional[torch.Tensor] = None, *,
+                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of the logits, in their dtype, from those of the log probabilities and (optional) the entropies; ``stats`` and
+    ``entropy`` are the forward's.  Padding takes no gradient of its log probability, a row of -inf alone none at all.  ``out`` may be the logits themselves."""
+    return _native.token_log_probs_backward(logits, targets, stats, entropy, d_log_probs, d_entropy, out)
 
 
 def device_status() -> int:

@@ -243,6 +243,29 @@ class _L1Fn(torch.autograd.Function):
         return ops._native.l1_backward(out, target, dloss, ctx.denom), None, None
 
 
+class _TokenLogProbsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top):
+        r = ops.token_log_probs(logits, targets, top=top)
+        ctx.save_for_backward(logits, targets, r.stats, r.entropy)
+        ctx.mark_non_differentiable(*[t for t in r[2:] if t is not None])
+        ctx.set_materialize_grads(False)
+        return tuple(r)
+
+    @staticmethod
+    def backward(ctx, d_log_probs, d_entropy, *_):
+        logits, targets, stats, entropy = ctx.saved_tensors
+        if d_log_probs is None and d_entropy is None:
+            return None, None, None
+        d = torch.zeros_like(entropy) if d_log_probs is None else d_log_probs.contiguous()
+        return ops.token_log_probs_backward(logits, targets, stats, entropy, d, None if d_entropy is None else d_entropy.contiguous()), None, None
+
+
+def token_log_probs(logits, targets, top=0) -> ops.TokenLogProbs:
+    """``ops.token_log_probs`` with gradients through the log probabilities and the entropies (not through the alternatives)."""
+    return ops.TokenLogProbs(*_TokenLogProbsFn.apply(logits, targets, top))
+
+
 class _MaxPoolFn(torch.autograd.Function):
     """Max pooling on NHWC fp16 (window winners recorded in the forward, gathered in the backward)."""
 
@@ -540,13 +563,22 @@ class TrainStep:
     """One optimisation step = micro-batches of forward + backward (gradients accumulate in the flat buffer),
     the bucketed all-reduce of the last micro-batch's backward, the finiteness check and the SGD-momentum update."""
 
-    def __init__(self, net: _Net, loss: str, lr=0.1, momentum=0.9, weight_decay=1e-4, loss_scale=16384.0):
+    def __init__(self, net: _Net, loss: str, lr=0.1, momentum=0.9, weight_decay=1e-4, loss_scale=16384.0, entropy_weight=0.0):
+        """loss: "cross_entropy" (torch's, of logits and labels), "token_log_probs" (the same in the library's kernels, less
+        ``entropy_weight`` times the entropy of the predictions; a negative label is left out) or "l1"."""
         self.net, self.loss_kind = net, loss
+        self.entropy_weight = entropy_weight
         self.lr, self.momentum, self.wd, self.loss_scale = lr, momentum, weight_decay, loss_scale
 
     def _loss(self, out, target, denom):
         if self.loss_kind == "cross_entropy":
             return torch.nn.functional.cross_entropy(out.float(), target, reduction="sum") / denom
+        if self.loss_kind == "token_log_probs":
+            r = token_log_probs(out, target)
+            gain = r.log_probs.sum()
+            if self.entropy_weight:
+                gain = gain + self.entropy_weight * r.entropy.sum()
+            return -gain / denom
         # (the kernels read pairs of values, so a view that starts on an odd one is left to torch, as is a count on the device)
         if (out.is_cuda and out.dtype == target.dtype == torch.float16 and out.shape == target.shape and out.is_contiguous()
                 and target.is_contiguous() and not target.requires_grad and out.numel() > 0
