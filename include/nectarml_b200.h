@@ -48,7 +48,7 @@ enum { NML_NCHW = 0, NML_NHWC = 1 };
  *  NML_MATH_3XTF32 fp32 operands split into tf32 hi + lo, three tensor-core products, fp32
  *                  accumulation (replaces cublasSgemm, conv2d.cpp:100-109)
  *  NML_MATH_TF32   single tf32 product (not used by the reference-compatible entry points) */
-enum { NML_MATH_F16 = 0, NML_MATH_3XTF32 = 1, NML_MATH_TF32 = 2 };
+enum { NML_MATH_F16 = 0, NML_MATH_3XTF32 = 1, NML_MATH_TF32 = 2, NML_MATH_3XF16 = 3 /* nml_orthogonalize, nml_muon_step */ };
 
 /* Geometry of one Conv2d (transposed = 0) or ConvTranspose2d (transposed = 1) layer plus the
  * storage formats of the tensors of one call.  batch/c_in/h/w describe the layer's INPUT;
@@ -288,6 +288,43 @@ int nml_grads_check(const float* grads, size_t n, float inv_scale, int* found_in
 int nml_sgd_momentum_step(float* params, const float* grads, float* velocity, void* params_f16, size_t n,
                           float lr, float momentum, float dampening, float weight_decay, float inv_scale,
                           const int* found_inf, void* stream);
+
+/* Orthogonalised matrices: `steps` (1 to 32) steps of X <- (a I + b A + c A^2) X with A = X X^T, starting at G / (|G| + eps) (Frobenius
+ * norm), (a, b, c) = coefficients[3 k ...] of step k (a host array).  With coefficients like 3.4445, -4.7750, 2.0315 five steps bring the
+ * singular values near 1 and keep the singular vectors.  A group of matrices of any sizes goes through the launches together.
+ *  NML_MATH_3XF16  fp32-accurate: operands as high and low fp16 halves, three products, fp32 accumulators (the normalised iterate
+ *                  fits fp16's range, which fp32 operands in general do not)
+ *  NML_MATH_F16    operands rounded to fp16, except X where it is carried to the next step: 2 to 3e-3 of the result's norm
+ * Zeros stay zeros; a matrix with a NaN or an infinity becomes NaN.  Matrices may be views: one of the strides (in elements) is 1, the other at least
+ * the length of the dense run; a result may lie where its matrix does but must not overlap another one.  Coefficients under which a singular value could
+ * grow beyond 64 are NML_ERR_UNSUPPORTED.  Results are bitwise repeatable and do not depend on the group. */
+typedef struct nml_matrix {
+    const void* in;
+    void* out;
+    int rows, cols;
+    long long in_row, in_col, out_row, out_col; /* strides */
+} nml_matrix;
+int nml_orthogonalize_workspace_size(const nml_matrix* matrices, int count, int math, int steps, size_t* bytes);
+int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int out_dtype, int math, int steps, const float* coefficients,
+                      float eps, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Optimizer step with such updates, in place on dense fp32 parameters:
+ *   g = grad * inv_scale;  v = momentum * v + g;  u = nesterov ? g + momentum * v : v
+ *   p = p (1 - lr weight_decay) - lr scale orthogonalize(u)     (rows > 0: a rows x cols matrix)
+ *   p = p (1 - lr weight_decay) - lr u                          (rows = 0: a vector of cols values)
+ * and, where param_f16 is set, the fp16 copy of p.  Nothing at all is changed when *found_inf (device int, see nml_grads_check;
+ * may be NULL) is set.  No parameter, momentum or copy may overlap another.  Beside nml_sgd_momentum_step. */
+typedef struct nml_muon_param {
+    float* param;
+    const float* grad;
+    float* momentum;
+    void* param_f16;
+    int rows, cols;
+    float scale;
+} nml_muon_param;
+int nml_muon_workspace_size(const nml_muon_param* params, int count, int math, int steps, size_t* bytes);
+int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, const float* coefficients, float eps, float lr, float momentum,
+                  int nesterov, float weight_decay, float inv_scale, const int* found_inf, void* workspace, size_t workspace_bytes, void* stream);
 long long nml_layers_launch_count(void);
 
 /* ---- reference-shaped entry points ------------------------------------------------------

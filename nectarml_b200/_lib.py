@@ -14,8 +14,18 @@ LIB_PATH = os.path.join(_HERE, "libnectarml_b200.so")
 NML_OK = 0
 NML_F32, NML_F16 = 0, 1
 NML_NCHW, NML_NHWC = 0, 1
-NML_MATH_F16, NML_MATH_3XTF32, NML_MATH_TF32 = 0, 1, 2
+NML_MATH_F16, NML_MATH_3XTF32, NML_MATH_TF32, NML_MATH_3XF16 = 0, 1, 2, 3
 NML_PASS_FORWARD, NML_PASS_BACKWARD_DATA, NML_PASS_BACKWARD_WEIGHT = 0, 1, 2
+
+
+class Matrix(C.Structure):
+    _fields_ = [("inp", C.c_void_p), ("out", C.c_void_p), ("rows", C.c_int), ("cols", C.c_int)] + [
+        (n, C.c_longlong) for n in ("in_row", "in_col", "out_row", "out_col")]
+
+
+class MuonParam(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("param", "grad", "momentum", "param_f16")] + [
+        ("rows", C.c_int), ("cols", C.c_int), ("scale", C.c_float)]
 
 
 class ConvDesc(C.Structure):
@@ -72,6 +82,11 @@ SYMBOLS = {
     "nml_maxpool_backward": (_I, [_VP, _VP, _I, _I, _I, _I, _I, _I, _I, _VP, _VP]),
     "nml_grads_check": (_I, [_VP, _SZ, C.c_float, _VP, _VP]),
     "nml_sgd_momentum_step": (_I, [_VP, _VP, _VP, _VP, _SZ, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, _VP, _VP]),
+    "nml_orthogonalize_workspace_size": (_I, [C.POINTER(Matrix), _I, _I, _I, C.POINTER(_SZ)]),
+    "nml_orthogonalize": (_I, [C.POINTER(Matrix), _I, _I, _I, _I, _I, C.POINTER(C.c_float), C.c_float, _VP, _SZ, _VP]),
+    "nml_muon_workspace_size": (_I, [C.POINTER(MuonParam), _I, _I, _I, C.POINTER(_SZ)]),
+    "nml_muon_step": (_I, [C.POINTER(MuonParam), _I, _I, _I, C.POINTER(C.c_float), C.c_float, C.c_float, C.c_float, _I, C.c_float, C.c_float,
+                           _VP, _VP, _SZ, _VP]),
     "nml_profile_begin": (_I, [_I]),
     "nml_profile_end": (_I, [C.POINTER(C.c_float), _I, C.POINTER(_I)]),
     # conv2d: ... dilation_w, groups, dtype, half_precision, result

@@ -1,8 +1,8 @@
 """In-tree build of the CUDA library (nvcc, sm_100a only).
 
 ``python -m nectarml_b200.build`` compiles ``csrc/nml_api.cu`` (which includes the contraction
-kernels), ``csrc/nml_layers.cu`` (normalisation / optimizer kernels of the training step) and ``csrc/nml_logits.cu`` (token log
-probabilities) into ``nectarml_b200/libnectarml_b200.so``,
+kernels), ``csrc/nml_layers.cu`` (normalisation / optimizer kernels of the training step), ``csrc/nml_logits.cu`` (token log
+probabilities) and ``csrc/nml_ortho.cu`` (orthogonalised updates) into ``nectarml_b200/libnectarml_b200.so``,
 ``csrc/nml_torch.cpp`` (the tensor-level host path on top of that library's C ABI) into ``nectarml_b200/_native.so``, and
 ``csrc/nml_dropin.cpp`` (the drop-in's calls of the same ABI) into ``nectarml_b200/_dropin.so``.
 nvcc cross-compiles without a GPU.
@@ -15,7 +15,7 @@ import sys
 import sysconfig
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = [os.path.join(_HERE, "csrc", n) for n in ("nml_api.cu", "nml_layers.cu", "nml_logits.cu")]
+SOURCES = [os.path.join(_HERE, "csrc", n) for n in ("nml_api.cu", "nml_layers.cu", "nml_logits.cu", "nml_ortho.cu")]
 HEADERS = [os.path.join(_HERE, "csrc", n) for n in ("nml_launch.cuh", "nml_host.cuh", "nml_ptx.cuh", "nml_umma.cuh", "nml_prepass.cuh", "nml_gemm.cuh")] + [
     os.path.join(os.path.dirname(_HERE), "include", "nectarml_b200.h")]
 OUTPUT = os.path.join(_HERE, "libnectarml_b200.so")

@@ -300,6 +300,8 @@ static int device_state(DeviceState** out) {
         if (rc_attr) return rc_attr;
         rc_attr = prepare_logits_kernels();
         if (rc_attr) return rc_attr;
+        rc_attr = prepare_ortho_kernels();
+        if (rc_attr) return rc_attr;
         s.err = static_cast<int*>(status);
         s.attr_set = true;
     }

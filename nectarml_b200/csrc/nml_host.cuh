@@ -16,5 +16,6 @@ NML_HIDDEN int cuda_failed(int error, const char* what);
 
 // Loads a file's kernels and raises their shared-memory limits on the current device (called once per device).
 NML_HIDDEN int prepare_logits_kernels();
+NML_HIDDEN int prepare_ortho_kernels();
 
 }  // namespace nml

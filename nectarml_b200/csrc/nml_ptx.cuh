@@ -13,6 +13,15 @@
 
 namespace nml {
 
+// Error codes written to the status word by a kernel that gave up on a wait.
+enum {
+    ERR_WAIT_EMPTY = 101,
+    ERR_WAIT_FULL = 102,
+    ERR_WAIT_TMEM_EMPTY = 103,
+    ERR_WAIT_TMEM_FULL = 104,
+    ERR_WAIT_DRAIN = 105
+};
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -166,6 +175,13 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, uint
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2),
         "r"(c3), "r"(c4)
         : "memory");
+}
+
+// Untiled copy into shared memory; both addresses and the size are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
 // TMA store of one box from shared memory (bulk async-group completion).

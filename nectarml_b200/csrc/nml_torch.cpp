@@ -22,6 +22,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <initializer_list>
 #include <memory>
@@ -1077,8 +1079,163 @@ PyObject* py_token_log_probs_backward(PyObject*, PyObject* const* a, Py_ssize_t 
     });
 }
 
+// ------------------------------------------------------------------ orthogonalised updates --
+// A Python sequence's items for as long as the object lives.
+struct Items {
+    PyObject* const fast;
+    Items(PyObject* o, const char* what) : fast(PySequence_Fast(o, what)) {
+        if (!fast) throw Fail();
+    }
+    Items(const Items&) = delete;
+    ~Items() { Py_DECREF(fast); }
+    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(fast); }
+    PyObject* operator[](Py_ssize_t k) const { return PySequence_Fast_GET_ITEM(fast, k); }
+};
+// The polynomial's coefficients: a flat sequence of three numbers for each step.
+std::vector<float> coefficients_of(PyObject* o) {
+    const Items items(o, "coefficients: a sequence of numbers");
+    std::vector<float> c;
+    for (Py_ssize_t k = 0; k < items.size(); ++k) c.push_back(static_cast<float>(as_double(items[k])));
+    require(!c.empty() && c.size() % 3 == 0, "three coefficients for each step");
+    return c;
+}
+int extent(int64_t v) {
+    require(v <= 0x7fffffff, "a matrix of at most 2^31 - 1 rows and columns");
+    return static_cast<int>(v);
+}
+// Strides of a matrix as nml_matrix takes them: where there is one row (column), the step to the next one means nothing.
+void strides_of(const at::Tensor& t, long long* row, long long* col, const char* what) {
+    const int64_t d = t.dim(), rows = t.size(d - 2), cols = t.size(d - 1);
+    *row = t.stride(d - 2);
+    *col = t.stride(d - 1);
+    if (rows == 1) *row = *col == 1 ? cols : 1;
+    if (cols == 1) *col = *row == 1 ? rows : 1;
+    require((*col == 1 && *row >= cols) || (*row == 1 && *col >= rows), what);
+}
+
+// orthogonalize(matrices, outs, out_dtype, math, coefficients, eps, workspace) -> list of results; the lists hold tensors of two
+// dimensions, or of three for a batch.  outs: None or one tensor (or None) for each.
+PyObject* py_orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 7)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const Items in(a[0], "matrices: a sequence of tensors");
+        const long out_code = as_int(a[2]);
+        const int math = static_cast<int>(as_int(a[3]));
+        const std::vector<float> c = coefficients_of(a[4]);
+        const float eps = static_cast<float>(as_double(a[5]));
+        const char* const kStrides = "matrices with one dense dimension";
+        std::vector<nml_matrix> list;
+        std::vector<at::Tensor> results;
+        const at::Tensor* first = nullptr;
+        int in_dtype = NML_F32, out_dtype = NML_F32;
+        for (Py_ssize_t k = 0; k < in.size(); ++k) {
+            const at::Tensor& x = tensor(in[k], "matrices");
+            const int dtype = dtype_of(x);
+            if (!x.is_cuda()) fail("tensors must live on a CUDA device (there is no CPU path)");
+            require(x.dim() == 2 || x.dim() == 3, "matrices [rows, cols] or batches of them [n, rows, cols]");
+            if (!first) {
+                first = &x;
+                in_dtype = dtype;
+            }
+            require(dtype == in_dtype && x.device() == first->device(), "matrices of one dtype on one device");
+            PyObject* given = Py_None;
+            if (a[1] != Py_None) {
+                const Items outs(a[1], "out: a sequence of tensors");
+                require(outs.size() == in.size(), "out: one tensor for each matrix");
+                given = outs[k];
+            }
+            results.push_back(output(given, x.sizes(), out_code, x));
+            const at::Tensor& y = results.back();
+            require(y.sizes() == x.sizes() && y.device() == x.device(), "out: shape and device of its matrix");
+            if (k == 0) out_dtype = dtype_of(y);
+            require(dtype_of(y) == out_dtype, "results of one dtype");
+            if (x.numel() == 0) continue;
+            nml_matrix m;
+            m.rows = extent(x.size(-2));
+            m.cols = extent(x.size(-1));
+            strides_of(x, &m.in_row, &m.in_col, kStrides);
+            strides_of(y, &m.out_row, &m.out_col, kStrides);
+            const int64_t batch = x.dim() == 3 ? x.size(0) : 1;
+            require(batch <= 1 || y.stride(0) != 0, "out: a batch's results in places of their own");
+            for (int64_t b = 0; b < batch; ++b) {
+                m.in = static_cast<const char*>(x.data_ptr()) + (x.dim() == 3 ? b * x.stride(0) * x.element_size() : 0);
+                m.out = static_cast<char*>(y.data_ptr()) + (x.dim() == 3 ? b * y.stride(0) * y.element_size() : 0);
+                list.push_back(m);
+            }
+        }
+        if (!list.empty()) {
+            const int count = extent(list.size()), steps = extent(c.size() / 3);
+            const c10::cuda::CUDAGuard device(first->device());
+            size_t need = 0;
+            check(nml_orthogonalize_workspace_size(list.data(), count, math, steps, &need));
+            const Scratch ws = scratch(a[6], need, *first);
+            issue([&](void* st) {
+                return nml_orthogonalize(list.data(), count, in_dtype, out_dtype, math, steps, c.data(), eps, ws.p, ws.bytes, st);
+            });
+        }
+        PyObject* r = PyList_New(results.size());
+        if (!r) throw Fail();
+        for (size_t k = 0; k < results.size(); ++k) PyList_SET_ITEM(r, k, THPVariable_Wrap(results[k]));
+        return r;
+    });
+}
+
+// muon_step(params, grads, momenta, halves, scaling, math, coefficients, eps, lr, momentum, nesterov, weight_decay, inv_scale,
+// found_inf, workspace): in place.  scaling: 0 none, 1 sqrt(max(1, rows / cols)), 2 0.2 sqrt(max(rows, cols)).
+PyObject* py_muon_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 15)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const Items params(a[0], "params: a sequence of tensors"), grads(a[1], "grads: a sequence of tensors"),
+            momenta(a[2], "momenta: a sequence of tensors");
+        const bool has_half = a[3] != Py_None;
+        const Items halves(has_half ? a[3] : a[0], "params_f16: a sequence of tensors");
+        require(grads.size() == params.size() && momenta.size() == params.size() && halves.size() == params.size(),
+                "one gradient, momentum and half copy for each parameter");
+        const long scaling = as_int(a[4]);
+        const int math = static_cast<int>(as_int(a[5]));
+        const std::vector<float> c = coefficients_of(a[6]);
+        const float eps = static_cast<float>(as_double(a[7])), lr = static_cast<float>(as_double(a[8]));
+        const float momentum = static_cast<float>(as_double(a[9])), decay = static_cast<float>(as_double(a[11]));
+        const float inv_scale = static_cast<float>(as_double(a[12]));
+        const int nesterov = as_int(a[10]) != 0;
+        std::vector<nml_muon_param> list;
+        const at::Tensor* first = nullptr;
+        for (Py_ssize_t k = 0; k < params.size(); ++k) {
+            const at::Tensor &p = tensor(params[k], "params"), &g = tensor(grads[k], "grads"), &v = tensor(momenta[k], "momenta");
+            if (!first) first = &p;
+            nml_muon_param m;
+            m.param = floats(operand(p, *first, at::kFloat, p.numel(), "parameters are float32 on one device"));
+            require(p.dim() >= 1, "parameters of one or more dimensions");
+            m.grad = floats(operand(g, p, at::kFloat, p.numel(), "gradients are float32, on the device and of the size of their parameters"));
+            m.momentum = floats(operand(v, p, at::kFloat, p.numel(), "momenta are float32, on the device and of the size of their parameters"));
+            const at::Tensor* h = has_half ? tensor_or_none(halves[k], "params_f16") : nullptr;
+            m.param_f16 = h ? ptr(operand(*h, p, at::kHalf, p.numel(), "half copies are float16, on the device and of the size of their parameters")) : nullptr;
+            if (p.numel() == 0) continue;
+            m.rows = p.dim() == 1 ? 0 : extent(p.size(0));
+            m.cols = extent(p.dim() == 1 ? p.numel() : p.numel() / p.size(0));
+            const double rows = m.rows, cols = m.cols;
+            m.scale = static_cast<float>(scaling == 1 ? std::sqrt(std::max(1.0, rows / cols)) : scaling == 2 ? 0.2 * std::sqrt(std::max(rows, cols)) : 1.0);
+            list.push_back(m);
+        }
+        if (list.empty()) return Py_NewRef(Py_None);
+        const int* found = nullptr;
+        if (const at::Tensor* f = tensor_or_none(a[13], "found_inf"))
+            found = static_cast<const int*>(ptr(operand(*f, *first, at::kInt, 1, "found_inf: one int32 on the parameters' device")));
+        const int count = extent(list.size()), steps = extent(c.size() / 3);
+        const c10::cuda::CUDAGuard device(first->device());
+        size_t need = 0;
+        check(nml_muon_workspace_size(list.data(), count, math, steps, &need));
+        const Scratch ws = scratch(a[14], need, *first);
+        issue([&](void* st) {
+            return nml_muon_step(list.data(), count, math, steps, c.data(), eps, lr, momentum, nesterov, decay, inv_scale, found, ws.p, ws.bytes, st);
+        });
+        return Py_NewRef(Py_None);
+    });
+}
+
 #define NML_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {NML_FAST(token_log_probs), NML_FAST(token_log_probs_backward), NML_FAST(geometry), NML_FAST(conv_forward), NML_FAST(conv_backward_data), NML_FAST(conv_backward_weight),
+PyMethodDef kMethods[] = {NML_FAST(token_log_probs), NML_FAST(token_log_probs_backward), NML_FAST(orthogonalize), NML_FAST(muon_step),
+                          NML_FAST(geometry), NML_FAST(conv_forward), NML_FAST(conv_backward_data), NML_FAST(conv_backward_weight),
                           NML_FAST(linear_forward), NML_FAST(linear_backward_data), NML_FAST(linear_backward_weight),
                           NML_FAST(bn_forward), NML_FAST(bn_backward), NML_FAST(act_forward), NML_FAST(act_backward),
                           NML_FAST(l1_forward), NML_FAST(l1_backward), NML_FAST(conv_layer), NML_FAST(bn_layer), {nullptr, nullptr, 0, nullptr}};

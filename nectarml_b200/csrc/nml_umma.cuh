@@ -38,15 +38,6 @@ enum { OUT_NHWC = 0, OUT_NCHW = 1, OUT_NHWC_TMA = 2, OUT_NCHW_TMA = 3 };  // _TM
 #define NML_IS_TMA_OUT(m) ((m) == OUT_NHWC_TMA || (m) == OUT_NCHW_TMA)
 enum { KIND_F16 = 0, KIND_TF32 = 2 };
 
-// Error codes written to the status word by a kernel that gave up on a wait.
-enum {
-    ERR_WAIT_EMPTY = 101,
-    ERR_WAIT_FULL = 102,
-    ERR_WAIT_TMEM_EMPTY = 103,
-    ERR_WAIT_TMEM_FULL = 104,
-    ERR_WAIT_DRAIN = 105
-};
-
 constexpr int kMaxPhases = 16;
 constexpr int kMaxTaps = 128;
 constexpr int kStreamTaps = 9, kStreamTapsSplit = 5;  // patch walk with streamed weights: taps of a stage, at most

@@ -23,12 +23,12 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
-from typing import NamedTuple, Optional, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import (NML_F16, NML_F32, NML_MATH_3XTF32, NML_MATH_F16, NML_MATH_TF32, NML_NCHW,
+from ._lib import (NML_F16, NML_F32, NML_MATH_3XF16, NML_MATH_3XTF32, NML_MATH_F16, NML_MATH_TF32, NML_NCHW,
                    NML_NHWC, ConvDesc, check)
 
 _MATH = {"f16": NML_MATH_F16, "3xtf32": NML_MATH_3XTF32, "tf32": NML_MATH_TF32}
@@ -210,6 +210,64 @@ def linear_backward_weight(x: torch.Tensor, dy: torch.Tensor, *, math: str = "f1
                            ws: Optional[Workspace] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """dw[out, in] = dy.T @ x (fp32), db[out] = dy.sum(0) (fp32)."""
     return _native.linear_backward_weight(x, dy, dw, db, _MATH[math], 1 if want_bias_grad else 0, ws or _default_ws)
+
+
+# Five steps with these bring every singular value above about 1e-3 of the norm into 0.7 ... 1.2.
+ORTHOGONALIZE_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_ORTHO_MATH = {"f16": NML_MATH_F16, "3xf16": NML_MATH_3XF16}
+_SCALING = {None: 0, "spectral": 1, "rms": 2}
+
+
+def _polynomial(steps: int, coefficients) -> Sequence[float]:
+    """Three numbers for each step: the same ones every time, or a row (a, b, c) for each."""
+    if coefficients and hasattr(coefficients[0], "__len__"):
+        if len(coefficients) != steps or any(len(c) != 3 for c in coefficients):
+            raise _lib.NectarB200Error(f"coefficients: (a, b, c), or one such row for each of the {steps} steps")
+        return [float(v) for c in coefficients for v in c]
+    if len(coefficients) != 3:
+        raise _lib.NectarB200Error(f"coefficients: (a, b, c), or one such row for each of the {steps} steps")
+    return tuple(coefficients) * steps
+
+
+def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps: int = 5, coefficients=ORTHOGONALIZE_COEFFICIENTS,
+                  eps: float = 1e-7, math: Optional[str] = None, out_dtype: Optional[torch.dtype] = None, out=None,
+                  ws: Optional[Workspace] = None) -> Union[torch.Tensor, List[torch.Tensor]]:
+    """Orthogonalised matrices: ``steps`` of X <- (a I + b A + c A^2) X with A = X X^T, from G / (|G| + eps).
+
+    ``g``: a matrix, a batch [n, rows, cols], or a sequence of such of any sizes, float32 or float16 (all of one), which go through
+    the kernels together.  One dimension of a matrix is dense; transposed ones and slices of rows or columns are read in place.  ``math``: "3xf16"
+    (float32's default, as accurate as float32 products) or "f16" (float16's, 2 to 3e-3 of the result's norm).  ``out`` may be ``g``
+    itself.  ``coefficients``: (a, b, c), or a row for each step."""
+    single = isinstance(g, torch.Tensor)
+    items = [g] if single else g
+    if math is None:
+        math = "f16" if len(items) and items[0].dtype == torch.float16 else "3xf16"
+    if math not in _ORTHO_MATH:
+        raise _lib.NectarB200Error(f"math: 'f16' or '3xf16', got {math!r}")
+    r = _native.orthogonalize(items, out if out is None or not single else [out], _out_dtype(out_dtype), _ORTHO_MATH[math],
+                              _polynomial(steps, coefficients), eps, ws or _default_ws)
+    return r[0] if single else r
+
+
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor],
+              params_f16: Optional[Sequence[Optional[torch.Tensor]]] = None, *, lr: float, momentum: float = 0.95, nesterov: bool = True,
+              weight_decay: float = 0.0, inv_scale: float = 1.0, found_inf: Optional[torch.Tensor] = None,
+              scaling: Optional[str] = "spectral", steps: int = 5, coefficients=ORTHOGONALIZE_COEFFICIENTS, eps: float = 1e-7,
+              math: str = "3xf16", ws: Optional[Workspace] = None) -> None:
+    """One optimizer step with orthogonalised updates, in place on dense float32 ``params`` and ``momenta`` (and their float16 copies):
+    with g = grad * inv_scale, v = momentum * v + g and u = g + momentum * v (``nesterov``) or v,
+
+        p = p * (1 - lr * weight_decay) - lr * scale * orthogonalize(u)
+
+    for parameters of two or more dimensions, taken as matrices [first, all others]; one-dimensional ones take u itself.  ``scaling``: of
+    the update, "spectral" sqrt(max(1, rows / cols)), "rms" 0.2 sqrt(max(rows, cols)), or None.  Where the int32 ``found_inf`` is set on
+    the device, nothing changes.  A parameter is listed once."""
+    if math not in _ORTHO_MATH:
+        raise _lib.NectarB200Error(f"math: 'f16' or '3xf16', got {math!r}")
+    if scaling not in _SCALING:
+        raise _lib.NectarB200Error(f"scaling: None, 'spectral' or 'rms', got {scaling!r}")
+    _native.muon_step(params, grads, momenta, params_f16, _SCALING[scaling], _ORTHO_MATH[math], _polynomial(steps, coefficients), eps, lr,
+                      momentum, nesterov, weight_decay, inv_scale, found_inf, ws or _default_ws)
 
 
 class TokenLogProbs(NamedTuple):

@@ -125,6 +125,7 @@ class ParamStore:
         self.sm_reserve = 16
         self.sms = torch.cuda.get_device_properties(self.device).multi_processor_count if self.device.type == "cuda" else 0
         self._views = {}
+        self._muon = None
         self._bucket_index = {a: self._bucket_of(a) for a, _ in self.layer_ranges}
 
     def _view(self, buf, i):
@@ -189,7 +190,20 @@ class ParamStore:
                                              self.found_inf.data_ptr(), st))
 
 
+    def muon_step(self, lr: float, momentum: float, weight_decay: float, inv_scale: float) -> None:
+        """Finiteness check + momentum update, orthogonalised where a parameter has two or more dimensions (``ops.muon_step``); weight
+        decay is decoupled.  The momenta are those of sgd_step."""
+        lib = _lib.load()
+        if self._muon is None:
+            every = range(len(self.shapes))
+            self._muon = [[self._view(buf, i) for i in every] for buf in (self.p32, self.grad, self.vel, self.p16)]
+        _lib.check(lib.nml_grads_check(self.grad.data_ptr(), self.n, inv_scale, self.found_inf.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        ops.muon_step(*self._muon, lr=lr, momentum=momentum, weight_decay=weight_decay, inv_scale=inv_scale, found_inf=self.found_inf,
+                      ws=_muon_ws)
+
+
 _bn_ws = ops.Workspace()
+_muon_ws = ops.Workspace()
 
 
 # ------------------------------------------------------------------ autograd nodes --
@@ -563,9 +577,14 @@ class TrainStep:
     """One optimisation step = micro-batches of forward + backward (gradients accumulate in the flat buffer),
     the bucketed all-reduce of the last micro-batch's backward, the finiteness check and the SGD-momentum update."""
 
-    def __init__(self, net: _Net, loss: str, lr=0.1, momentum=0.9, weight_decay=1e-4, loss_scale=16384.0, entropy_weight=0.0):
+    def __init__(self, net: _Net, loss: str, lr=0.1, momentum=0.9, weight_decay=1e-4, loss_scale=16384.0, entropy_weight=0.0,
+                 optimizer="sgd"):
         """loss: "cross_entropy" (torch's, of logits and labels), "token_log_probs" (the same in the library's kernels, less
-        ``entropy_weight`` times the entropy of the predictions; a negative label is left out) or "l1"."""
+        ``entropy_weight`` times the entropy of the predictions; a negative label is left out) or "l1".
+        optimizer: "sgd" (momentum) or "muon" (orthogonalised momentum, see ParamStore.muon_step)."""
+        if optimizer not in ("sgd", "muon"):
+            raise ValueError(f"optimizer: 'sgd' or 'muon', got {optimizer!r}")
+        self.optimizer = optimizer
         self.net, self.loss_kind = net, loss
         self.entropy_weight = entropy_weight
         self.lr, self.momentum, self.wd, self.loss_scale = lr, momentum, weight_decay, loss_scale
@@ -691,7 +710,9 @@ class TrainStep:
             store.wait_exchange()
 
     def optimizer_step(self) -> None:
-        self.net.store.sgd_step(self.lr, self.momentum, self.wd, 1.0 / self.loss_scale)
+        store = self.net.store
+        update = store.muon_step if self.optimizer == "muon" else store.sgd_step
+        update(self.lr, self.momentum, self.wd, 1.0 / self.loss_scale)
 
     def __call__(self, micro_batches, global_count: int, optimize: bool = True) -> torch.Tensor:
         """micro_batches: list of (input NHWC fp16, target); global_count: samples (cross-entropy) or elements (L1)
@@ -708,5 +729,5 @@ class TrainStep:
         store.accumulate = False
         store.wait_exchange()
         if optimize:
-            store.sgd_step(self.lr, self.momentum, self.wd, 1.0 / self.loss_scale)
+            self.optimizer_step()
         return total if total is not None else torch.zeros((), device=self.net.device)
