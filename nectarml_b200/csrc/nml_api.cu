@@ -2784,7 +2784,7 @@ static int read_status_word(int* word, int* code) {
     snprintf(g_last_device_error, sizeof(g_last_device_error), "a kernel abandoned bounded wait %d (%s)", v,
              v == ERR_WAIT_EMPTY ? "producer: free stage" : v == ERR_WAIT_FULL ? "operands to land"
              : v == ERR_WAIT_TMEM_EMPTY ? "accumulator to drain" : v == ERR_WAIT_TMEM_FULL ? "accumulator to fill"
-             : v == ERR_WAIT_DRAIN ? "copies in flight at unwinding" : "unknown");
+             : v == ERR_WAIT_DRAIN ? "copies in flight at unwinding" : v == ERR_WAIT_TILES ? "tiles of other blocks" : "unknown");
     return NML_ERR_DEVICE;
 }
 

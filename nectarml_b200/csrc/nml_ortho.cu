@@ -6,11 +6,16 @@
 // to every matrix of a model (momentum, orthogonalisation, weight decay, fp16 copy).  The reference's optimizers
 // (nectarml/optim/sgd.py:60-90) have no such update; this stands beside nml_sgd_momentum_step.
 //
-// A group of matrices is worked on at once, each turned so that it is wide: X is m x n with m <= n.  A step is three products, each one
-// launch for the whole group:
-//   gram     A = X X^T         symmetric, the blocks on and below the diagonal; stores A and P = b I + c A
-//   square   U = a I + P A     symmetric too (polynomials of A commute)
-//   update   X = U X           (the last one writes the result, or the parameters, in the caller's layout)
+// A group of matrices is worked on at once, each turned so that it is wide: X is m x n with m <= n.  A step is three products:
+//   A = X X^T         symmetric, the blocks on and below the diagonal, with P = b I + c A beside it
+//   U = a I + P A     symmetric too (polynomials of A commute)
+//   X = U X           (the last one writes the result, or the parameters, in the caller's layout)
+// or, chained, two products X X^T and Q X for several steps (see Polynomial).
+//
+// One launch runs all products of all matrices: 15 to 17 launches in a row cost a small matrix 8 us each and a group its idle SMs at the
+// end of each.  Blocks take tiles from one counter, in an order in which every tile follows those it needs, and wait for
+// a matrix's earlier products by a counter of its own; so whatever number of blocks is running, the first waiting tile's predecessors are done or
+// being worked on.
 //
 // Operands are fp16.  |X| <= 1 bounds every element of every matrix here, so powers of two chosen on the host put all of them
 // into fp16's range, which needs no look at the data.
@@ -29,6 +34,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include <algorithm>
@@ -63,6 +69,35 @@ constexpr int kSumElements = 8192;     // of a block of the sum of squares
 // Polynomial) where steps are chained.
 enum { kGram = 0, kPoly = 1, kUpdate = 2, kUpdate2 = 3, kT = 4, kQ = 5, kQ2 = 6 };
 
+// What a product's epilogue makes of the accumulators D.
+enum {
+    POLY = 0,    // symmetric: A = D f0, and P = D f1 + d1 I beside it
+    PLAIN = 1,   // symmetric: D f0 + d1 I
+    ITERATE = 2, // X = D f1
+    RESULT = 3   // D f1 in the caller's layout, or the parameters' update
+};
+struct Symmetric {  // buffers of one symmetric product
+    int left, right, out;
+    float f0, d1;
+};
+// A product of every matrix of a class.
+struct Op {
+    int kind, jobs;            // of symmetric products: the tiles of a second one follow those of the first
+    int gram, from;            // POLY: of X X^T; which copy of X is read
+    Symmetric job[2];
+    float f1, d1;
+    int left;                  // ITERATE, RESULT: the symmetric factor
+    uint32_t identity;         // "f16": block of this step's a I
+    int symmetric_before, wide_before;  // symmetric products and products Q X of the class in front of this one
+};
+// Matrices whose steps are chained and those whose steps are single run different products; a round is one product of each.
+constexpr int kClasses = 2;
+constexpr int kMaxRounds = 4 * kMaxSteps;
+struct Round {
+    int first, of_first;       // tiles of all rounds in front, of the first class in this one
+    Op op[kClasses];
+};
+
 // One matrix of a group as the caller has it, turned wide: element (i, j), i < m <= n, is at in + i * in_i + j * in_j.
 struct Source {
     const void* in;       // the matrix, or the gradient of a parameter
@@ -82,6 +117,7 @@ struct alignas(16) Work {
     int first_half, first_gram, first_update;  // its halves of X, tiles of the symmetric products, tiles of the update
     int wide;                           // blocks of n to a tile of the update: 1 or 2
     float sx;                           // X is stored times this
+    int chained;
 };
 template <int N>
 struct Group {
@@ -89,8 +125,10 @@ struct Group {
 };
 
 struct Common {
-    const Work* table;
-    const double* sums;
+    Work* table;
+    double* sums;
+    Round* rounds;
+    int* done;        // the tile counter, and behind it every matrix's finished eighths of tiles
     uint8_t* blocks;
     const int* skip;  // the optimizer step's: do nothing where this is set
     int count;
@@ -135,18 +173,41 @@ __device__ __forceinline__ float load_as_float<__half>(const __half* p) { return
 
 // ---------------------------------------------------------------- sum of squares --
 // Partial sums of squares in double, kSumElements elements a block, in memory order; the optimizer step's momentum on the way.
-// The first block leaves the group's table in the workspace.
+// The first block leaves the group's table in the workspace and clears the counters.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&v)[4]);
+template <>
+__device__ __forceinline__ void load4<float>(const float* p, float (&v)[4]) {
+    const float4 t = load_global(reinterpret_cast<const float4*>(p));
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+}
+template <>
+__device__ __forceinline__ void load4<__half>(const __half* p, float (&v)[4]) {
+    const uint2 t = load_global(reinterpret_cast<const uint2*>(p));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&t.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&t.y));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+template <typename T>
+__device__ __forceinline__ bool vectors_of_4(const T* p) { return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0; }
+
+__device__ __forceinline__ float moved(const Momentum& mo, float grad, float old, float& next) {
+    const float g = grad * mo.inv_scale;
+    next = mo.momentum * old + g;
+    return mo.nesterov ? g + mo.momentum * next : next;
+}
+
 template <int N, typename T>
-__global__ void __launch_bounds__(256) ortho_sums_kernel(const __grid_constant__ Group<N> group, int count, Momentum mo, Work* table,
-                                                         double* sums, const int* skip) {
+__global__ void __launch_bounds__(256) ortho_sums_kernel(const __grid_constant__ Group<N> group, const Common c, const Momentum mo) {
     pdl_enter();
     __shared__ double part[8];
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < count; i += blockDim.x) table[i] = group.w[i];
-    if (skipped(skip)) return;
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < c.count; i += blockDim.x) c.table[i] = group.w[i];
+        for (int i = threadIdx.x; i <= kGroup; i += blockDim.x) c.done[i] = 0;
+    }
+    if (skipped(c.skip)) return;
     int k = 0;
     {
-        int lo = 0, hi = count - 1;
+        int lo = 0, hi = c.count - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
             if (group.w[mid].first_sum <= static_cast<int>(blockIdx.x)) lo = mid; else hi = mid - 1;
@@ -159,20 +220,40 @@ __global__ void __launch_bounds__(256) ortho_sums_kernel(const __grid_constant__
     const long long pitch = turned ? s.in_j : s.in_i;
     const long long total = static_cast<long long>(s.m) * s.n;
     const long long first = static_cast<long long>(blockIdx.x - group.w[k].first_sum) * kSumElements;
-    const long long last = min(total, first + kSumElements);
+    const int count = static_cast<int>(min(total - first, static_cast<long long>(kSumElements)));
     const T* in = static_cast<const T*>(s.in);
     double sum = 0.0;
-#pragma unroll 4
-    for (long long e = first + threadIdx.x; e < last; e += 256) {
-        const long long outer = e / inner;
-        float v = load_as_float(in + outer * pitch + (e - outer * inner));
+    const bool dense = pitch == inner || total == inner;
+    if (dense && count == kSumElements && vectors_of_4(in) && (!mo.on || vectors_of_4(s.momentum))) {
+        constexpr int kLoads = kSumElements / 1024;
+        float v[kLoads][4];
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) load4(in + first + l * 1024 + threadIdx.x * 4, v[l]);
         if (mo.on) {
-            v *= mo.inv_scale;
-            const float b = mo.momentum * load_global(s.momentum + e) + v;  // (dense, as the parameter)
-            s.momentum[e] = b;
-            v = mo.nesterov ? v + mo.momentum * b : b;
+            float b[kLoads][4];
+#pragma unroll
+            for (int l = 0; l < kLoads; ++l) load4<float>(s.momentum + first + l * 1024 + threadIdx.x * 4, b[l]);
+#pragma unroll
+            for (int l = 0; l < kLoads; ++l) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[l][q] = moved(mo, v[l][q], b[l][q], b[l][q]);
+                reinterpret_cast<float4*>(s.momentum + first + l * 1024)[threadIdx.x] = make_float4(b[l][0], b[l][1], b[l][2], b[l][3]);
+            }
         }
-        sum += static_cast<double>(v) * static_cast<double>(v);
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum += static_cast<double>(v[l][q]) * static_cast<double>(v[l][q]);
+    } else {
+        const long long outer0 = first / inner;
+        const unsigned rest = static_cast<unsigned>(first - outer0 * inner);
+#pragma unroll 4
+        for (int e = threadIdx.x; e < count; e += 256) {
+            const unsigned outer = (rest + e) / inner;
+            float v = load_as_float(in + (outer0 + outer) * pitch + (rest + e - outer * inner));
+            if (mo.on) v = moved(mo, v, load_global(s.momentum + first + e), s.momentum[first + e]);  // (dense, as the parameter)
+            sum += static_cast<double>(v) * static_cast<double>(v);
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -180,7 +261,7 @@ __global__ void __launch_bounds__(256) ortho_sums_kernel(const __grid_constant__
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 8; ++w) sum += part[w];
-        sums[blockIdx.x] = sum;
+        c.sums[blockIdx.x] = sum;
     }
 }
 
@@ -191,50 +272,39 @@ __device__ __forceinline__ uint8_t* block_at(uint8_t* blocks, uint32_t first, in
 // A block on or below the diagonal of a symmetric matrix.
 __device__ __forceinline__ int lower(int i, int j) { return i * (i + 1) / 2 + j; }
 
-// High and low half of a value.
-__device__ __forceinline__ void split(float v, __half& h, __half& l) {
-    h = __float2half_rn(v);
-    l = __float2half_rn(v - __half2float(h));
-}
-// Sixteen adjacent columns (two 16-byte chunks, c the first) of a row of a half, in its swizzle: one 32-byte store a plane.
-template <bool kLow>
-__device__ __forceinline__ void store16(uint8_t* half, int row, int c, const float (&v)[16]) {
-    uint32_t h[8], l[8];
+// High and low halves of eight values.
+__device__ __forceinline__ void split8(const float* v, uint4& high, uint4& low) {
+    uint32_t h[4], l[4];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        __half h0, l0, h1, l1;
-        split(v[2 * q], h0, l0);
-        split(v[2 * q + 1], h1, l1);
-        __half2 a = __halves2half2(h0, h1), b = __halves2half2(l0, l1);
-        h[q] = *reinterpret_cast<uint32_t*>(&a);
-        l[q] = *reinterpret_cast<uint32_t*>(&b);
+    for (int q = 0; q < 4; ++q) {
+        const __half2 a = __floats2half2_rn(v[2 * q], v[2 * q + 1]);
+        const float2 f = __half22float2(a);
+        const __half2 b = __floats2half2_rn(v[2 * q] - f.x, v[2 * q + 1] - f.y);
+        h[q] = *reinterpret_cast<const uint32_t*>(&a);
+        l[q] = *reinterpret_cast<const uint32_t*>(&b);
     }
-    // chunk c lies at c ^ (row & 7): the pair is 32-byte aligned, in turned order in odd rows
-    const bool odd = row & 1;
-    uint8_t* p = half + row * 128 + (((c ^ (row & 7)) & ~1) << 4);
-    auto put = [&](uint8_t* at, const uint32_t (&w)[8]) {
-        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(at)), "r"(odd ? w[4] : w[0]),
-                     "r"(odd ? w[5] : w[1]), "r"(odd ? w[6] : w[2]), "r"(odd ? w[7] : w[3]), "r"(odd ? w[0] : w[4]), "r"(odd ? w[1] : w[5]),
-                     "r"(odd ? w[2] : w[6]), "r"(odd ? w[3] : w[7])
-                     : "memory");
-    };
-    put(p, h);
-    if (kLow) put(p + kPlane, l);
+    high = make_uint4(h[0], h[1], h[2], h[3]);
+    low = make_uint4(l[0], l[1], l[2], l[3]);
 }
+// Place of chunk c of a row in a half of a block: the 128-byte swizzle.
+__device__ __forceinline__ uint32_t swizzled(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
 
 // ---------------------------------------------------------------- first iterate --
 // One half (128 x 64) of X to a block: the matrix over its norm, in two planes, zeros beyond its edges.  The blocks behind write the
-// identity blocks of "f16": a_k I for every step.
+// identity blocks of "f16", a_k I for every step, and the last one the rounds.
+template <int N>
 struct PackParams {
     Common c;
     Momentum mo;
     float eps;
-    int halves;
+    int halves, rounds;
     uint32_t identity;  // first block
+    int identities;
     float diagonal[kMaxSteps];
+    Round round[N];
 };
-template <typename T>
-__global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__ PackParams P) {
+template <int N, typename T>
+__global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__ PackParams<N> P) {
     pdl_enter();
     if (skipped(P.c.skip)) return;
     __shared__ float tile[64][129];
@@ -243,11 +313,18 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__
     const int tid = threadIdx.x;
     if (static_cast<int>(blockIdx.x) >= P.halves) {
         const int k = blockIdx.x - P.halves, half = k & 1;
-        for (int o = tid; o < 128 * 4; o += 256) {
-            float v[16];
+        if (k < 2 * P.identities) {
+            uint8_t* const out = block_at(P.c.blocks, P.identity, k / 2) + half * kHalf;
+            for (int o = tid; o < 128 * 8; o += 256) {
+                float v[8];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) v[q] = half * 64 + (o & 3) * 16 + q == o / 4 ? P.diagonal[k / 2] : 0.f;
-            store16<true>(block_at(P.c.blocks, P.identity, k / 2) + half * kHalf, o / 4, (o & 3) * 2, v);
+                for (int q = 0; q < 8; ++q) v[q] = half * 64 + (o & 7) * 8 + q == o / 8 ? P.diagonal[k / 2] : 0.f;
+                uint4 h, l;
+                split8(v, h, l);
+                *reinterpret_cast<uint4*>(out + swizzled(o / 8, o & 7)) = h;
+            }
+        } else {
+            for (int o = tid; o < P.rounds; o += 256) P.c.rounds[o] = P.round[o];
         }
         return;
     }
@@ -256,6 +333,9 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__
     const int k = owner_of(first, P.c.count, blockIdx.x);
     const Work w = load_work(P.c.table + k);
     const Source& s = w.s;
+    const int half = blockIdx.x - first[k], i0 = half / (2 * w.nb) * kBlock, j0 = half % (2 * w.nb) * 64;
+    uint8_t* const out = block_at(P.c.blocks, w.x[0], half / 2) + (half & 1) * kHalf;
+    if (j0 >= w.nb * kBlock) return;
     // the norm, from the partial sums in a fixed order
     double sum = 0.0;
     for (int i = tid; i < w.sums; i += 256) sum += load_double(P.c.sums + w.first_sum + i);
@@ -268,30 +348,63 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__
     for (int q = 1; q < 8; ++q) sum += part[q];
     const double norm = sqrt(sum) + static_cast<double>(P.eps);
     const double inv = norm == 0.0 ? 0.0 : static_cast<double>(w.sx) / norm;  // (zeros stay zeros without an eps too)
-    const int half = blockIdx.x - first[k], i0 = half / (2 * w.nb) * kBlock, j0 = half % (2 * w.nb) * 64;
-    const T* in = static_cast<const T*>(s.in);
-    auto value = [&](int i, int j) -> float {
-        if (i >= s.m || j >= s.n) return 0.f;
-        float v = load_as_float(in + i * s.in_i + j * s.in_j);
+    const T* const in = static_cast<const T*>(s.in);
+    auto update = [&](float v, float momentum) {  // of the element's gradient and new momentum
         if (P.mo.on) {
             v *= P.mo.inv_scale;
-            const float b = load_global(s.momentum + i * s.in_i + j * s.in_j);
-            v = P.mo.nesterov ? v + P.mo.momentum * b : b;
+            v = P.mo.nesterov ? v + P.mo.momentum * momentum : momentum;
         }
         return static_cast<float>(static_cast<double>(v) * inv);
     };
-    if (s.in_i == 1 && s.in_j != 1)
-        for (int e = tid; e < 128 * 64; e += 256) tile[e >> 7][e & 127] = value(i0 + (e & 127), j0 + (e >> 7));
-    else
-        for (int e = tid; e < 128 * 64; e += 256) tile[e & 63][e >> 6] = value(i0 + (e >> 6), j0 + (e & 63));
-    __syncthreads();
-    uint8_t* const out = block_at(P.c.blocks, w.x[0], half / 2) + (half & 1) * kHalf;
-    for (int o = tid; o < 128 * 4; o += 256) {
-        const int row = o & 127, c = o >> 7;
-        float v[16];
+    const bool turned = s.in_i == 1 && s.in_j != 1;
+    const long long pitch = turned ? s.in_j : s.in_i;
+    const bool vectors = pitch % 4 == 0 && vectors_of_4(in) && (!P.mo.on || vectors_of_4(s.momentum));
+    // four elements that lie behind one another in memory, of which `count` exist
+    auto four = [&](long long at, int count, float (&v)[4]) {
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (vectors && count >= 4) {
+            load4(in + at, v);
+            if (P.mo.on) load4<float>(s.momentum + at, b);
+        } else {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) v[q] = tile[c * 16 + q][row];
-        store16<true>(out, row, c * 2, v);
+            for (int q = 0; q < 4; ++q) {
+                v[q] = q < count ? load_as_float(in + at + q) : 0.f;
+                if (P.mo.on && q < count) b[q] = load_global(s.momentum + at + q);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = update(v[q], b[q]);
+    };
+    if (turned) {
+#pragma unroll 2
+        for (int j = tid / 32; j < 64; j += 8) {
+            const int i = (tid & 31) * 4;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            if (j0 + j < s.n && i0 + i < s.m) four(i0 + i + (j0 + j) * pitch, s.m - i0 - i, v);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tile[j][i + q] = v[q];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int o = tid; o < 128 * 8; o += 256) {
+        const int row = o >> 3, chunk = o & 7;
+        float v[8];
+        if (turned) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = tile[chunk * 8 + q][row];
+        } else {
+            const int i = i0 + row, j = j0 + chunk * 8;
+            float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
+            if (i < s.m && j < s.n) four(i * pitch + j, s.n - j, a);
+            if (i < s.m && j + 4 < s.n) four(i * pitch + j + 4, s.n - j - 4, b);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = a[q], v[4 + q] = b[q];
+        }
+        uint4 h, l;
+        split8(v, h, l);
+        *reinterpret_cast<uint4*>(out + swizzled(row, chunk)) = h;
+        *reinterpret_cast<uint4*>(out + kPlane + swizzled(row, chunk)) = l;
     }
 }
 
@@ -301,126 +414,147 @@ __device__ __forceinline__ long long load_wide(const long long* p) {
     asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(__cvta_generic_to_global(p)));
     return v;
 }
-// Sixteen results of a row, of which `count` exist, to places `step` apart; in 16-byte vectors where they lie densely.
-__device__ __forceinline__ bool dense16(const void* p, long long step, int count) { return step == 1 && count >= 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-__device__ __forceinline__ void write16(float* p, long long step, int count, const float (&v)[16]) {
-    if (dense16(p, step, count)) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) reinterpret_cast<float4*>(p)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-    } else {
-#pragma unroll
-        for (int q = 0; q < 16; ++q, p += step)
-            if (q < count) *p = v[q];
-    }
-}
-__device__ __forceinline__ void write16(__half* p, long long step, int count, const float (&v)[16]) {
-    if (dense16(p, step, count)) {
-        uint32_t h[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            __half2 t = __floats2half2_rn(v[2 * q], v[2 * q + 1]);
-            h[q] = *reinterpret_cast<uint32_t*>(&t);
-        }
-        reinterpret_cast<uint4*>(p)[0] = make_uint4(h[0], h[1], h[2], h[3]);
-        reinterpret_cast<uint4*>(p)[1] = make_uint4(h[4], h[5], h[6], h[7]);
-    } else {
-#pragma unroll
-        for (int q = 0; q < 16; ++q, p += step)
-            if (q < count) *p = __float2half_rn(v[q]);
-    }
-}
-// The same for parameters: p = p keep - rate v, and their fp16 copy.
-__device__ __forceinline__ void apply16(float* p, __half* half, long long step, int count, float (&v)[16], float keep, float rate) {
-    if (dense16(p, step, count)) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float4 w = load_global(reinterpret_cast<const float4*>(p) + q);
-            v[4 * q] = w.x * keep - rate * v[4 * q];
-            v[4 * q + 1] = w.y * keep - rate * v[4 * q + 1];
-            v[4 * q + 2] = w.z * keep - rate * v[4 * q + 2];
-            v[4 * q + 3] = w.w * keep - rate * v[4 * q + 3];
-        }
-    } else {
-        const float* r = p;
-#pragma unroll
-        for (int q = 0; q < 16; ++q, r += step)
-            if (q < count) v[q] = load_global(r) * keep - rate * v[q];
-    }
-    write16(p, step, count, v);
-    if (half) write16(half, step, count, v);
-}
-
-// What a product's epilogue makes of the accumulators D.
-enum {
-    POLY = 0,    // symmetric: A = D, and P = b I + c A beside it
-    PLAIN = 1,   // symmetric: D + d1 I
-    ITERATE = 2, // X
-    RESULT = 3   // X in the caller's layout, or the parameters' update
-};
-struct Symmetric {  // buffers of one symmetric product
-    int left, right, out;
-    float f0, d1;   // stored: D f0 (+ d1 on the diagonal)
-};
 struct ProductParams {
     Common c;
     int* err;
-    int tiles, stages, from;   // from: which copy of X is read
-    bool gram;                 // POLY of X X^T; else the jobs' operands
-    Symmetric job[2];          // the tiles of a second one follow those of the first
-    int jobs;
-    float f1, d1;              // POLY: P = D f1 + d1 I
-    float f0;                  // ITERATE, RESULT
-    int left;                  // ITERATE, RESULT: the symmetric factor
-    uint32_t identity;         // "f16": block of this step's a I
+    unsigned long long limit_ns;  // of a wait
+    int rounds, tiles;
+    int first_class;           // matrices of the first class
     int out_half;              // RESULT is fp16
     bool apply;                // RESULT goes into parameters: p = p keep - rate scale result
     float keep, rate;
 };
 
+// Results at elements e ... of the output, of which `have` exist.
+__device__ __forceinline__ void put1(const ProductParams& P, uint8_t* out, uint8_t* half, long long e, float v, float rate) {
+    if (P.apply) {
+        float* const p = reinterpret_cast<float*>(out) + e;
+        const float next = load_global(p) * P.keep - rate * v;
+        *p = next;
+        if (half) reinterpret_cast<__half*>(half)[e] = __float2half_rn(next);
+    } else if (P.out_half) {
+        reinterpret_cast<__half*>(out)[e] = __float2half_rn(v);
+    } else {
+        reinterpret_cast<float*>(out)[e] = v;
+    }
+}
+__device__ __forceinline__ void put4(const ProductParams& P, uint8_t* out, uint8_t* half, long long e, int have, float4 v, float rate) {
+    const bool f16 = P.out_half != 0;
+    const bool vectors = have >= 4 && (reinterpret_cast<uintptr_t>(out) + e * (f16 ? 2 : 4)) % (f16 ? 8 : 16) == 0 &&
+                         (!half || (reinterpret_cast<uintptr_t>(half) + e * 2) % 8 == 0);
+    if (!vectors) {
+        put1(P, out, half, e, v.x, rate);
+        if (have > 1) put1(P, out, half, e + 1, v.y, rate);
+        if (have > 2) put1(P, out, half, e + 2, v.z, rate);
+        if (have > 3) put1(P, out, half, e + 3, v.w, rate);
+        return;
+    }
+    if (P.apply) {
+        const float4 w = load_global(reinterpret_cast<const float4*>(out + e * 4));
+        v = make_float4(w.x * P.keep - rate * v.x, w.y * P.keep - rate * v.y, w.z * P.keep - rate * v.z, w.w * P.keep - rate * v.w);
+    }
+    __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    const uint2 h = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+    if (f16) {
+        *reinterpret_cast<uint2*>(out + e * 2) = h;
+    } else {
+        *reinterpret_cast<float4*>(out + e * 4) = v;
+        if (half) *reinterpret_cast<uint2*>(half + e * 2) = h;
+    }
+}
+
+
 constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kStageBytes = 196608;  // of the ring, at most
+constexpr int kThreads = 128 + 32 * kEpilogueWarps;
+// Registers: a thread of the epilogue holds 128 accumulators beside the eight columns it is splitting.  The block is launched with kLaunchRegs for each thread;
+// the four warps of the producer and the MMA give of theirs to the others' (128 x 72 + 256 x 216 = 384 x 168).
+constexpr int kLaunchRegs = 168, kControlRegs = 72, kEpilogueRegs = 216;
+static_assert(128 * kControlRegs + 32 * kEpilogueWarps * kEpilogueRegs <= kThreads * kLaunchRegs, "more than the block has: the warps that ask for more would wait for good");
+// Shared memory, all that a block may have: the ring, and 4 KB for each epilogue warp.
+constexpr int kRing = 196608, kStaging = 4096;
+constexpr size_t kProductSmem = kRing + kEpilogueWarps * kStaging + 1024;
 constexpr int kMaxStages = 6;
-constexpr size_t kProductSmem = kStageBytes + 1024;
+constexpr int kQueue = 4;            // tiles that the producer may be ahead
+
 // The tensor core truncates where it adds to an accumulator: about 2^-24 of the sum for each instruction, all to one side (measured: 2.5 x 2^-24 of a
 // sum of positive products over K = 64, 98 over 1024).  In three products over K = 8192 that was 7e-5 of the result.  So with two halves the epilogue
 // warps take the accumulators of every K slice of 64 and add them in registers, rounded to nearest, while the next slice goes to the other
 // accumulators; and within a slice the mixed products come first, while the sums are 2^11 times smaller: four additions count.
 // (One product of halves, of 2^-12, does not need it.)
 
-// What a tile of a product is made of.
+struct Info {        // of a matrix
+    int m, n, nb, wide;
+    uint32_t x[2], sym;
+    float sx;
+};
+// Thirty-two rows and columns of a result, from a warp's room in shared memory.
+__device__ __forceinline__ void write_columns(const ProductParams& P, const uint8_t* staging, uint8_t* out, uint8_t* half, float rate, long long out_i,
+                                           long long out_j, int i0, int m, int j0, int n) {
+    const int lane = threadIdx.x & 31;
+    if (out_j == 1) {
+        const int j = j0 + (lane & 7) * 4, have = n - j;
+        if (have <= 0) return;
+#pragma unroll 2
+        for (int q = 0; q < 8; ++q) {
+            const int r = q * 4 + lane / 8;
+            if (i0 + r < m) put4(P, out, half, (i0 + r) * out_i + j, have, *reinterpret_cast<const float4*>(staging + swizzled(r, lane & 7)), rate);
+        }
+    } else if (i0 + lane < m) {
+        long long e = (i0 + lane) * out_i + j0 * out_j;
+#pragma unroll 2
+        for (int q = 0; q < min(32, n - j0); ++q, e += out_j)
+            put1(P, out, half, e, *reinterpret_cast<const float*>(staging + swizzled(lane, q >> 2) + (q & 3) * 4), rate);
+    }
+}
+
+// A tile, as the producer passes it on.
 struct Tile {
-    int k;           // matrix of the group
+    int k;           // matrix of the group; -1: no more tiles
     int i, j;        // its block row; its (first) block column
     int job;
     int groups;      // 64-column groups of it
     int slices;      // of 64 along K
     int extra;       // "f16" update: slices of a I times X's low half behind them
+    int unused;
+    Info w;
+    Op op;
 };
-struct Info {        // of a matrix, in shared memory
-    int m, n, nb, wide;
-    uint32_t x[2], sym;
-    float sx;
-};
+constexpr int kOpWords = sizeof(Op) / 4;
+static_assert(kOpWords <= 32, "a lane to a word");
+__device__ __forceinline__ int claim(int* counter) {
+    int v;
+    asm volatile("atom.relaxed.gpu.global.add.s32 %0, [%1], 1;" : "=r"(v) : "l"(__cvta_generic_to_global(counter)) : "memory");
+    return v;
+}
+__device__ __forceinline__ int load_acquire(const int* p) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(__cvta_generic_to_global(p)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void add_release(int* p, int v) {
+    asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(__cvta_generic_to_global(p)), "r"(v) : "memory");
+}
+// Both directions, shared and global memory: what generic loads and stores did is seen by bulk copies, and the other way round.
+__device__ __forceinline__ void fence_proxies() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
-template <int kPlanes, int kKind>
+template <int kPlanes>
 __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid_constant__ ProductParams P) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tfull_bar[2], tempty_bar[2], drain_bar;
+    __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tfull_bar[2], tempty_bar[2], qfull_bar[kQueue], qempty_bar[kQueue],
+        drain_bar;
     __shared__ __align__(8) int abort_state[4];
     __shared__ uint32_t tmem_base;
-    __shared__ int first[kGroup];
-    __shared__ Info info[kGroup];
+    __shared__ int first_gram[kGroup], first_update[kGroup];
+    __shared__ __align__(16) Tile queue[kQueue];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     volatile int* const abort_flag = abort_state;
-    constexpr bool kWide = kKind >= ITERATE;
-    constexpr uint32_t b_bytes = kWide ? 2 * kHalf : kHalf;  // a plane of the B operand in a stage
-    constexpr uint32_t stage_bytes = kPlanes * (kHalf + b_bytes);
+    // A stage holds a K slice of both operands: 128 rows of the left one and 128 columns (symmetric products) or 256 (X) of the right one.
+    constexpr uint32_t kNarrow = kPlanes * 2 * kHalf, kWideStage = kPlanes * 3 * kHalf;
 
     if (warp == 0) nml::tmem_alloc(nml::smem_u32(&tmem_base), 512);
     if (tid == 32) {
-        for (int s = 0; s < P.stages; ++s) {
+        for (int s = 0; s < kMaxStages; ++s) {
             nml::mbar_init(nml::smem_u32(&full_bar[s]), 1);
             nml::mbar_init(nml::smem_u32(&empty_bar[s]), 1);
         }
@@ -428,105 +562,209 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
             nml::mbar_init(nml::smem_u32(&tfull_bar[b]), 1);
             nml::mbar_init(nml::smem_u32(&tempty_bar[b]), kEpilogueWarps);
         }
+        for (int q = 0; q < kQueue; ++q) {
+            nml::mbar_init(nml::smem_u32(&qfull_bar[q]), 1);
+            nml::mbar_init(nml::smem_u32(&qempty_bar[q]), 1 + kEpilogueWarps);
+        }
         nml::mbar_init(nml::smem_u32(&drain_bar), 1);
         nml::fence_mbar_init();
-        nml::abort_state_init(abort_flag, 0);
+        nml::abort_state_init(abort_flag, P.limit_ns);
     }
     pdl_enter();
     const bool skip = skipped(P.c.skip);
-    for (int i = tid; i < P.c.count; i += kThreads) {
-        const Work* w = P.c.table + i;
-        auto word = [](const uint32_t* p) { return static_cast<uint32_t>(load_global(reinterpret_cast<const int*>(p))); };
-        first[i] = load_global(kWide ? &w->first_update : &w->first_gram) * (kWide ? 1 : P.jobs);
-        info[i] = {load_global(&w->s.m), load_global(&w->s.n), load_global(&w->nb), load_global(&w->wide), {word(&w->x[0]), word(&w->x[1])},
-                   word(&w->sym), load_global(&w->sx)};
+    const int count = P.c.count;
+    for (int i = tid; i < count; i += kThreads) {
+        first_update[i] = load_global(&P.c.table[i].first_update);
+        first_gram[i] = load_global(&P.c.table[i].first_gram);
     }
     nml::tc_fence_before();
     __syncthreads();
     nml::tc_fence_after();
     const uint32_t tmem = tmem_base;
-    const int tiles = skip ? 0 : P.tiles;
-
-    auto tile_of = [&](int t) {
-        Tile r;
-        r.k = owner_of(first, P.c.count, t);
-        t -= first[r.k];
-        const Info& w = info[r.k];
-        r.extra = r.job = 0;
-        if (kWide) {
-            const int per = (w.nb + w.wide - 1) / w.wide;
-            r.i = t / per;
-            r.j = t % per * w.wide;
-            r.groups = min(2 * w.wide, (w.n - r.j * kBlock + 63) / 64);
-            r.slices = (w.m + 63) / 64;
-            if (kPlanes == 1) r.extra = min(2, r.slices - 2 * r.i);
-        } else {
-            const int mb = (w.m + kBlock - 1) / kBlock;
-            if (t >= lower(mb, 0)) t -= lower(mb, 0), r.job = 1;
-            r.i = static_cast<int>((sqrtf(8.f * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
-            while (lower(r.i, 0) > t) --r.i;
-            while (lower(r.i + 1, 0) <= t) ++r.i;
-            r.j = t - lower(r.i, 0);
-            r.groups = 2;
-            r.slices = ((P.gram ? w.n : w.m) + 63) / 64;
-        }
-        return r;
-    };
     auto symmetric_first = [&](const Info& w, int buffer) { return w.sym + buffer * lower((w.m + kBlock - 1) / kBlock, 0); };
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        return __all_sync(0xffffffffu, nml::mbar_wait(nml::smem_u32(bar), parity, abort_flag, P.err, code)) != 0;
+    };
 
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
     if (warp == 0) {
-        // ------------------------------------------------------------ producer: a lane to a copy of 8 KB
-        int s = 0, issued = 0;
-        uint32_t parity = 0;
+        // ------------------------------------------------------------ producer: takes tiles, then a lane to a copy of 8 KB
+        const int tiles = skip ? 0 : P.tiles;
+        const Round* const rounds = P.c.rounds;
+        int slot = 0, s = 0, stages = 0;
+        uint32_t qparity = 0, parity = 0, used = 0;  // bits of parity: phase of each stage's next use; of used: stages not known to be free
+        uint32_t now_stage = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-            const Tile tile = tile_of(t);
-            const Info w = info[tile.k];
-            const bool same = P.gram && tile.i == tile.j;
-            const int b_pieces = same ? 0 : tile.groups, pieces = kPlanes * (2 + b_pieces);
-            // this lane's copy: operand, plane, piece
-            const bool is_a = lane < 2 * kPlanes;
-            const int at = is_a ? lane : lane - 2 * kPlanes, per = is_a ? 2 : max(1, b_pieces);
-            const int plane = at / per, piece = at % per;
-            const uint32_t dst = (is_a ? plane * kHalf : kPlanes * kHalf + plane * b_bytes) + piece * kPiece;
-            const uint32_t buffer = symmetric_first(w, kWide ? P.left : is_a ? P.job[tile.job].left : P.job[tile.job].right);
-            const uint32_t x = w.x[P.from];
-            for (int q = 0; q < tile.slices + tile.extra; ++q) {
-                if (!__all_sync(0xffffffffu, nml::mbar_wait(nml::smem_u32(&empty_bar[s]), parity ^ 1, abort_flag, P.err, nml::ERR_WAIT_EMPTY))) {
+        int round = 0;
+        int next_first = tiles ? load_global(&rounds[min(1, P.rounds - 1)].first) : 0;
+        while (ok) {
+            // (not before the last tile's copies are issued: a block that held a second tile of a product would make that product twice as long)
+            int t = 0;
+            if (lane == 0) t = claim(P.c.done);
+            t = __shfl_sync(0xffffffffu, t, 0);
+            Tile tile;
+            tile.k = -1;
+            if (t < tiles) {
+                while (round + 1 < P.rounds && t >= next_first) {
+                    ++round;
+                    next_first = load_global(&rounds[min(round + 1, P.rounds - 1)].first);
+                }
+                t -= load_global(&rounds[round].first);
+                const int of_first = load_global(&rounds[round].of_first), cls = t >= of_first;
+                if (cls) t -= of_first;
+                const int* const words = reinterpret_cast<const int*>(&rounds[round].op[cls]);
+                const int word = lane < kOpWords ? load_global(words + lane) : 0;
+                const int kind = __shfl_sync(0xffffffffu, word, offsetof(Op, kind) / 4), jobs = __shfl_sync(0xffffffffu, word, offsetof(Op, jobs) / 4);
+                const int gram = __shfl_sync(0xffffffffu, word, offsetof(Op, gram) / 4);
+                const bool is_wide = kind >= ITERATE;
+                // (matrices of the first class come first, and their tiles count from 0; those of the second behind all of the first)
+                const int n0 = P.first_class;
+                const int lo = cls ? n0 : 0, hi = cls ? count : n0;
+                const int* const first = is_wide ? first_update : first_gram;
+                const int base = first[lo], per_job = is_wide ? 1 : jobs;
+                int a = lo, b = hi - 1;
+                while (a < b) {
+                    const int mid = (a + b + 1) / 2;
+                    if ((first[mid] - base) * per_job <= t) a = mid; else b = mid - 1;
+                }
+                tile.k = a;
+                t -= (first[a] - base) * per_job;
+                Info w;
+                {
+                    const Work* const from = P.c.table + a;
+                    auto word = [](const uint32_t* p) { return static_cast<uint32_t>(load_global(reinterpret_cast<const int*>(p))); };
+                    w = {load_global(&from->s.m), load_global(&from->s.n), load_global(&from->nb), load_global(&from->wide),
+                         {word(&from->x[0]), word(&from->x[1])}, word(&from->sym), load_global(&from->sx)};
+                }
+                const int mb = (w.m + kBlock - 1) / kBlock;
+                tile.extra = tile.job = 0;
+                if (is_wide) {
+                    const int per = (w.nb + w.wide - 1) / w.wide;
+                    tile.i = t / per;
+                    tile.j = t % per * w.wide;
+                    tile.groups = min(2 * w.wide, (w.n - tile.j * kBlock + 63) / 64);
+                    tile.slices = (w.m + 63) / 64;
+                    if (kPlanes == 1) tile.extra = min(2, tile.slices - 2 * tile.i);
+                } else {
+                    if (t >= lower(mb, 0)) t -= lower(mb, 0), tile.job = 1;
+                    tile.i = static_cast<int>((sqrtf(8.f * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
+                    while (lower(tile.i, 0) > t) --tile.i;
+                    while (lower(tile.i + 1, 0) <= t) ++tile.i;
+                    tile.j = t - lower(tile.i, 0);
+                    tile.groups = min(2, (w.m - tile.j * kBlock + 63) / 64);
+                    tile.slices = ((gram ? w.n : w.m) + 63) / 64;
+                }
+                // pass it on
+                if (!wait(&qempty_bar[slot], qparity ^ 1, nml::ERR_WAIT_EMPTY)) {
                     ok = false;
                     break;
                 }
-                const uint32_t bar = nml::smem_u32(&full_bar[s]), to = nml::smem_u32(smem) + s * stage_bytes + dst;
-                if (lane == 0) nml::mbar_arrive_expect_tx(bar, pieces * kPiece);
-                __syncwarp();
-                if (lane < pieces) {
-                    const bool low = q >= tile.slices;  // a I times X's low half
-                    const int kq = low ? 2 * tile.i + q - tile.slices : q, kb = kq >> 1, h = kq & 1;
-                    const uint8_t* from;
-                    const uint32_t straight = (h * 2 + piece) * kPiece, across = (piece * 2 + h) * kPiece;  // K-major; MN-major
-                    auto symmetric = [&](int row) {
-                        return kb <= row ? block_at(P.c.blocks, buffer, lower(row, kb)) + straight : block_at(P.c.blocks, buffer, lower(kb, row)) + across;
-                    };
-                    if (!kWide) {
-                        const int row = is_a ? tile.i : tile.j;
-                        from = P.gram ? block_at(P.c.blocks, x, row * w.nb + kb) + straight : symmetric(row);
-                    } else if (is_a) {
-                        from = low ? block_at(P.c.blocks, P.identity, 0) + straight : symmetric(tile.i);
-                    } else {  // X's rows along K: two 64-column groups to a block
-                        from = block_at(P.c.blocks, x, kb * w.nb + tile.j + (piece >> 1)) + (low ? kPlane : 0) + ((piece & 1) * 2 + h) * kPiece;
-                    }
-                    nml::bulk_load(to, from + plane * kPlane, kPiece, bar);
+                if (lane < kOpWords) reinterpret_cast<int*>(&queue[slot].op)[lane] = word;
+                if (lane == 0) {
+                    queue[slot].k = tile.k, queue[slot].i = tile.i, queue[slot].j = tile.j, queue[slot].job = tile.job;
+                    queue[slot].groups = tile.groups, queue[slot].slices = tile.slices, queue[slot].extra = tile.extra;
+                    queue[slot].w = w;
                 }
                 __syncwarp();
-                ++issued;
-                if (++s == P.stages) s = 0, parity ^= 1;
+                if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qfull_bar[slot]));
+                const Op& op = queue[slot].op;  // (the producer's own copy stays until it comes round to the slot again)
+                if (++slot == kQueue) slot = 0, qparity ^= 1;
+
+                // the matrix's earlier products
+                const int tiles_gram = lower(mb, 0), tiles_update = mb * ((w.nb + w.wide - 1) / w.wide);
+                const int need = kEpilogueWarps * (op.symmetric_before * tiles_gram + op.wide_before * tiles_update);
+                if (need > 0) {
+                    int gave_up = 0;
+                    if (lane == 0) {
+                        const int* const done = P.c.done + 1 + tile.k;
+                        uint64_t t0 = 0;
+                        for (uint32_t it = 1; load_acquire(done) < need; ++it) {
+                            __nanosleep(40);
+                            if ((it & 0xff) != 0) continue;
+                            const uint64_t now = nml::globaltimer_ns();
+                            if (t0 == 0) t0 = now;
+                            if (*abort_flag || now - t0 > *reinterpret_cast<volatile unsigned long long*>(abort_flag + 2)) {
+                                *abort_flag = 1;
+                                atomicCAS(P.err, 0, nml::ERR_WAIT_TILES);
+                                gave_up = 1;
+                                break;
+                            }
+                        }
+                    }
+                    if (__shfl_sync(0xffffffffu, gave_up, 0)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_proxies();
+                }
+
+                // its K slices; a ring of stages of the other size only begins when the last one's are free
+                const uint32_t stage_bytes = is_wide ? kWideStage : kNarrow, b_bytes = is_wide ? 2 * kHalf : kHalf;
+                if (now_stage != stage_bytes) {
+                    for (int e = 0; ok && e < stages; ++e)
+                        if (used >> e & 1) ok = wait(&empty_bar[e], (parity >> e & 1) ^ 1, nml::ERR_WAIT_EMPTY);
+                    if (!ok) break;
+                    used = 0;
+                    s = 0;
+                    now_stage = stage_bytes;
+                    stages = kRing / stage_bytes;
+                }
+                const bool same = gram && tile.i == tile.j;
+                const int b_pieces = same ? 0 : tile.groups, pieces = kPlanes * (2 + b_pieces);
+                const bool is_a = lane < 2 * kPlanes;
+                const int at = is_a ? lane : lane - 2 * kPlanes, per = is_a ? 2 : max(1, b_pieces);
+                const int plane = at / per, piece = at % per;
+                const uint32_t dst = (is_a ? plane * kHalf : kPlanes * kHalf + plane * b_bytes) + piece * kPiece;
+                const uint32_t buffer = symmetric_first(w, is_wide ? op.left : is_a ? op.job[tile.job].left : op.job[tile.job].right);
+                const uint32_t x = op.from ? w.x[1] : w.x[0];
+                for (int q = 0; q < tile.slices + tile.extra; ++q) {
+                    if (used >> s & 1) {
+                        if (!wait(&empty_bar[s], (parity >> s & 1) ^ 1, nml::ERR_WAIT_EMPTY)) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                    const uint32_t bar = nml::smem_u32(&full_bar[s]), to = nml::smem_u32(smem) + s * stage_bytes + dst;
+                    if (lane == 0) nml::mbar_arrive_expect_tx(bar, pieces * kPiece);
+                    __syncwarp();
+                    if (lane < pieces) {
+                        const bool low = q >= tile.slices;  // a I times X's low half
+                        const int kq = low ? 2 * tile.i + q - tile.slices : q, kb = kq >> 1, h = kq & 1;
+                        const uint8_t* from;
+                        const uint32_t straight = (h * 2 + piece) * kPiece, across = (piece * 2 + h) * kPiece;  // K-major; MN-major
+                        auto symmetric = [&](int row) {
+                            return kb <= row ? block_at(P.c.blocks, buffer, lower(row, kb)) + straight : block_at(P.c.blocks, buffer, lower(kb, row)) + across;
+                        };
+                        if (!is_wide) {
+                            const int row = is_a ? tile.i : tile.j;
+                            from = gram ? block_at(P.c.blocks, x, row * w.nb + kb) + straight : symmetric(row);
+                        } else if (is_a) {
+                            from = low ? block_at(P.c.blocks, op.identity, 0) + straight : symmetric(tile.i);
+                        } else {  // X's rows along K: two 64-column groups to a block
+                            from = block_at(P.c.blocks, x, kb * w.nb + tile.j + (piece >> 1)) + (low ? kPlane : 0) + ((piece & 1) * 2 + h) * kPiece;
+                        }
+                        nml::bulk_load(to, from + plane * kPlane, kPiece, bar);
+                    }
+                    __syncwarp();
+                    used |= 1u << s;
+                    parity ^= 1u << s;
+                    if (++s == stages) s = 0;
+                }
+            } else {
+                if (!wait(&qempty_bar[slot], qparity ^ 1, nml::ERR_WAIT_EMPTY)) ok = false;
+                if (ok && lane == 0) {
+                    queue[slot].k = -1;
+                    nml::mbar_arrive(nml::smem_u32(&qfull_bar[slot]));
+                }
+                break;
             }
         }
         if (!ok || *abort_flag) {  // no copy may be in flight when the block's shared memory goes away
-            for (int back = min(issued, P.stages); back > 0; --back) {
-                if (--s < 0) s = P.stages - 1, parity ^= 1;
+            for (int e = 0; e < stages; ++e) {
+                if (!(used >> e & 1)) continue;
                 const uint64_t t0 = nml::globaltimer_ns();
-                while (!nml::mbar_try_wait(nml::smem_u32(&full_bar[s]), parity)) {
+                while (!nml::mbar_try_wait(nml::smem_u32(&full_bar[e]), (parity >> e & 1) ^ 1)) {
                     if (nml::globaltimer_ns() - t0 > 2000000ull) {
                         if (lane == 0) atomicCAS(P.err, 0, nml::ERR_WAIT_DRAIN);
                         break;
@@ -536,49 +774,64 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA
-        int s = 0, buf = 0;
-        uint32_t parity = 0, tparity = 0;
+        int slot = 0, s = 0, stages = 0, buf = 0;
+        uint32_t qparity = 0, parity = 0, tparity = 0, now_stage = 0;
         bool ok = true;
         const uint32_t ring = nml::smem_u32(smem);
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-            const Tile tile = tile_of(t);
-            const bool same = P.gram && tile.i == tile.j;
-            const int slices = tile.slices + tile.extra;
+        while (ok) {
+            if (!wait(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL)) {
+                ok = false;
+                break;
+            }
+            const int k = queue[slot].k, row = queue[slot].i, column = queue[slot].j, groups = queue[slot].groups, real = queue[slot].slices;
+            const int slices = real + queue[slot].extra;
+            const bool is_wide = queue[slot].op.kind >= ITERATE, gram = queue[slot].op.gram != 0;
+            if (k < 0) break;
+            __syncwarp();
+            if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qempty_bar[slot]));
+            if (++slot == kQueue) slot = 0, qparity ^= 1;
+            const uint32_t stage_bytes = is_wide ? kWideStage : kNarrow, b_bytes = is_wide ? 2 * kHalf : kHalf;
+            if (now_stage != stage_bytes) {
+                s = 0;
+                now_stage = stage_bytes;
+                stages = kRing / stage_bytes;
+            }
+            const bool same = gram && row == column;
             for (int q = 0; q < slices; ++q) {
                 if (kPlanes == 2 || q == 0) {
-                    if (!__all_sync(0xffffffffu, nml::mbar_wait(nml::smem_u32(&tempty_bar[buf]), tparity ^ 1, abort_flag, P.err, nml::ERR_WAIT_TMEM_EMPTY))) {
+                    if (!wait(&tempty_bar[buf], tparity ^ 1, nml::ERR_WAIT_TMEM_EMPTY)) {
                         ok = false;
                         break;
                     }
                     nml::tc_fence_after();
                 }
-                if (!__all_sync(0xffffffffu, nml::mbar_wait(nml::smem_u32(&full_bar[s]), parity, abort_flag, P.err, nml::ERR_WAIT_FULL))) {
+                if (!wait(&full_bar[s], parity >> s & 1, nml::ERR_WAIT_FULL)) {
                     ok = false;
                     break;
                 }
                 nml::tc_fence_after();
-                const bool low = q >= tile.slices, last = kPlanes == 2 || q + 1 == slices;
+                const bool low = q >= real, last = kPlanes == 2 || q + 1 == slices;
                 const int kb = q >> 1;
-                const int a_mn = !P.gram && !low && kb > tile.i;
-                const int b_mn = kWide ? 1 : !P.gram && kb > tile.j;
-                const uint32_t idesc = nml::make_instr_desc(0, a_mn, b_mn, 128, tile.groups * 64);
+                const int a_mn = !gram && !low && kb > row;
+                const int b_mn = is_wide ? 1 : !gram && kb > column;
+                const uint32_t idesc = nml::make_instr_desc(0, a_mn, b_mn, 128, groups * 64);
                 const uint32_t sa = ring + s * stage_bytes, sb = same ? sa : sa + kPlanes * kHalf, bp = same ? kHalf : b_bytes;
                 if (nml::elect_one()) {
+                    const uint64_t a0 = nml::make_smem_desc(sa, kPiece, 1024, 2), b0 = nml::make_smem_desc(sb, kPiece, 1024, 2);
+                    const uint32_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
 #pragma unroll
                     for (int p = kPlanes == 2 ? 2 : 0; p >= 0; --p) {  // low x high, high x low, high x high
-                        const uint32_t pa = p == 2, pb = p == 1;
+                        uint64_t ad = a0 + (p == 2 ? kHalf >> 4 : 0), bd = b0 + (p == 1 ? bp >> 4 : 0);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint64_t ad = nml::make_smem_desc(sa + pa * kHalf + k * (a_mn ? 2048 : 32), kPiece, 1024, 2);
-                            const uint64_t bd = nml::make_smem_desc(sb + pb * bp + k * (b_mn ? 2048 : 32), kPiece, 1024, 2);
-                            nml::umma_f16(tmem + buf * 256, ad, bd, idesc, kPlanes == 2 ? k > 0 || p < 2 : k > 0 || q > 0);
-                        }
+                        for (int e = 0; e < 4; ++e, ad += a_step, bd += b_step)
+                            nml::umma_f16(tmem + buf * 256, ad, bd, idesc, kPlanes == 2 ? e > 0 || p < 2 : e > 0 || q > 0);
                     }
                     nml::umma_commit(nml::smem_u32(&empty_bar[s]));
                     if (last) nml::umma_commit(nml::smem_u32(&tfull_bar[buf]));
                 }
                 __syncwarp();
-                if (++s == P.stages) s = 0, parity ^= 1;
+                parity ^= 1u << s;
+                if (++s == stages) s = 0;
                 if (last && ++buf == 2) buf = 0, tparity ^= 1;
             }
         }
@@ -593,38 +846,59 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 }
             }
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         // ------------------------------------------------------------ epilogue: a thread to a row and half of the columns of the tile
-        constexpr int kGroups16 = kWide ? 8 : 4;  // of sixteen columns, to a thread
-        int buf = 0;
-        uint32_t tparity = 0;
-        const int quarter = warp & 3, row = quarter * 32 + lane, side = (warp - 2) >> 2;
-        bool ok = true;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-            const Tile tile = tile_of(t);
-            const Info w = info[tile.k];
-            const int g0 = side * (tile.groups * 2);  // this thread's first sixteen columns; as many for the other side
-            const int chunks = kPlanes == 2 ? tile.slices : 1, mine = tile.groups * 2;
-            float acc[kGroups16][16];
+        int slot = 0, buf = 0, pending = -1;  // pending: matrix of a tile that is stored but not reported
+        uint32_t qparity = 0, tparity = 0;
+        const int quarter = warp & 3, row = quarter * 32 + lane, side = (warp - 4) >> 2;
+        uint8_t* const staging = smem + kRing + (warp - 4) * kStaging;
+        // A tile is reported when its stores are visible, which takes a while: where the next one is there already, its first slice comes first.
+        auto report = [&]() {
+            if (pending >= 0) {
+                fence_proxies();
+                __syncwarp();
+                if (lane == 0) add_release(P.c.done + 1 + pending, 1);
+                pending = -1;
+            }
+        };
+        while (true) {
+            if (!__all_sync(0xffffffffu, nml::mbar_test(nml::smem_u32(&qfull_bar[slot]), qparity))) report();
+            if (!wait(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL)) break;
+            const int k = queue[slot].k, tile_i = queue[slot].i, tile_j = queue[slot].j, groups = queue[slot].groups, slices = queue[slot].slices;
+            const int kind = queue[slot].op.kind, gram = queue[slot].op.gram, from_x = queue[slot].op.from;
+            const Symmetric job = queue[slot].op.job[queue[slot].job];
+            const float op_f1 = queue[slot].op.f1, op_d1 = queue[slot].op.d1;
+            const Info w = queue[slot].w;
+            if (k < 0) break;
+            __syncwarp();
+            if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qempty_bar[slot]));
+            if (++slot == kQueue) slot = 0, qparity ^= 1;
+            const int mine = groups * 2, g0 = side * mine;  // this thread's columns in sixteens; the first
+            const int chunks = kPlanes == 2 ? slices : 1;
+            float acc[8][16];
 #pragma unroll
-            for (int c = 0; c < kGroups16; ++c)
+            for (int c = 0; c < 8; ++c)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[c][e] = 0.f;
+            bool ok = true;
             for (int q = 0; q < chunks; ++q) {
-                if (!__all_sync(0xffffffffu, nml::mbar_wait(nml::smem_u32(&tfull_bar[buf]), tparity, abort_flag, P.err, nml::ERR_WAIT_TMEM_FULL))) {
+                if (q == 0 && !__all_sync(0xffffffffu, nml::mbar_test(nml::smem_u32(&tfull_bar[buf]), tparity))) report();
+                if (!wait(&tfull_bar[buf], tparity, nml::ERR_WAIT_TMEM_FULL)) {
                     ok = false;
                     break;
                 }
                 nml::tc_fence_after();
                 const uint32_t from = tmem + buf * 256 + g0 * 16 + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
-                for (int c = 0; c < kGroups16; ++c) {
+                for (int c = 0; c < 8; c += 2) {
                     if (c < mine) {
-                        uint32_t r[16];
-                        nml::tmem_ld_32x16(from + c * 16, r);
+                        uint32_t r[32];
+                        nml::tmem_ld_32x32(from + c * 16, r);
                         nml::tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[c][e] += __uint_as_float(r[e]);
+                        for (int e = 0; e < 32; ++e) acc[c + e / 16][e % 16] += __uint_as_float(r[e]);
                     }
                 }
                 nml::tc_fence_before();
@@ -633,57 +907,91 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 if (++buf == 2) buf = 0, tparity ^= 1;
             }
             if (!ok) break;
-            const int i = tile.i * kBlock + row;
-            if (kKind == RESULT) {
-                const Source* src = &P.c.table[tile.k].s;
-                const int m = w.m, j0 = tile.j * kBlock + g0 * 16;
-                const long long step = load_wide(&src->out_j), at = i * load_wide(&src->out_i) + j0 * step;
+            report();
+            if (kind == RESULT) {
+                const Source* src = &P.c.table[k].s;
+                const long long out_i = load_wide(&src->out_i), out_j = load_wide(&src->out_j);
                 uint8_t* const out = reinterpret_cast<uint8_t*>(load_wide(reinterpret_cast<const long long*>(&src->out)));
                 uint8_t* const half = reinterpret_cast<uint8_t*>(load_wide(reinterpret_cast<const long long*>(&src->half)));
-                const float f0 = P.f0 / w.sx, rate = P.rate * load_global(&src->scale);  // (a power of two)
-                const int in_row = i < m ? min(mine * 16, w.n - j0) : 0;  // this thread's elements
+                const float f0 = op_f1 / w.sx, rate = P.rate * load_global(&src->scale);  // (a power of two)
+                const int i0 = tile_i * kBlock + quarter * 32, j0 = tile_j * kBlock + g0 * 16;
+                // Thirty-two columns at a time go through shared memory: where rows lie densely, eight lanes write a row's 128 bytes; else the lanes
+                // of a warp lie beside one another along a column.
 #pragma unroll
-                for (int c = 0; c < kGroups16; ++c) {
-                    if (c * 16 >= in_row) continue;
-                    float v[16];
+                for (int c = 0; c < 8; c += 2) {
+                    if (c < mine) {
+                        __syncwarp();
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) v[q] = acc[c][q] * f0;
-                    const long long e = at + c * 16 * step;
-                    const int count = in_row - c * 16;
-                    if (P.apply) apply16(reinterpret_cast<float*>(out) + e, half ? reinterpret_cast<__half*>(half) + e : nullptr, step, count, v, P.keep, rate);
-                    else if (P.out_half) write16(reinterpret_cast<__half*>(out) + e, step, count, v);
-                    else write16(reinterpret_cast<float*>(out) + e, step, count, v);
+                        for (int q = 0; q < 8; ++q)
+                            *reinterpret_cast<float4*>(staging + swizzled(lane, q)) =
+                                make_float4(acc[c + q / 4][q % 4 * 4] * f0, acc[c + q / 4][q % 4 * 4 + 1] * f0, acc[c + q / 4][q % 4 * 4 + 2] * f0,
+                                            acc[c + q / 4][q % 4 * 4 + 3] * f0);
+                        __syncwarp();
+                        write_columns(P, staging, out, half, rate, out_i, out_j, i0, w.m, j0 + c * 16, w.n);
+                    }
                 }
             } else {
-                const Symmetric& job = P.job[tile.job];
-                const uint32_t to = kKind == ITERATE ? w.x[P.from ^ 1] : symmetric_first(w, job.out), poly = symmetric_first(w, kPoly);
-                const int block = kKind == ITERATE ? tile.i * w.nb + tile.j : lower(tile.i, tile.j);
-                const float over = P.gram ? 1.f / (w.sx * w.sx) : 1.f;  // (a power of two)
-                const float f0 = (kKind == ITERATE ? P.f0 : job.f0) * over, f1 = P.f1 * over;
-                const int diagonal = kKind != ITERATE && tile.i == tile.j ? row - g0 * 16 : -1;  // column of the diagonal, among this thread's
+                const bool iterate = kind == ITERATE;
+                const uint32_t to = iterate ? (from_x ? w.x[0] : w.x[1]) : symmetric_first(w, job.out);
+                const int block = iterate ? tile_i * w.nb + tile_j : lower(tile_i, tile_j);
+                const float over = gram ? 1.f / (w.sx * w.sx) : 1.f;  // (a power of two)
+                // Thirty-two columns of both planes at a time go through shared memory, so that four lanes write 64 contiguous bytes of a row (a thread's
+                // own 32 bytes, in 32 lines a store, took 1.1 us a matrix and tile; bulk copies of 4 KB out of shared memory, whose room
+                // has to be waited for, 3).
+                auto store = [&](uint32_t base, bool low) {
 #pragma unroll
-                for (int c = 0; c < kGroups16; ++c) {
-                    if (c >= mine) continue;
-                    const int g = g0 + c, half = g >> 2, at16 = (g & 3) * 2;
-                    float v[16];
+                    for (int c = 0; c < 8; c += 2) {
+                        if (c < mine) {
+                            const int half = (g0 + c) >> 2, part = (g0 + c) >> 1 & 1;
+                            uint8_t* const at = block_at(P.c.blocks, base, block + (half >> 1)) + (half & 1) * kHalf + quarter * 4096;
+                            __syncwarp();
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        v[q] = acc[c][q] * f0;
-                        if (kKind == PLAIN && c * 16 + q == diagonal) v[q] += job.d1;
-                    }
-                    uint8_t* const at = block_at(P.c.blocks, to, block + (half >> 1)) + (half & 1) * kHalf;
-                    store16<kKind == ITERATE || kPlanes == 2>(at, row, at16, v);
-                    if (kKind == POLY) {
+                            for (int q = 0; q < 4; ++q) {
+                                uint4 h, l;
+                                split8(&acc[c + q / 2][q % 2 * 8], h, l);
+                                uint8_t* const mine_at = staging + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4);
+                                *reinterpret_cast<uint4*>(mine_at) = h;
+                                if (low) *reinterpret_cast<uint4*>(mine_at + 2048) = l;
+                            }
+                            __syncwarp();
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            v[q] = acc[c][q] * f1;
-                            if (c * 16 + q == diagonal) v[q] += P.d1;
+                            for (int e = 0; e < 4; ++e) {
+                                const int r = e * 8 + (lane >> 2), q = lane & 3;
+                                const uint8_t* const from = staging + r * 64 + ((q ^ (r >> 1 & 3)) << 4);
+                                uint8_t* const out = at + swizzled(r, part * 4 + q);
+                                *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from);
+                                if (low) *reinterpret_cast<uint4*>(out + kPlane) = *reinterpret_cast<const uint4*>(from + 2048);
+                            }
                         }
-                        store16<kPlanes == 2>(block_at(P.c.blocks, poly, block) + half * kHalf, row, at16, v);
                     }
+                };
+                auto scale = [&](float f) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[c][e] *= f;
+                };
+                auto add_diagonal = [&](float d) {  // (symmetric tiles: at most 64 columns to a thread)
+                    if (tile_i == tile_j)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) acc[c][e] += c * 16 + e == row - g0 * 16 ? d : 0.f;
+                };
+                // (of a last block of 64 rows or fewer, half is never read: K slices and columns end at a multiple of 64, and what the other rows of an
+                // operand hold, which may be anything, ends in rows and columns that are not stored either)
+                const bool in_use = tile_i * kBlock + (quarter & 2) * 32 < w.m;
+                const int matrices = in_use ? kind == POLY ? 2 : 1 : 0;
+#pragma unroll 1
+                for (int e = 0; e < matrices; ++e) {  // (A and P: f0 is a power of two)
+                    scale(e ? op_f1 / job.f0 : (iterate ? op_f1 : job.f0) * over);
+                    if (e || kind == PLAIN) add_diagonal(e ? op_d1 : job.d1);
+                    store(e ? symmetric_first(w, kPoly) : to, iterate || kPlanes == 2);
                 }
+                pending = k;
             }
         }
+        report();
     }
     nml::tc_fence_before();
     __syncthreads();
@@ -744,13 +1052,12 @@ struct Step {
 struct Polynomial {
     Step step[kMaxSteps];
     int steps = 0;
-    bool chained = false;
     double largest = 1.0;    // singular value at the chains' starts, hence element of X
 };
 static int exponent_below(double bound) {  // largest e with bound * 2^e <= 2^15
     return std::max(-24, std::min(24, static_cast<int>(floor(log2(32768.0 / std::max(bound, 1e-6))))));
 }
-static bool polynomial(const float* coefficients, int steps, int math, Polynomial* p) {
+static bool polynomial(const float* coefficients, int steps, bool chained, Polynomial* p) {
     constexpr int kPoints = 128;        // singular values, at which the matrices' eigenvalues are followed
     constexpr double kBetween = 1.01;   // and what lies between two of them
     double l = kBetween, lambda[kPoints + 1], q[kPoints + 1], growth = 1.0;
@@ -787,62 +1094,128 @@ static bool polynomial(const float* coefficients, int steps, int math, Polynomia
         s.eq = exponent_below(mq * kBetween);
         growth *= std::max(1.0, mu * mu);
         if (!(next <= 4096.0)) return false;  // singular values beyond 64
-        s.ends = math == NML_MATH_F16 || k == steps - 1 || growth > kGrowth;
+        s.ends = !chained || k == steps - 1 || growth > kGrowth;
         starts = s.ends;
-        if (!s.ends) p->chained = true;
         if (s.ends) l = std::max(sqrt(next) * kBetween, 1e-3), p->largest = std::max(p->largest, l);
     }
     return true;
 }
 
+// Which matrices are chained: where the long side is so much longer that products of m x m matrices are the cheaper ones, and m is so large that
+// the rounding errors, which are random, add to little in any one direction (relative to fp32 products, errors were 2.0 at m = 256, 7 at 64).  1024 x
+// 4096 510 us instead of 652, 256 x 1024 211 / 229, 1024 x 1024 385 / 347, 128 x 512 170 / 176.
+static bool chained(const Source& s, int math) { return math == NML_MATH_3XF16 && s.m >= 256 && 2ll * s.n >= 3ll * s.m; }
+
 struct Plan {
-    int sums = 0, halves = 0, gram_tiles = 0, update_tiles = 0;
+    int sums = 0, halves = 0, first_class = 0;
+    int gram_tiles[kClasses] = {0, 0}, update_tiles[kClasses] = {0, 0};
     uint32_t blocks = 0, identity = 0;
-    size_t table_at = 0, sums_at = 0, blocks_at = 0, bytes = 0;
+    size_t sums_at = 0, rounds_at = 0, done_at = 0, blocks_at = 0, bytes = 0;
 };
-// Lays a group of at most kGroup matrices out; the sources' sizes are set.
-static Plan plan_group(Work* w, int count, int math, const Polynomial& poly, int sms) {
+// Lays a group of at most kGroup matrices out, chained ones first, longer ones first; the sources are set.
+static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
     Plan p;
     long long wide_tiles = 0;
     for (int k = 0; k < count; ++k) {
+        w[k].chained = steps > 1 && chained(w[k].s, math);
         w[k].mb = (w[k].s.m + kBlock - 1) / kBlock;
         w[k].nb = (w[k].s.n + kBlock - 1) / kBlock;
         wide_tiles += static_cast<long long>(w[k].mb) * ((w[k].nb + 1) / 2);
     }
+    std::sort(w, w + count, [](const Work& a, const Work& b) {
+        if (a.chained != b.chained) return a.chained > b.chained;
+        if (a.s.m != b.s.m) return a.s.m > b.s.m;
+        return a.s.n != b.s.n ? a.s.n > b.s.n : a.s.in < b.s.in;
+    });
+    int gram = 0, update = 0;
     for (int k = 0; k < count; ++k) {
         Work& v = w[k];
-        const long long elements = static_cast<long long>(v.s.m) * v.s.n;
+        const int c = v.chained ? 0 : 1, tiles = v.mb * (v.mb + 1) / 2;
+        if (v.chained) p.first_class = k + 1;
         v.first_sum = p.sums;
-        v.sums = static_cast<int>((elements + kSumElements - 1) / kSumElements);
+        v.sums = static_cast<int>((static_cast<long long>(v.s.m) * v.s.n + kSumElements - 1) / kSumElements);
         p.sums += v.sums;
         v.first_half = p.halves;
         p.halves += v.mb * v.nb * 2;
-        v.first_gram = p.gram_tiles;
-        p.gram_tiles += v.mb * (v.mb + 1) / 2;
+        v.first_gram = gram;
+        gram += tiles;
+        p.gram_tiles[c] += tiles;
         v.wide = wide_tiles >= sms ? 2 : 1;
-        v.first_update = p.update_tiles;
-        p.update_tiles += v.mb * ((v.nb + v.wide - 1) / v.wide);
+        v.first_update = update;
+        const int updates = v.mb * ((v.nb + v.wide - 1) / v.wide);
+        update += updates;
+        p.update_tiles[c] += updates;
         for (uint32_t* at : {&v.x[0], &v.x[1]}) *at = p.blocks, p.blocks += v.mb * v.nb;
         v.sym = p.blocks;
-        p.blocks += (poly.chained ? 7 : 3) * (v.mb * (v.mb + 1) / 2);
-        const int e = std::min(exponent_below(poly.largest), static_cast<int>(lround(0.5 * log2(static_cast<double>(elements)))));
-        v.sx = static_cast<float>(ldexp(1.0, e));
+        p.blocks += (v.chained ? 7 : 3) * tiles;
     }
     p.identity = p.blocks;
-    if (math == NML_MATH_F16) p.blocks += poly.steps;
+    if (math == NML_MATH_F16) p.blocks += steps;
     p.sums_at = round_up(sizeof(Work) * kGroup, 256);
-    p.blocks_at = p.sums_at + round_up(sizeof(double) * p.sums, 1024);
+    p.rounds_at = p.sums_at + round_up(sizeof(double) * p.sums, 256);
+    p.done_at = p.rounds_at + round_up(sizeof(Round) * kMaxRounds, 256);
+    p.blocks_at = p.done_at + round_up(sizeof(int) * (kGroup + 1), 1024);
+    p.blocks_at = round_up(p.blocks_at, 1024);
     p.bytes = p.blocks_at + static_cast<size_t>(p.blocks) * 2 * kPlane;
     return p;
 }
 
-typedef void (*ProductKernel)(const ProductParams);
-static ProductKernel product_kernel(int planes, int kind) {
-    if (planes == 1)
-        return kind == POLY ? ortho_product_kernel<1, POLY> : kind == PLAIN ? ortho_product_kernel<1, PLAIN>
-               : kind == ITERATE ? ortho_product_kernel<1, ITERATE> : ortho_product_kernel<1, RESULT>;
-    return kind == POLY ? ortho_product_kernel<2, POLY> : kind == PLAIN ? ortho_product_kernel<2, PLAIN>
-           : kind == ITERATE ? ortho_product_kernel<2, ITERATE> : ortho_product_kernel<2, RESULT>;
+// The products of a class, in order; their number.
+static int build_ops(const Polynomial& poly, uint32_t identity, Op* ops) {
+    int n = 0, from = 0, symmetric_before = 0, wide_before = 0;
+    auto add = [&](Op op) {
+        op.jobs = std::max(op.jobs, 1);
+        op.symmetric_before = symmetric_before;
+        op.wide_before = wide_before;
+        if (op.kind >= ITERATE) ++wide_before; else symmetric_before += op.jobs;
+        ops[n++] = op;
+    };
+    // a product of two symmetric matrices stored times 2^el and 2^er, to be stored times 2^eo, + d on the diagonal
+    auto symmetric = [](int left, int el, int right, int er, int out, int eo, double d) {
+        return Symmetric{left, right, out, static_cast<float>(ldexp(1.0, eo - el - er)), static_cast<float>(ldexp(d, eo))};
+    };
+    int u = kUpdate, q = kQ;   // the current U and Q
+    int eu_last = 0, eq = 0;   // exponents of the last step's U and of Q
+    for (int k = 0; k < poly.steps; ++k) {
+        const Step& s = poly.step[k];
+        Op a = {};             // A and P
+        a.kind = POLY;
+        a.gram = s.starts;
+        a.from = from;
+        if (s.starts) a.job[0] = {0, 0, kGram, static_cast<float>(ldexp(1.0, s.ea)), 0.f};
+        else a.job[0] = symmetric(u, eu_last, kT, poly.step[k - 1].et, kGram, s.ea, 0.0);
+        a.f1 = static_cast<float>(ldexp(s.c, s.ep - (s.starts ? 0 : eu_last + poly.step[k - 1].et)));
+        a.d1 = static_cast<float>(ldexp(s.b, s.ep));
+        add(a);
+        u = s.starts || u != kUpdate ? kUpdate : kUpdate2;
+        if (s.starts) q = u, eq = s.eu;
+        Op b = {};             // U
+        b.kind = PLAIN;
+        b.job[0] = symmetric(kPoly, s.ep, kGram, s.ea, u, s.eu, s.a);
+        add(b);
+        Op c = {};             // T = U A where the chain goes on, and Q = U Q
+        c.kind = PLAIN;
+        if (!s.ends) c.job[c.jobs++] = symmetric(u, s.eu, kGram, s.ea, kT, s.et, 0.0);
+        if (!s.starts) {
+            const int to = q == kQ ? kQ2 : kQ;
+            c.job[c.jobs++] = symmetric(u, s.eu, q, eq, to, s.eq, 0.0);
+            q = to;
+            eq = s.eq;
+        }
+        if (c.jobs) add(c);
+        eu_last = s.eu;
+        if (s.ends) {
+            Op x = {};
+            x.kind = k == poly.steps - 1 ? RESULT : ITERATE;
+            x.from = from;
+            x.left = q;
+            x.f1 = static_cast<float>(ldexp(1.0, -eq));
+            x.identity = identity + k;
+            add(x);
+            from ^= 1;
+        }
+    }
+    return n;
 }
 
 struct Call {
@@ -855,105 +1228,96 @@ struct Call {
 };
 
 template <int N>
-static void launch_sums(const Work* w, int count, const Call& call, const Plan& p, Work* table, double* sums, cudaStream_t st) {
+static void launch_sums(const Work* w, const Common& c, const Call& call, int blocks, cudaStream_t st) {
     Group<N> g;
-    std::copy(w, w + count, g.w);
-    if (call.in_dtype == NML_F16)
-        nml::launch(ortho_sums_kernel<N, __half>, p.sums, 256, 0, st, g, count, call.mo, table, sums, call.skip);
-    else
-        nml::launch(ortho_sums_kernel<N, float>, p.sums, 256, 0, st, g, count, call.mo, table, sums, call.skip);
+    std::copy(w, w + c.count, g.w);
+    nml::launch(call.in_dtype == NML_F16 ? ortho_sums_kernel<N, __half> : ortho_sums_kernel<N, float>, blocks, 256, 0, st, g, c, call.mo);
+}
+// `rounds` of them are set; the others' room does not travel where they are few.
+template <int N>
+static void launch_pack(const PackParams<kMaxRounds>& all, const Call& call, int blocks, cudaStream_t st) {
+    PackParams<N> q = {all.c, all.mo, all.eps, all.halves, all.rounds, all.identity, all.identities, {}, {}};
+    std::copy(all.diagonal, all.diagonal + kMaxSteps, q.diagonal);
+    std::copy(all.round, all.round + std::min(N, all.rounds), q.round);
+    nml::launch(call.in_dtype == NML_F16 ? ortho_pack_kernel<N, __half> : ortho_pack_kernel<N, float>, blocks, 256, 0, st, q);
+}
+constexpr int kFewRounds = 20;
+
+// The polynomials of the two classes.
+struct Steps {
+    Polynomial of[kClasses];
+};
+static bool steps_of(const float* coefficients, int steps, Steps* s) {
+    return polynomial(coefficients, steps, true, &s->of[0]) && polynomial(coefficients, steps, false, &s->of[1]);
 }
 
-// One group: the launches of all its steps.
-static int run_group(Work* w, int count, const Call& call, const Polynomial& poly, void* workspace, size_t bytes, cudaStream_t st) {
+// One group: three launches.
+static int run_group(Work* w, int count, const Call& call, const Steps& steps, void* workspace, size_t bytes, cudaStream_t st) {
     int* err;
     int sms;
     if (const int rc = nml::current_device(&err, &sms)) return rc;
-    const Plan p = plan_group(w, count, call.math, poly, sms);
+    const Plan p = plan_group(w, count, call.math, steps.of[0].steps, sms);
     uint8_t* const base = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<uintptr_t>(workspace), 1024));
     if (!workspace || base + p.bytes > static_cast<uint8_t*>(workspace) + bytes) return NML_ERR_WORKSPACE;
-    Work* const table = reinterpret_cast<Work*>(base);
-    double* const sums = reinterpret_cast<double*>(base + p.sums_at);
-    if (count <= 8) launch_sums<8>(w, count, call, p, table, sums, st);
-    else launch_sums<kGroup>(w, count, call, p, table, sums, st);
-    const Common common = {table, sums, base + p.blocks_at, call.skip, count};
-    PackParams pack = {common, call.mo, call.eps, p.halves, p.identity, {}};
-    for (int k = 0; k < poly.steps; ++k) pack.diagonal[k] = static_cast<float>(ldexp(poly.step[k].a, poly.step[k].eu));
-    const int pack_grid = p.halves + (call.math == NML_MATH_F16 ? 2 * poly.steps : 0);
-    nml::launch(call.in_dtype == NML_F16 ? ortho_pack_kernel<__half> : ortho_pack_kernel<float>, pack_grid, 256, 0, st, pack);
-    const int planes = call.math == NML_MATH_F16 ? 1 : 2;
-    int launched = 2, from = 0;
-    auto product = [&](int kind, ProductParams& q) {
-        const bool wide = kind >= ITERATE;
-        q.c = common;
-        q.err = err;
-        q.jobs = std::max(q.jobs, 1);
-        q.tiles = wide ? p.update_tiles : p.gram_tiles * q.jobs;
-        q.stages = std::min<int>(kMaxStages, kStageBytes / (planes * (wide ? 3 * kHalf : 2 * kHalf)));
-        q.from = from;
-        nml::launch(product_kernel(planes, kind), std::min(q.tiles, sms), kThreads, kProductSmem, st, q);
-        ++launched;
-    };
-    // a product of two symmetric matrices stored times 2^el and 2^er, to be stored times 2^eo, + d on the diagonal
-    auto symmetric = [](int left, int el, int right, int er, int out, int eo, double d) {
-        return Symmetric{left, right, out, static_cast<float>(ldexp(1.0, eo - el - er)), static_cast<float>(ldexp(d, eo))};
-    };
-    int u = kUpdate, q_at = kQ;       // the current U and Q
-    int eq = 0, eu_last = 0;          // Q's exponent; that of the last step's U, which is in the other buffer
-    for (int k = 0; k < poly.steps; ++k) {
-        const Step& s = poly.step[k];
-        {   // A and P
-            ProductParams q = {};
-            q.gram = s.starts;
-            if (s.starts) q.job[0].out = kGram, q.job[0].f0 = static_cast<float>(ldexp(1.0, s.ea));
-            else q.job[0] = symmetric(u, eu_last, kT, poly.step[k - 1].et, kGram, s.ea, 0.0);
-            const double f = s.starts ? 1.0 : ldexp(1.0, -eu_last - poly.step[k - 1].et);
-            q.f1 = static_cast<float>(ldexp(s.c * f, s.ep));
-            q.d1 = static_cast<float>(ldexp(s.b, s.ep));
-            product(POLY, q);
-        }
-        {   // U
-            if (!s.starts) u = u == kUpdate ? kUpdate2 : kUpdate;
-            if (s.starts) q_at = u, eq = s.eu;
-            ProductParams q = {};
-            q.job[0] = symmetric(kPoly, s.ep, kGram, s.ea, u, s.eu, s.a);
-            product(PLAIN, q);
-            eu_last = s.eu;
-        }
-        {   // Q = U Q, and T = U A where the chain goes on
-            ProductParams q = {};
-            if (!s.ends) q.job[q.jobs++] = symmetric(u, s.eu, kGram, s.ea, kT, s.et, 0.0);
-            if (!s.starts) {
-                const int to = q_at == kQ ? kQ2 : kQ;
-                q.job[q.jobs++] = symmetric(u, s.eu, q_at, eq, to, s.eq, 0.0);
-                q_at = to;
-                eq = s.eq;
-            }
-            if (q.jobs) product(PLAIN, q);
-        }
-        if (s.ends) {
-            const bool last = k == poly.steps - 1;
-            ProductParams q = {};
-            q.left = q_at;
-            q.f0 = static_cast<float>(ldexp(1.0, -eq));
-            q.identity = p.identity + k;
-            q.out_half = call.out_dtype == NML_F16;
-            q.apply = call.apply;
-            q.keep = call.keep;
-            q.rate = call.rate;
-            product(last ? RESULT : ITERATE, q);
-            from ^= 1;
-        }
+    for (int k = 0; k < count; ++k) {
+        const double elements = static_cast<double>(w[k].s.m) * w[k].s.n;
+        const int e = std::min(exponent_below(steps.of[w[k].chained ? 0 : 1].largest), static_cast<int>(lround(0.5 * log2(elements))));
+        w[k].sx = static_cast<float>(ldexp(1.0, e));
     }
+    const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), reinterpret_cast<Round*>(base + p.rounds_at),
+                      reinterpret_cast<int*>(base + p.done_at), base + p.blocks_at, call.skip, count};
+
+    // rounds: a product of each class, with as many tiles as its matrices have
+    PackParams<kMaxRounds> pack = {c, call.mo, call.eps, p.halves, 0, p.identity, call.math == NML_MATH_F16 ? steps.of[1].steps : 0, {}, {}};
+    Op ops[kClasses][kMaxRounds];
+    int number[kClasses];
+    for (int cls = 0; cls < kClasses; ++cls) number[cls] = build_ops(steps.of[cls], p.identity, ops[cls]);
+    if (p.first_class == 0) number[0] = 0;
+    if (p.first_class == count) number[1] = 0;
+    pack.rounds = std::max(number[0], number[1]);
+    long long tiles = 0, widest = 0;
+    for (int r = 0; r < pack.rounds; ++r) {
+        Round& round = pack.round[r];
+        round.first = static_cast<int>(tiles);
+        round.of_first = 0;
+        for (int cls = 0; cls < kClasses; ++cls) {
+            if (r >= number[cls]) continue;
+            const Op& op = round.op[cls] = ops[cls][r];
+            const long long n = op.kind >= ITERATE ? p.update_tiles[cls] : static_cast<long long>(op.jobs) * p.gram_tiles[cls];
+            if (cls == 0) round.of_first = static_cast<int>(n);
+            tiles += n;
+        }
+        widest = std::max(widest, tiles - round.first);
+    }
+    if (tiles > (1 << 27)) return NML_ERR_UNSUPPORTED;
+    // no wait is longer than all the work by one block, at 2 us a K slice (0.8 measured)
+    double slices = 0.0;
+    for (int k = 0; k < count; ++k) {
+        const double m = w[k].s.m / 64 + 1, n = w[k].s.n / 64 + 1, t = w[k].mb * (w[k].mb + 1) / 2;
+        slices += steps.of[1].steps * (t * n + 3 * t * m + w[k].mb * (w[k].nb / w[k].wide + 1.0) * (m + 2));
+    }
+
+    if (count <= 8) launch_sums<8>(w, c, call, p.sums, st);
+    else launch_sums<kGroup>(w, c, call, p.sums, st);
+    for (int k = 0; k < steps.of[1].steps; ++k) pack.diagonal[k] = static_cast<float>(ldexp(steps.of[1].step[k].a, steps.of[1].step[k].eu));
+    const int blocks = p.halves + 2 * pack.identities + 1;
+    if (pack.rounds <= kFewRounds) launch_pack<kFewRounds>(pack, call, blocks, st);
+    else launch_pack<kMaxRounds>(pack, call, blocks, st);
+    const ProductParams q = {c, err, static_cast<unsigned long long>(1.5e9 + 2e3 * slices), pack.rounds, static_cast<int>(tiles), p.first_class,
+                             call.out_dtype == NML_F16, call.apply, call.keep, call.rate};
+    // (no more blocks than a round has tiles)
+    const int grid = static_cast<int>(std::min<long long>(widest, sms));
+    if (call.math == NML_MATH_F16) nml::launch(ortho_product_kernel<1>, grid, kThreads, kProductSmem, st, q);
+    else nml::launch(ortho_product_kernel<2>, grid, kThreads, kProductSmem, st, q);
     NMLO_CUDA(cudaGetLastError());
-    nml::count_launches(launched);
+    nml::count_launches(3);
     return NML_OK;
 }
 
 static bool math_ok(int math) { return math == NML_MATH_F16 || math == NML_MATH_3XF16; }
+constexpr int kLongest = 1 << 24;  // (indexes of blocks, tiles and sums are 32-bit)
 static bool size_ok(int rows, int cols) {
-    // (indexes of blocks, tiles and sums are 32-bit)
-    return rows > 0 && cols > 0 && static_cast<long long>(rows) * cols <= (1ll << 36);
+    return rows > 0 && cols > 0 && rows <= kLongest && cols <= kLongest && static_cast<long long>(rows) * cols <= (1ll << 36);
 }
 static void set_sizes(Source& s, int rows, int cols) {
     s.m = std::min(rows, cols);
@@ -988,15 +1352,12 @@ static bool apart(const nml_muon_param* params, int count) {
 // Workspace of the largest group of `count` matrices whose sizes `size(k, source)` sets (false: not a matrix, left out).
 template <class F>
 static int workspace_of(int count, int math, int steps, F&& size, size_t* bytes) {
-    Polynomial poly;
-    poly.steps = steps;
-    poly.chained = math != NML_MATH_F16 && steps > 1;  // (whether they are depends on the coefficients)
     Work w[kGroup];
     *bytes = 0;
     int sms = nml::usable_sms(), filled = 0;
     for (int k = 0; k <= count; ++k) {
         if (filled == kGroup || (k == count && filled > 0)) {
-            *bytes = std::max(*bytes, plan_group(w, filled, math, poly, sms).bytes + 1024);
+            *bytes = std::max(*bytes, plan_group(w, filled, math, steps, sms).bytes + 1024);
             filled = 0;
         }
         if (k < count) {
@@ -1012,13 +1373,18 @@ static int workspace_of(int count, int math, int steps, F&& size, size_t* bytes)
 using namespace nml_ortho;
 
 int nml::prepare_ortho_kernels() {
-    for (int planes = 1; planes <= 2; ++planes)
-        for (int kind = POLY; kind <= RESULT; ++kind)
-            NMLO_CUDA(cudaFuncSetAttribute(product_kernel(planes, kind), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem)));
+    NMLO_CUDA(cudaFuncSetAttribute(ortho_product_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem)));
+    NMLO_CUDA(cudaFuncSetAttribute(ortho_product_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem)));
     cudaFuncAttributes a;
+    for (auto f : {ortho_product_kernel<1>, ortho_product_kernel<2>}) {
+        NMLO_CUDA(cudaFuncGetAttributes(&a, f));
+        if (a.numRegs != kLaunchRegs) return NML_ERR_UNSUPPORTED;  // (a build whose register split would not hold)
+    }
     const void* others[] = {(const void*)ortho_sums_kernel<8, float>, (const void*)ortho_sums_kernel<8, __half>,
                             (const void*)ortho_sums_kernel<kGroup, float>, (const void*)ortho_sums_kernel<kGroup, __half>,
-                            (const void*)ortho_pack_kernel<float>, (const void*)ortho_pack_kernel<__half>, (const void*)momentum_vectors_kernel};
+                            (const void*)ortho_pack_kernel<kFewRounds, float>, (const void*)ortho_pack_kernel<kFewRounds, __half>,
+                            (const void*)ortho_pack_kernel<kMaxRounds, float>, (const void*)ortho_pack_kernel<kMaxRounds, __half>,
+                            (const void*)momentum_vectors_kernel};
     for (const void* f : others) NMLO_CUDA(cudaFuncGetAttributes(&a, f));
     return NML_OK;
 }
@@ -1045,8 +1411,8 @@ int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int o
         };
         if (!dense(x.in_row, x.in_col) || !dense(x.out_row, x.out_col)) return NML_ERR_INVALID;
     }
-    Polynomial poly;
-    if (!polynomial(coefficients, steps, math, &poly)) return NML_ERR_UNSUPPORTED;
+    Steps poly;
+    if (!steps_of(coefficients, steps, &poly)) return NML_ERR_UNSUPPORTED;
     if (count > 0 && (!workspace || workspace_bytes < need)) return NML_ERR_WORKSPACE;
     Call call;
     call.in_dtype = in_dtype;
@@ -1087,8 +1453,8 @@ int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, 
         if (!p.param || !p.grad || !p.momentum || !aligned_to(p.param, 4) || !aligned_to(p.grad, 4) || !aligned_to(p.momentum, 4) || !aligned_to(p.param_f16, 2))
             return NML_ERR_INVALID;
     }
-    Polynomial poly;
-    if (!polynomial(coefficients, steps, math, &poly)) return NML_ERR_UNSUPPORTED;
+    Steps poly;
+    if (!steps_of(coefficients, steps, &poly)) return NML_ERR_UNSUPPORTED;
     if (need > 0 && (!workspace || workspace_bytes < need)) return NML_ERR_WORKSPACE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Call call;

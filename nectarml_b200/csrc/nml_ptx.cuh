@@ -19,7 +19,8 @@ enum {
     ERR_WAIT_FULL = 102,
     ERR_WAIT_TMEM_EMPTY = 103,
     ERR_WAIT_TMEM_FULL = 104,
-    ERR_WAIT_DRAIN = 105
+    ERR_WAIT_DRAIN = 105,
+    ERR_WAIT_TILES = 106
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -91,6 +92,21 @@ __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity) {
         "{\n\t"
         ".reg .pred P;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// Whether the phase is over, at once.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred P;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, P;\n\t"
         "}\n"
         : "=r"(ok)

@@ -23,13 +23,17 @@ def _need(lib, shapes, math=_lib.NML_MATH_3XF16, steps=5):
 
 def test_workspace_size(lib):
     assert _need(lib, []) == (0, 0)
-    block = 65536
-    rc, one = _need(lib, [(128, 256)])          # two iterates of two blocks, seven symmetric matrices of one
-    assert rc == 0 and 11 * block <= one <= 11 * block + 40000
+    block, tables = 65536, 65536
+    rc, one = _need(lib, [(128, 256)])          # two iterates of two blocks, three symmetric matrices of one
+    assert rc == 0 and 7 * block <= one <= 7 * block + tables
     assert _need(lib, [(256, 128)])[1] == one   # turned wide
-    assert _need(lib, [(128, 256)], _lib.NML_MATH_F16)[1] == one + block   # three symmetric ones, and a block of the identity for each step
+    assert _need(lib, [(128, 256)], _lib.NML_MATH_F16)[1] == one + 5 * block   # a block of the identity for each step
+    chained = _need(lib, [(256, 512)])[1]       # two iterates of eight blocks, seven symmetric matrices of three
+    assert 37 * block <= chained <= 37 * block + tables
+    assert _need(lib, [(256, 512)], steps=1)[1] == chained - 12 * block
     group = _need(lib, [(128, 256)] * 128)[1]
-    assert group >= 128 * 11 * block and _need(lib, [(128, 256)] * 1000)[1] == group   # one group at a time
+    assert group >= 128 * 7 * block and _need(lib, [(128, 256)] * 1000)[1] == group   # one group at a time
+    assert _need(lib, [(1, (1 << 24) + 1)])[0] == INVALID
     for bad in ([(0, 4)], [(4, 0)], [(-1, 4)], [(1 << 30, 1 << 30)]):
         assert _need(lib, bad)[0] == INVALID
     for steps in (0, 33, -1):
