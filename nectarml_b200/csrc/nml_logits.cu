@@ -9,12 +9,17 @@
 // the maximum grows.  The reference has no counterpart beyond its softmax and cross-entropy kernels
 // (nectarml/csrc/kernels/tensor/fused/), which write the whole distribution.
 //
+// What bounds it.  Memory: 2 or 4 bytes a logit.  An fp16 logit at the memory's rate leaves an SM 10.7 instructions of a lane and 1.3 of its
+// special function unit, so the inner loop is short: powers of two (the logits times log2 e, less that of the maximum, in one FMA) and pairs of
+// fp32 operations in one instruction; 4.5 instructions and one power a logit.
+//
 // Units.  A row is read in units of 32 bytes (one load of 256 bits) that start on 32-byte boundaries of memory, so a row of an
 // odd vocabulary, which starts anywhere, is read like any other; its first and last unit are taken element by element.
 //
-// Alternatives.  The pass also notes the largest logit of every unit.  The `top` largest elements of a row lie in the `top`
-// units with the largest maxima (a unit that holds one of them has a maximum no element outside those units beats; ties go to the lower index on
-// both levels, as units are contiguous), so those few units are read again and searched; the row is not.
+// Alternatives.  The pass also notes the largest logit of every unit.  Let t be the `top`-th largest among the maxima of 128 groups of
+// units: at least `top` logits are t or more, so only units whose maximum is that are read again, and of their logits only those; each of them
+// then counts those that come before it, which is its place.  The row is not searched.  Where ties make that too many (a row that is
+// masked as a whole), the largest unit is taken `top` times instead.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -35,11 +40,12 @@ using nml::pdl_enter;
         if (e_ != cudaSuccess) return nml::cuda_failed(static_cast<int>(e_), #expr); \
     } while (0)
 
-constexpr int kMaxTop = 32;          // a lane for each selected unit
+constexpr int kMaxTop = 32;          // a lane to each
 constexpr int kUnitBytes = 32;
-constexpr int kGroups = 256;         // of units, for the search: eight to a lane
-constexpr int kMaxUnits = 63 * kGroups;  // of one block's share of a row: its maxima take 63 KB
+constexpr int kGroups = 128;         // of units, for the search
+constexpr int kMaxUnits = 127 * kGroups;  // of one block's share of a row: its maxima take 63.5 KB
 constexpr int kMaxCluster = 8;
+constexpr int kChosen = 256, kCandidates = 512;  // units and logits of the search
 
 __device__ __forceinline__ void load_unit(const void* p, uint32_t (&v)[8]) {
     asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -57,36 +63,100 @@ __device__ __forceinline__ long long load_index(const long long* p) {
     return v;
 }
 
+// Two fp32 values in one register pair.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ float low(uint64_t v) { return unpack2(v).x; }
+__device__ __forceinline__ float high(uint64_t v) { return unpack2(v).y; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// 2^y, 0 below 2^-126; two units in the last place.
+__device__ __forceinline__ float power2(float y) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+    return e;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+
 template <typename T>
 struct Elements;
 template <>
 struct Elements<float> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void unpack(const uint32_t (&v)[8], float (&x)[N]) {
+    // Largest of a unit; NaN where it has one.
+    static __device__ __forceinline__ float largest(const uint32_t (&v)[8]) {
+        float m = __uint_as_float(v[0]);
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = __uint_as_float(v[j]);
+        for (int j = 1; j < 8; ++j) m = max_nan(m, __uint_as_float(v[j]));
+        return m;
     }
-    static __device__ __forceinline__ void pack(const float (&x)[N], uint32_t (&v)[8]) {
+    // As pairs, with what is masked (-inf, or the lowest value) at a finite distance.
+    static __device__ __forceinline__ void pairs(const uint32_t (&v)[8], uint64_t (&x)[N / 2]) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = __float_as_uint(x[j]);
+        for (int j = 0; j < N / 2; ++j) x[j] = pack2(fmaxf(__uint_as_float(v[2 * j]), -1e32f), fmaxf(__uint_as_float(v[2 * j + 1]), -1e32f));
     }
+    static __device__ __forceinline__ float get(const uint32_t (&v)[8], int j) { return __uint_as_float(v[j]); }
+    static __device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+    static __device__ __forceinline__ void pack(const uint64_t (&x)[N / 2], uint32_t (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) v[2 * j] = __float_as_uint(low(x[j])), v[2 * j + 1] = __float_as_uint(high(x[j]));
+    }
+    static __device__ __forceinline__ uint32_t load_bits(const float* p) { return __float_as_uint(load_global(p)); }
     static __device__ __forceinline__ float load(const float* p) { return load_global(p); }
     static __device__ __forceinline__ float round(float x) { return x; }
 };
 template <>
 struct Elements<__half> {
     static constexpr int N = 16;
-    static __device__ __forceinline__ void unpack(const uint32_t (&v)[8], float (&x)[N]) {
+    static __device__ __forceinline__ __half2 at(const uint32_t (&v)[8], int j) { return *reinterpret_cast<const __half2*>(&v[j]); }
+    static __device__ __forceinline__ float largest(const uint32_t (&v)[8]) {
+        __half2 m = at(v, 0);
+#pragma unroll
+        for (int j = 1; j < 8; ++j) m = __hmax2_nan(m, at(v, j));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ void pairs(const uint32_t (&v)[8], uint64_t (&x)[N / 2]) {
+        const __half2 lowest = __half2half2(__ushort_as_half(0xfbff));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[j]));
-            x[2 * j] = f.x;
-            x[2 * j + 1] = f.y;
+            const float2 f = __half22float2(__hmax2(at(v, j), lowest));
+            x[j] = pack2(f.x, f.y);
         }
     }
-    static __device__ __forceinline__ void pack(const float (&x)[N], uint32_t (&v)[8]) {
+    static __device__ __forceinline__ float get(const uint32_t (&v)[8], int j) {
+        return j & 1 ? __high2float(at(v, j / 2)) : __low2float(at(v, j / 2));
+    }
+    static __device__ __forceinline__ void pack(const uint64_t (&x)[N / 2], uint32_t (&v)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) *reinterpret_cast<__half2*>(&v[j]) = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+        for (int j = 0; j < 8; ++j) {
+            const __half2 h = __floats2half2_rn(low(x[j]), high(x[j]));
+            v[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
     }
     static __device__ __forceinline__ float load(const __half* p) { return __half2float(load_global(p)); }
     static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
@@ -95,96 +165,127 @@ struct Elements<__half> {
 // Floats in the order of unsigned integers (-0 and 0 are one value; NaN above everything).  0 is below every float: "none".
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return x != x ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // A row as units: unit u holds the elements u * N - lead ... of which those in [0, vocab) exist.
 template <typename T>
 struct Row {
+    static constexpr int N = Elements<T>::N;
     const T* base;  // of unit 0: at or before the row's first element, on a 32-byte boundary
     int lead, vocab, units;
+    int full0, full1;  // units without a gap
     __device__ __forceinline__ Row(const T* row, int vocab_) {
         lead = static_cast<int>((reinterpret_cast<uintptr_t>(row) & (kUnitBytes - 1)) / sizeof(T));
         base = row - lead;
         vocab = vocab_;
-        units = static_cast<int>((static_cast<long long>(lead) + vocab + Elements<T>::N - 1) / Elements<T>::N);
+        const long long end = static_cast<long long>(lead) + vocab;
+        units = static_cast<int>((end + N - 1) / N);
+        full0 = lead ? 1 : 0;
+        full1 = static_cast<int>(end / N);
     }
-    __device__ __forceinline__ bool full(int u) const {
-        return (u > 0 || lead == 0) && (u + 1 < units || (lead + static_cast<long long>(vocab)) % Elements<T>::N == 0);
-    }
-    // The unit's elements; `none` where there is none.
-    __device__ __forceinline__ void load(int u, float none, float (&x)[Elements<T>::N]) const {
-        const T* p = base + static_cast<long long>(u) * Elements<T>::N;
-        if (full(u)) {
-            uint32_t v[8];
-            load_unit(p, v);
-            Elements<T>::unpack(v, x);
-        } else {
+    __device__ __forceinline__ const T* at(int u) const { return base + static_cast<long long>(u) * N; }
+    __device__ __forceinline__ long long first(int u) const { return static_cast<long long>(u) * N - lead; }
+    __device__ __forceinline__ bool has(long long i) const { return i >= 0 && i < vocab; }
+    // The bits of a unit with gaps; those of -inf in them.
+    __device__ __forceinline__ void load_broken(int u, uint32_t (&v)[8]) const {
+        uint32_t w[N];
 #pragma unroll
-            for (int j = 0; j < Elements<T>::N; ++j) {
-                const long long i = static_cast<long long>(u) * Elements<T>::N + j - lead;
-                x[j] = i >= 0 && i < vocab ? Elements<T>::load(p + j) : none;
-            }
+        for (int j = 0; j < N; ++j) {
+            const float x = has(first(u) + j) ? Elements<T>::load(at(u) + j) : -INFINITY;
+            w[j] = sizeof(T) == 4 ? __float_as_uint(x) : static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x)));
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = sizeof(T) == 4 ? w[j % N] : w[2 * j % N] | w[(2 * j + 1) % N] << 16;
     }
 };
 
-// Running statistics: the maximum, sum e^(x - m) and sum (x - m) e^(x - m).  While everything is -inf, m is -inf and the sums are 0.
+// Running statistics: the maximum m, and against 2^M, M = m log2 e rounded, the sums of 2^y and y 2^y with y = x log2 e - M.
+// While everything is -inf, m is -inf and the sums are 0.  Where m is no number or infinite, so is the row, and the sums do not matter.
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Where a maximum leaves no room below it for what is masked (fp16: near the lowest value), or is so large that the product with log2 e
+// would not be finite, logits are taken by their distance from m, which is then the reference itself.
+template <typename T>
+__device__ __forceinline__ bool extreme(float m) { return sizeof(T) == 4 ? !(fabsf(m) < 1e30f) : m < -65000.f; }
+template <typename T>
+__device__ __forceinline__ float reference(float m) { return extreme<T>(m) ? 0.f : __fmul_rn(m, kLog2e); }  // (rounded wherever it stands)
+constexpr float kFar = -1e30f;  // instead of a distance of -inf
+
 struct Stats {
     float m, s, t;
 };
-constexpr float kLog2e = 1.4426950408889634f;
-// e^d underflows to 0 well above this; it keeps (x - m) e^(x - m) at 0 where x is -inf.
-constexpr float kLowest = -200.f;
-
-__device__ __forceinline__ float exp_of(float d) { return exp2f(d * kLog2e); }
-
-// The same statistics against a larger maximum.
-__device__ __forceinline__ void raise(Stats& a, float m) {
-    if (a.m < m) {
-        if (a.s != 0.f) {  // (so m is finite; a sum that is NaN stays it)
-            const float d = a.m - m, f = exp_of(d);
-            a.t = (a.t + fmaxf(d, kLowest) * a.s) * f;
-            a.s *= f;
-        }
-        a.m = m;
-    }
-}
-__device__ __forceinline__ void merge(Stats& a, Stats b) {
-    const float m = fmaxf(a.m, b.m);
-    raise(a, m);
-    raise(b, m);
-    a.s += b.s;
-    a.t += b.t;
-}
-
+// How far y moves where the maximum a becomes b >= a.
 template <typename T>
-__device__ __forceinline__ float add_unit(Stats& a, const float (&x)[Elements<T>::N]) {
-    float m = x[0];
-#pragma unroll
-    for (int j = 1; j < Elements<T>::N; ++j) m = fmaxf(m, x[j]);
-    raise(a, m);
-    const float ref = a.m == -INFINITY ? 0.f : a.m;
-#pragma unroll
-    for (int j = 0; j < Elements<T>::N; ++j) {
-        const float d = x[j] - ref, e = exp_of(d);
-        a.s += e;
-        a.t += fmaxf(d, kLowest) * e;
+__device__ __forceinline__ float moved_by(float a, float b) {
+    return extreme<T>(a) || extreme<T>(b) ? fmaxf((a - b) * kLog2e, kFar) : reference<T>(a) - reference<T>(b);
+}
+// The statistics of the lanes of a warp (or of its first `width`), in every lane: against the largest maximum, once, then two plain sums.
+template <typename T>
+__device__ __forceinline__ Stats merge_lanes(Stats a, int width = 32) {
+    float m = a.m;
+    for (int o = width / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float d = a.s != 0.f ? moved_by<T>(a.m, m) : 0.f, f = power2(d);
+    a.t = (a.t + d * a.s) * f;
+    a.s *= f;
+    for (int o = width / 2; o > 0; o /= 2) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
     }
-    return m;
+    a.m = m;
+    return a;
 }
 
-__device__ __forceinline__ Stats shuffle(const Stats& a, int o) {
-    return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)};
-}
+// A thread's own, the sums over even and odd elements apart.
+template <typename T>
+struct Running {
+    float m = -INFINITY, M = 0.f;
+    uint64_t s = 0, t = 0;
+
+    // -> the unit's largest
+    __device__ __forceinline__ float add(const uint32_t (&v)[8]) {
+        constexpr int N = Elements<T>::N;
+        const float most = Elements<T>::largest(v);
+        if (!(most <= m)) {
+            const float now = max_nan(m, most), d = s != 0 ? moved_by<T>(m, now) : 0.f, f = power2(d);
+            t = mul2(fma2(pack2(d, d), s, t), pack2(f, f));
+            s = mul2(s, pack2(f, f));
+            m = now;
+            M = reference<T>(m);
+        }
+        if (extreme<T>(m) && m != -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float y = fmaxf((Elements<T>::get(v, j) - m) * kLog2e, kFar), e = power2(y);
+                s = add2(s, pack2(e, 0.f));
+                t = add2(t, pack2(y * e, 0.f));
+            }
+            return most;
+        }
+        uint64_t x[N / 2];
+        Elements<T>::pairs(v, x);
+        const uint64_t k = pack2(kLog2e, kLog2e), r = pack2(-M, -M);
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            const uint64_t y = fma2(x[j], k, r), e = pack2(power2(low(y)), power2(high(y)));
+            s = add2(s, e);
+            t = fma2(y, e, t);
+        }
+        return most;
+    }
+    __device__ __forceinline__ Stats done() const { return {m, low(s) + high(s), low(t) + high(t)}; }
+};
 
 // One block's part of the search, and a cluster's exchange.
 struct Shared {
     Stats warp[8], block;
-    uint32_t group[kGroups];
-    int chosen[kMaxTop];
-    uint32_t key[kMaxTop];   // the block's alternatives, in order
+    alignas(16) uint32_t group[kGroups];  // (read as vectors)
+    uint32_t threshold;
+    int units, candidates;
+    int unit[kChosen];
+    uint32_t candidate_key[kCandidates];
+    int candidate_index[kCandidates];
+    uint32_t key[kMaxTop];   // the block's alternatives, in order; 0: fewer
     int index[kMaxTop];
 };
 
@@ -193,100 +294,142 @@ __device__ __forceinline__ void block_sync() {
     if (kThreads == 32) __syncwarp(); else __syncthreads();
 }
 
-// The `top` largest of up to 32 x 8 candidates in registers, by value, then by index; lane r receives the r-th.
-template <int N>
-__device__ __forceinline__ void select(uint32_t (&key)[N], const int (&index)[N], int top, uint32_t& out_key, int& out_index) {
-    const int lane = threadIdx.x & 31;
-    out_key = 0;
-    out_index = 0;
-    for (int r = 0; r < top; ++r) {
-        uint32_t best = 0;
-#pragma unroll
-        for (int j = 0; j < N; ++j) best = max(best, key[j]);
-        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-        uint32_t first = 0xffffffffu;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (key[j] == most) first = min(first, static_cast<uint32_t>(index[j]));
-        const uint32_t who = __reduce_min_sync(0xffffffffu, first);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (key[j] == most && static_cast<uint32_t>(index[j]) == who) key[j] = 0;
-        if (lane == r) {
-            out_key = most;
-            out_index = static_cast<int>(who);
+// Places of `count` candidates by value, then by index: the first `top` go to key and index.
+template <int kThreads>
+__device__ __forceinline__ void place(const uint32_t* keys, const int* indices, int count, int top, uint32_t* key, int* index) {
+    for (int c = threadIdx.x; c < count; c += kThreads) {
+        const uint32_t k = keys[c];
+        const int i = indices[c];
+        int before = 0;
+        for (int o = 0; o < count; ++o) before += keys[o] > k || (keys[o] == k && indices[o] < i);
+        if (before < top && k != 0) {
+            key[before] = k;
+            index[before] = i;
         }
     }
+}
+
+// The largest unit, `top` times: for rows with so many ties that the search below finds no short list, and for rows of one warp.  Takes the maxima of
+// the units that it chooses away.
+template <typename T>
+__device__ __forceinline__ void search_units(const Row<T>& row, int first, int n, int per, int top, uint32_t* maxima, Shared& sh) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kMine = kGroups / 32, N = Elements<T>::N;
+    uint32_t group[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) group[j] = sh.group[lane * kMine + j];
+    int found = 0;
+    uint32_t last = 0;
+    for (; found < top; ++found) {
+        uint32_t best = 0;
+        int at = 0;
+#pragma unroll
+        for (int j = kMine - 1; j >= 0; --j)
+            if (group[j] >= best) best = group[j], at = j;
+        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+        if (most == 0) break;  // fewer units than alternatives
+        last = most;
+        const int owner = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
+        const int lo = __shfl_sync(0xffffffffu, lane * kMine + at, owner) * per, hi = min(n, lo + per);
+        // its first unit with that maximum, and its maximum without that unit
+        uint32_t unit = 0xffffffffu, rest = 0;
+        for (int u = lo + lane; u < hi; u += 32)
+            if (maxima[u] == most) unit = min(unit, static_cast<uint32_t>(u));
+        unit = __reduce_min_sync(0xffffffffu, unit);
+        for (int u = lo + lane; u < hi; u += 32)
+            if (u != static_cast<int>(unit)) rest = max(rest, maxima[u]);
+        rest = __reduce_max_sync(0xffffffffu, rest);
+        __syncwarp();
+        if (lane == 0) {
+            maxima[unit] = 0;
+            sh.unit[found] = static_cast<int>(unit);
+        }
+        if (lane == owner) {
+#pragma unroll
+            for (int j = 0; j < kMine; ++j)
+                if (j == at) group[j] = rest;
+        }
+        __syncwarp();
+    }
+    if (found < top) last = 1;
+    // their elements that are as large as the last one's, at most 32 x 16
+    int count = 0;
+    for (int e0 = 0; e0 < found * N; e0 += 32) {
+        const int e = e0 + lane, u = first + (e < found * N ? sh.unit[e / N] : 0);
+        const long long i = row.first(u) + e % N;
+        const uint32_t k = e < found * N && row.has(i) ? order_key(Elements<T>::load(row.at(u) + e % N)) : 0;
+        const bool in = k != 0 && k >= last;
+        const unsigned who = __ballot_sync(0xffffffffu, in);
+        if (in) {
+            const int slot = count + __popc(who & ((1u << lane) - 1));
+            sh.candidate_key[slot] = k;
+            sh.candidate_index[slot] = static_cast<int>(i);
+        }
+        count += __popc(who);
+    }
+    __syncwarp();
+    place<32>(sh.candidate_key, sh.candidate_index, count, top, sh.key, sh.index);
+    __syncwarp();
 }
 
 // The block's alternatives among its units [0, n) (unit 0 is unit `first` of the row), from the units' maxima, into sh.key and sh.index.
 template <typename T, int kThreads>
 __device__ __forceinline__ void search(const Row<T>& row, int first, int n, int top, uint32_t* maxima, Shared& sh) {
+    constexpr int N = Elements<T>::N;
+    const int tid = threadIdx.x;
     const int per = ((n + kGroups - 1) / kGroups) | 1;  // odd: a thread's stride through shared memory meets every bank
-    for (int g = threadIdx.x; g < kGroups; g += kThreads) {
+    for (int g = tid; g < kGroups; g += kThreads) {
         uint32_t best = 0;
-        for (int i = g * per; i < min(n, (g + 1) * per); ++i) best = max(best, maxima[i]);
+        for (int u = g * per; u < min(n, (g + 1) * per); ++u) best = max(best, maxima[u]);
         sh.group[g] = best;
     }
+    if (tid < kMaxTop) sh.key[tid] = 0, sh.index[tid] = 0;
+    if (tid == 0) sh.units = sh.candidates = 0;
     block_sync<kThreads>();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        uint32_t group[kGroups / 32];
-#pragma unroll
-        for (int j = 0; j < kGroups / 32; ++j) group[j] = sh.group[lane * (kGroups / 32) + j];
-        int found = 0;
-        for (; found < top; ++found) {
-            uint32_t best = 0;
-            int at = 0;
-#pragma unroll
-            for (int j = kGroups / 32 - 1; j >= 0; --j)
-                if (group[j] >= best) best = group[j], at = j;
-            const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-            if (most == 0) break;  // fewer units than alternatives
-            const int owner = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
-            const int g = __shfl_sync(0xffffffffu, lane * (kGroups / 32) + at, owner);
-            // its first unit with that maximum, and its maximum without that unit
-            const int lo = g * per, a = lo + lane, b = a + 32;
-            const bool has_a = lane < per && a < n, has_b = lane + 32 < per && b < n;
-            const uint32_t va = has_a ? maxima[a] : 0, vb = has_b ? maxima[b] : 0;
-            const unsigned in_a = __ballot_sync(0xffffffffu, has_a && va == most), in_b = __ballot_sync(0xffffffffu, has_b && vb == most);
-            const int unit = lo + (in_a ? __ffs(in_a) - 1 : 32 + __ffs(in_b) - 1);
-            const uint32_t rest = __reduce_max_sync(0xffffffffu, max(a == unit ? 0u : va, b == unit ? 0u : vb));
-            if (lane == 0) {
-                maxima[unit] = 0;
-                sh.chosen[found] = unit;
-            }
-            if (lane == owner) {
-#pragma unroll
-                for (int j = 0; j < kGroups / 32; ++j)
-                    if (j == at) group[j] = rest;
-            }
-            __syncwarp();
+    if constexpr (kThreads == 32) {  // (a warp would be 128 x 128 comparisons about it)
+        search_units(row, first, n, per, top, maxima, sh);
+    } else {
+    for (int g = tid; g < kGroups; g += kThreads) {
+        const uint32_t k = sh.group[g];
+        int before = 0;
+#pragma unroll 8
+        for (int o = 0; o < kGroups / 4; ++o) {
+            const uint4 v = reinterpret_cast<const uint4*>(sh.group)[o];
+            before += (v.x > k) + (v.y > k) + (v.z > k) + (v.w > k);
+            before += (v.x == k && 4 * o < g) + (v.y == k && 4 * o + 1 < g) + (v.z == k && 4 * o + 2 < g) + (v.w == k && 4 * o + 3 < g);
         }
-        // a lane to a unit; the elements are compared by value, then index
-        uint32_t key[Elements<T>::N];
-        int index[Elements<T>::N];
-#pragma unroll
-        for (int j = 0; j < Elements<T>::N; ++j) key[j] = 0, index[j] = 0;
-        if (lane < found) {
-            const int u = first + sh.chosen[lane];
-            float x[Elements<T>::N];
-            row.load(u, 0.f, x);
-#pragma unroll
-            for (int j = 0; j < Elements<T>::N; ++j) {
-                const long long i = static_cast<long long>(u) * Elements<T>::N + j - row.lead;
-                index[j] = static_cast<int>(i);
-                key[j] = i >= 0 && i < row.vocab ? order_key(x[j]) : 0;
+        if (before == top - 1) sh.threshold = max(k, 1u);  // (fewer groups than alternatives: whatever exists)
+    }
+    block_sync<kThreads>();
+    const uint32_t threshold = sh.threshold;
+    for (int u = tid; u < n; u += kThreads)
+        if (maxima[u] >= threshold) {
+            const int slot = atomicAdd(&sh.units, 1);
+            if (slot < kChosen) sh.unit[slot] = u;
+        }
+    block_sync<kThreads>();
+    const int units = sh.units;
+    if (units <= kChosen) {
+        for (int e = tid; e < units * N; e += kThreads) {
+            const int u = first + sh.unit[e / N];
+            const long long i = row.first(u) + e % N;
+            const uint32_t k = row.has(i) ? order_key(Elements<T>::load(row.at(u) + e % N)) : 0;
+            if (k >= threshold) {
+                const int slot = atomicAdd(&sh.candidates, 1);
+                if (slot < kCandidates) {
+                    sh.candidate_key[slot] = k;
+                    sh.candidate_index[slot] = static_cast<int>(i);
+                }
             }
         }
-        uint32_t k;
-        int i;
-        select(key, index, top, k, i);
-        if (lane < top) {
-            sh.key[lane] = k;
-            sh.index[lane] = i;
-        }
-        __syncwarp();
+    }
+    block_sync<kThreads>();
+    if (units <= kChosen && sh.candidates <= kCandidates) {
+        place<kThreads>(sh.candidate_key, sh.candidate_index, sh.candidates, top, sh.key, sh.index);
+    } else if (tid < 32) {
+        search_units(row, first, n, per, top, maxima, sh);
+    }
+    block_sync<kThreads>();
     }
 }
 
@@ -304,35 +447,48 @@ template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const ForwardParams P) {
     pdl_enter();
     namespace cg = cooperative_groups;
-    __shared__ Shared sh;
+    __shared__ __align__(16) Shared sh;
     extern __shared__ uint32_t maxima[];
-    constexpr int N = Elements<T>::N;
     const int rank = P.cluster > 1 ? static_cast<int>(blockIdx.x % P.cluster) : 0;
     const int tid = threadIdx.x;
     for (long long r = blockIdx.x / P.cluster; r < P.rows; r += gridDim.x / P.cluster) {
         const Row<T> row(static_cast<const T*>(P.logits) + r * P.pitch, P.vocab);
         const int share = (row.units + P.cluster - 1) / P.cluster;
         const int u0 = min(row.units, rank * share), u1 = min(row.units, u0 + share);
-        Stats a = {-INFINITY, 0.f, 0.f};
-        for (int u = u0 + tid; u < u1; u += kThreads) {
-            float x[N];
-            row.load(u, -INFINITY, x);
-            const float m = add_unit<T>(a, x);
-            if (P.top) {
-                float best = m;  // (a maximum passes over NaN)
-#pragma unroll
-                for (int j = 0; j < N; ++j) best = x[j] != x[j] ? x[j] : best;
-                maxima[u - u0] = order_key(best);
+        Running<T> run;
+        auto take = [&](int u, const uint32_t (&v)[8]) {
+            const float most = run.add(v);
+            if (P.top) maxima[u - u0] = order_key(most);
+        };
+        const int f0 = max(u0, row.full0), f1 = min(u1, row.full1);
+        int u = f0 + tid;
+        for (; u + kThreads < f1; u += 2 * kThreads) {
+            uint32_t a[8], b[8];
+            load_unit(row.at(u), a);
+            load_unit(row.at(u + kThreads), b);
+            take(u, a);
+            take(u + kThreads, b);
+        }
+        if (u < f1) {
+            uint32_t a[8];
+            load_unit(row.at(u), a);
+            take(u, a);
+        }
+        // the first and the last unit, where they have gaps
+        if (tid < 2) {
+            const int e = tid == 0 ? 0 : row.units - 1;
+            const bool broken = tid == 0 ? row.full0 == 1 : row.full1 < row.units && !(row.full0 == 1 && row.units == 1);
+            if (broken && e >= u0 && e < u1) {
+                uint32_t a[8];
+                row.load_broken(e, a);
+                take(e, a);
             }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2) merge(a, shuffle(a, o));
+        Stats a = merge_lanes<T>(run.done());
         if (kThreads > 32) {
             if ((tid & 31) == 0) sh.warp[tid / 32] = a;
             __syncthreads();
-            a = sh.warp[0];
-#pragma unroll
-            for (int w = 1; w < kThreads / 32; ++w) merge(a, sh.warp[w]);
+            if (tid < 32) a = merge_lanes<T>(sh.warp[tid % (kThreads / 32)], kThreads / 32);
         }
         if (P.top) {
             block_sync<kThreads>();
@@ -344,26 +500,28 @@ __global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const Forward
             cg::cluster_group cluster = cg::this_cluster();
             if (tid == 0) sh.block = a;
             cluster.sync();
-            if (rank == 0 && tid < 32) {
-                for (int c = 1; c < P.cluster; ++c) merge(a, *cluster.map_shared_rank(&sh.block, c));
+            if (rank == 0) {
+                if (tid < 32) a = merge_lanes<T>(*cluster.map_shared_rank(&sh.block, tid % P.cluster), P.cluster);
                 if (P.top) {
-                    uint32_t keys[kMaxCluster];
-                    int indices[kMaxCluster];
-#pragma unroll
-                    for (int c = 0; c < kMaxCluster; ++c) {
-                        keys[c] = c < P.cluster && tid < P.top ? cluster.map_shared_rank(sh.key, c)[tid] : 0;
-                        indices[c] = c < P.cluster && tid < P.top ? cluster.map_shared_rank(sh.index, c)[tid] : 0;
+                    const int count = P.cluster * P.top;
+                    for (int e = tid; e < count; e += kThreads) {
+                        sh.candidate_key[e] = cluster.map_shared_rank(sh.key, e / P.top)[e % P.top];
+                        sh.candidate_index[e] = cluster.map_shared_rank(sh.index, e / P.top)[e % P.top];
                     }
-                    select(keys, indices, P.top, key, index);
+                    __syncthreads();
+                    place<kThreads>(sh.candidate_key, sh.candidate_index, count, P.top, sh.key, sh.index);
+                    __syncthreads();
                 }
             }
-        } else if (P.top && tid < P.top) {
+        }
+        if (P.top && tid < P.top) {
             key = sh.key[tid];
             index = sh.index[tid];
         }
         if (rank == 0 && tid < 32) {
-            const bool dead = a.s == 0.f;  // nothing but -inf
-            const float log_sum = dead ? 0.f : logf(a.s);
+            const bool dead = a.m == -INFINITY, bad = !(a.m < INFINITY);  // nothing but -inf; a NaN or +inf
+            const float off = extreme<T>(a.m) ? 0.f : fmaf(a.m, kLog2e, -reference<T>(a.m));  // of the reference, from m log2 e
+            const float log_sum = dead ? 0.f : bad ? NAN : logf(a.s) - off * kLn2;
             if (tid < P.top) {
                 P.top_indices[r * P.top + tid] = index;
                 P.top_log_probs[r * P.top + tid] = dead ? -INFINITY : (key_value(key) - a.m) - log_sum;
@@ -378,7 +536,7 @@ __global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const Forward
                     lp = dead ? -INFINITY : (x - a.m) - log_sum;
                 }
                 P.log_probs[r] = lp;
-                P.entropy[r] = dead ? 0.f : log_sum - a.t / a.s;
+                P.entropy[r] = dead ? 0.f : bad ? NAN : logf(a.s) - kLn2 * (a.t / a.s);
                 P.stats[2 * r] = a.m;
                 P.stats[2 * r + 1] = log_sum;
             }
@@ -411,26 +569,53 @@ __global__ void __launch_bounds__(256) token_log_probs_backward_kernel(const Bac
     const float g = target < 0 ? 0.f : target < P.vocab ? load_global(P.d_log_probs + r) : NAN;
     const float gh = P.d_entropy ? load_global(P.d_entropy + r) : 0.f;
     const float h = P.d_entropy ? load_global(P.entropy + r) : 0.f;
-    const bool dead = m == -INFINITY && log_sum == 0.f;
+    const bool dead = m == -INFINITY && log_sum == 0.f, far = extreme<T>(m);
+    // With y = log2 p: d = -2^y (g + gh (y ln 2 + h)).  y = x log2 e - M - k, where M is m log2 e rounded and k what else belongs to it.
+    const float M = __fmul_rn(m, kLog2e), k = fmaf(m, kLog2e, -M) + log_sum * kLog2e;
+    const uint64_t l2 = pack2(kLog2e, kLog2e), m2 = pack2(-M, -M), k2 = pack2(-k, -k);
+    const float slope = -gh * kLn2, level = -fmaf(gh, h, g);
+    const uint64_t slope2 = pack2(slope, slope), level2 = pack2(level, level);
+    const bool entropy = P.d_entropy != nullptr;
     for (int u = part * blockDim.x + threadIdx.x; u < row.units; u += P.blocks_per_row * blockDim.x) {
-        float x[N];
-        row.load(u, 0.f, x);
-        const long long first = static_cast<long long>(u) * N - row.lead;
+        const bool full = u >= row.full0 && u < row.full1;
+        uint32_t v[8];
+        if (full) load_unit(row.at(u), v); else row.load_broken(u, v);
+        uint64_t x[N / 2];
+        if (!far) {
+            Elements<T>::pairs(v, x);
+        } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float lp = (x[j] - m) - log_sum, p = exp_of(lp);
-            float d = -p * (g + gh * (fmaxf(lp, kLowest) + h));
-            if (first + j == target) d += g;
-            x[j] = dead ? 0.f : d;
+            for (int j = 0; j < N / 2; ++j)
+                x[j] = pack2(fmaxf((Elements<T>::get(v, 2 * j) - m) * kLog2e, -1e5f), fmaxf((Elements<T>::get(v, 2 * j + 1) - m) * kLog2e, -1e5f));
         }
-        if (P.together && row.full(u)) {
-            uint32_t v[8];
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            uint64_t y;
+            if (far) y = add2(x[j], pack2(-log_sum * kLog2e, -log_sum * kLog2e));
+            else y = add2(fma2(x[j], l2, m2), k2);
+            if (sizeof(T) == 4) y = pack2(fmaxf(low(y), -1e5f), fmaxf(high(y), -1e5f));  // (times a gradient of any size)
+            const uint64_t e = pack2(power2(low(y)), power2(high(y)));
+            x[j] = mul2(e, entropy ? fma2(y, slope2, level2) : level2);
+        }
+        const long long first = row.first(u);
+        if (target >= first && target < first + N && target >= 0) {
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) {
+                if (target - first == 2 * j) x[j] = pack2(low(x[j]) + g, high(x[j]));
+                if (target - first == 2 * j + 1) x[j] = pack2(low(x[j]), high(x[j]) + g);
+            }
+        }
+        if (dead) {
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) x[j] = 0;
+        }
+        if (P.together && full) {
             Elements<T>::pack(x, v);
             store_unit(out + first, v);
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (first + j >= 0 && first + j < P.vocab) out[first + j] = Elements<T>::round(x[j]);
+                if (row.has(first + j)) out[first + j] = Elements<T>::round(j & 1 ? high(x[j / 2]) : low(x[j / 2]));
         }
     }
 }
@@ -444,7 +629,7 @@ static ForwardPlan forward_plan(long long rows, int vocab, int dtype, int top) {
     const int n = dtype == NML_F16 ? Elements<__half>::N : Elements<float>::N;
     const int units = static_cast<int>((static_cast<long long>(vocab) + 2 * n - 2) / n);  // at the worst start of a row
     ForwardPlan p;
-    p.threads = units <= 128 ? 32 : units <= 1024 ? 128 : 256;
+    p.threads = units <= 128 ? 32 : units <= 4096 ? 128 : 256;
     while (p.cluster < kMaxCluster && p.threads == 256 && (rows * p.cluster < 148 || (top && (units + p.cluster - 1) / p.cluster > kMaxUnits))) p.cluster *= 2;
     const int share = (units + p.cluster - 1) / p.cluster;
     p.ok = !top || share <= kMaxUnits;
@@ -513,7 +698,7 @@ int nml_token_log_probs_backward(const void* logits, int dtype, long long rows, 
     if (const int rc = nml::current_device(&status, &sms)) return rc;
     const int size = dtype == NML_F16 ? 2 : 4, n = kUnitBytes / size;
     const long long units = (static_cast<long long>(vocab) + 2 * n - 2) / n;
-    long long per_row = (units + 1023) / 1024;  // four units a thread
+    long long per_row = (units + 2047) / 2048;  // eight units a thread
     if (rows * per_row > 0x7fffffff) per_row = 1;
     if (rows > 0x7fffffff) return NML_ERR_UNSUPPORTED;
     const bool together = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(d_logits)) % kUnitBytes == 0 &&

@@ -37,7 +37,7 @@ def plain(x, targets, top=0):
 def chain(vocab, dtype):
     per = 16 if dtype == torch.float16 else 8
     units = -(-vocab // per) + 1
-    threads = 32 if units <= 128 else 128 if units <= 1024 else 256
+    threads = 32 if units <= 128 else 128
     return 5 * per * -(-units // threads) + 16
 
 
@@ -142,8 +142,14 @@ def test_masks(vocab, dtype):
     x[7, ::2] = 0.0                       # one value
     x[8] = torch.finfo(dtype).max
     x[9, 3] = torch.finfo(dtype).max
+    x[10] = -math.inf
+    x[10, 2::3] = lowest                  # masked both ways, nothing else left
+    x[11, vocab // 3:] = -math.inf
+    x[11, : vocab // 4] = lowest
     t = torch.tensor([1, 2, vocab - 1, 0, vocab - 1, 0, 3, 4, 5, 3, -1, vocab], device=DEV)
     r = check_forward(x, t, min(20, vocab))
+    for entropy in (False, True):
+        check_backward(x, t.clamp(max=vocab - 1), entropy)
     assert r.log_probs[0] == -math.inf and r.entropy[0] == 0 and r.stats[0].tolist() == [-math.inf, 0.0]
     assert r.top_log_probs[0].eq(-math.inf).all() and r.top_indices[0].tolist() == list(range(min(20, vocab)))
     assert r.entropy[4] == 0 and r.log_probs[4] == 0
