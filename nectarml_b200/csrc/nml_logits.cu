@@ -45,6 +45,7 @@ constexpr int kUnitBytes = 32;
 constexpr int kGroups = 128;         // of units, for the search
 constexpr int kMaxUnits = 127 * kGroups;  // of one block's share of a row: its maxima take 63.5 KB
 constexpr int kMaxCluster = 8;
+constexpr int kWarpRows = 4;         // rows of a warp each, to a block
 constexpr int kChosen = 256, kCandidates = 512;  // units and logits of the search
 
 __device__ __forceinline__ void load_unit(const void* p, uint32_t (&v)[8]) {
@@ -283,10 +284,8 @@ struct Shared {
     uint32_t threshold;
     int units, candidates;
     int unit[kChosen];
-    uint32_t candidate_key[kCandidates];
-    int candidate_index[kCandidates];
-    uint32_t key[kMaxTop];   // the block's alternatives, in order; 0: fewer
-    int index[kMaxTop];
+    alignas(16) uint64_t candidate[kCandidates];
+    uint64_t best[kMaxTop];  // the block's alternatives, in order; 0: fewer
 };
 
 template <int kThreads>
@@ -294,23 +293,29 @@ __device__ __forceinline__ void block_sync() {
     if (kThreads == 32) __syncwarp(); else __syncthreads();
 }
 
-// Places of `count` candidates by value, then by index: the first `top` go to key and index.
+// An element as a number: by value, then the lower index first; 0: none.
+__device__ __forceinline__ uint64_t candidate(uint32_t key, long long index) { return key ? static_cast<uint64_t>(key) << 32 | (0xffffffffu - static_cast<uint32_t>(index)) : 0; }
+__device__ __forceinline__ float value_of(uint64_t c) { return key_value(static_cast<uint32_t>(c >> 32)); }
+__device__ __forceinline__ int index_of(uint64_t c) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(c)); }
+
+// Places of `count` candidates (all different): the first `top` go to best.
 template <int kThreads>
-__device__ __forceinline__ void place(const uint32_t* keys, const int* indices, int count, int top, uint32_t* key, int* index) {
+__device__ __forceinline__ void place(uint64_t* candidates, int count, int top, uint64_t* best) {
     for (int c = threadIdx.x; c < count; c += kThreads) {
-        const uint32_t k = keys[c];
-        const int i = indices[c];
+        const uint64_t mine = candidates[c];
         int before = 0;
-        for (int o = 0; o < count; ++o) before += keys[o] > k || (keys[o] == k && indices[o] < i);
-        if (before < top && k != 0) {
-            key[before] = k;
-            index[before] = i;
+#pragma unroll 4
+        for (int o = 0; o < count / 2; ++o) {
+            const ulonglong2 v = reinterpret_cast<const ulonglong2*>(candidates)[o];
+            before += (v.x > mine) + (v.y > mine);
         }
+        if (count & 1) before += candidates[count - 1] > mine;
+        if (before < top && mine != 0) best[before] = mine;
     }
 }
 
-// The largest unit, `top` times: for rows with so many ties that the search below finds no short list, and for rows of one warp.  Takes the maxima of
-// the units that it chooses away.
+// The largest unit, `top` times: for rows with so many ties that the search below finds no short list.  One warp; takes the maxima of the
+// units that it chooses away.
 template <typename T>
 __device__ __forceinline__ void search_units(const Row<T>& row, int first, int n, int per, int top, uint32_t* maxima, Shared& sh) {
     const int lane = threadIdx.x & 31;
@@ -354,6 +359,7 @@ __device__ __forceinline__ void search_units(const Row<T>& row, int first, int n
     if (found < top) last = 1;
     // their elements that are as large as the last one's, at most 32 x 16
     int count = 0;
+#pragma unroll 4
     for (int e0 = 0; e0 < found * N; e0 += 32) {
         const int e = e0 + lane, u = first + (e < found * N ? sh.unit[e / N] : 0);
         const long long i = row.first(u) + e % N;
@@ -361,18 +367,63 @@ __device__ __forceinline__ void search_units(const Row<T>& row, int first, int n
         const bool in = k != 0 && k >= last;
         const unsigned who = __ballot_sync(0xffffffffu, in);
         if (in) {
-            const int slot = count + __popc(who & ((1u << lane) - 1));
-            sh.candidate_key[slot] = k;
-            sh.candidate_index[slot] = static_cast<int>(i);
+            sh.candidate[count + __popc(who & ((1u << lane) - 1))] = candidate(k, i);
         }
         count += __popc(who);
     }
     __syncwarp();
-    place<32>(sh.candidate_key, sh.candidate_index, count, top, sh.key, sh.index);
+    place<32>(sh.candidate, count, top, sh.best);
     __syncwarp();
 }
 
-// The block's alternatives among its units [0, n) (unit 0 is unit `first` of the row), from the units' maxima, into sh.key and sh.index.
+// The top-th largest of the groups' maxima, as the threshold: one warp takes the largest away, as often.
+__device__ __forceinline__ void largest_groups(int top, Shared& sh) {
+    const int tid = threadIdx.x;
+    if (tid >= 32) return;
+    constexpr int kMine = kGroups / 32;
+    uint32_t group[kMine], most = 0;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) group[j] = sh.group[j * 32 + tid];
+    for (int k = 0; k < top; ++k) {
+        uint32_t mine = group[0];
+#pragma unroll
+        for (int j = 1; j < kMine; ++j) mine = max(mine, group[j]);
+        most = __reduce_max_sync(0xffffffffu, mine);
+        const bool owner = tid == __ffs(__ballot_sync(0xffffffffu, mine == most)) - 1;
+        bool gone = !owner;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j)
+            if (!gone && group[j] == most) group[j] = 0, gone = true;
+    }
+    if (tid == 0) sh.threshold = max(most, 1u);  // (fewer groups than alternatives: whatever exists)
+}
+
+// Fewer candidates, where there are many: those that are at least the top-th largest among the maxima of 128 groups of them.
+template <int kThreads>
+__device__ __forceinline__ void refine(int top, Shared& sh) {
+    const int tid = threadIdx.x, count = sh.candidates;
+    if (count <= 2 * kMaxTop + 32) return;
+    for (int g = tid; g < kGroups; g += kThreads) {
+        uint64_t most = 0;
+        for (int c = g; c < count; c += kGroups) most = max(most, sh.candidate[c]);
+        sh.group[g] = static_cast<uint32_t>(most >> 32);
+    }
+    constexpr int kMine = kCandidates / kThreads;
+    uint64_t mine[kMine];
+#pragma unroll
+    for (int c = 0; c < kMine; ++c) mine[c] = c * kThreads + tid < count ? sh.candidate[c * kThreads + tid] : 0;
+    block_sync<kThreads>();
+    if (tid == 0) sh.candidates = 0;
+    largest_groups(top, sh);
+    block_sync<kThreads>();
+    const uint32_t threshold = sh.threshold;
+#pragma unroll
+    for (int c = 0; c < kMine; ++c)
+        if (static_cast<uint32_t>(mine[c] >> 32) >= threshold) sh.candidate[atomicAdd(&sh.candidates, 1)] = mine[c];
+    block_sync<kThreads>();
+}
+
+// The block's alternatives among its units [0, n) (unit 0 is unit `first` of the row), from the units' maxima, into sh.best.
 template <typename T, int kThreads>
 __device__ __forceinline__ void search(const Row<T>& row, int first, int n, int top, uint32_t* maxima, Shared& sh) {
     constexpr int N = Elements<T>::N;
@@ -383,23 +434,10 @@ __device__ __forceinline__ void search(const Row<T>& row, int first, int n, int 
         for (int u = g * per; u < min(n, (g + 1) * per); ++u) best = max(best, maxima[u]);
         sh.group[g] = best;
     }
-    if (tid < kMaxTop) sh.key[tid] = 0, sh.index[tid] = 0;
+    if (tid < kMaxTop) sh.best[tid] = 0;
     if (tid == 0) sh.units = sh.candidates = 0;
     block_sync<kThreads>();
-    if constexpr (kThreads == 32) {  // (a warp would be 128 x 128 comparisons about it)
-        search_units(row, first, n, per, top, maxima, sh);
-    } else {
-    for (int g = tid; g < kGroups; g += kThreads) {
-        const uint32_t k = sh.group[g];
-        int before = 0;
-#pragma unroll 8
-        for (int o = 0; o < kGroups / 4; ++o) {
-            const uint4 v = reinterpret_cast<const uint4*>(sh.group)[o];
-            before += (v.x > k) + (v.y > k) + (v.z > k) + (v.w > k);
-            before += (v.x == k && 4 * o < g) + (v.y == k && 4 * o + 1 < g) + (v.z == k && 4 * o + 2 < g) + (v.w == k && 4 * o + 3 < g);
-        }
-        if (before == top - 1) sh.threshold = max(k, 1u);  // (fewer groups than alternatives: whatever exists)
-    }
+    largest_groups(top, sh);
     block_sync<kThreads>();
     const uint32_t threshold = sh.threshold;
     for (int u = tid; u < n; u += kThreads)
@@ -416,42 +454,48 @@ __device__ __forceinline__ void search(const Row<T>& row, int first, int n, int 
             const uint32_t k = row.has(i) ? order_key(Elements<T>::load(row.at(u) + e % N)) : 0;
             if (k >= threshold) {
                 const int slot = atomicAdd(&sh.candidates, 1);
-                if (slot < kCandidates) {
-                    sh.candidate_key[slot] = k;
-                    sh.candidate_index[slot] = static_cast<int>(i);
-                }
+                if (slot < kCandidates) sh.candidate[slot] = candidate(k, i);
             }
         }
     }
     block_sync<kThreads>();
-    if (units <= kChosen && sh.candidates <= kCandidates) {
-        place<kThreads>(sh.candidate_key, sh.candidate_index, sh.candidates, top, sh.key, sh.index);
+    const bool listed = units <= kChosen && sh.candidates <= kCandidates;
+    block_sync<kThreads>();
+    if (listed) {
+        refine<kThreads>(top, sh);
+        place<kThreads>(sh.candidate, sh.candidates, top, sh.best);
     } else if (tid < 32) {
         search_units(row, first, n, per, top, maxima, sh);
     }
     block_sync<kThreads>();
-    }
 }
 
 struct ForwardParams {
     const void* logits;
     const long long* targets;
     long long rows, pitch;
-    int vocab, top, cluster;
+    int vocab, top, cluster, share;  // share: room for maxima
     float *log_probs, *entropy, *stats, *top_log_probs;
     long long* top_indices;
 };
 
 // A row to a block, or to a cluster of blocks that take equal runs of its units and meet in the first one's shared memory.
-template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const ForwardParams P) {
+// kFlight units of a thread are in flight: four where there are few rows, and latency counts (1 x 131072 fp32 9.4 -> 7.3 us); with two, of many rows more
+// warps fit an SM (16384 x 32768 fp16 212 -> 189 us).
+template <typename T, int kThreads, int kFlight>
+__global__ void __launch_bounds__(kThreads == 32 ? 32 * kWarpRows : kThreads) token_log_probs_kernel(const ForwardParams P) {
     pdl_enter();
     namespace cg = cooperative_groups;
-    __shared__ __align__(16) Shared sh;
-    extern __shared__ uint32_t maxima[];
+    constexpr int kRows = kThreads == 32 ? kWarpRows : 1;
+    __shared__ __align__(16) Shared all[kRows];
+    extern __shared__ uint32_t all_maxima[];
+    Shared& sh = all[kRows > 1 ? threadIdx.y : 0];
+    uint32_t* const maxima = all_maxima + (kRows > 1 ? threadIdx.y * P.share : 0);
     const int rank = P.cluster > 1 ? static_cast<int>(blockIdx.x % P.cluster) : 0;
     const int tid = threadIdx.x;
-    for (long long r = blockIdx.x / P.cluster; r < P.rows; r += gridDim.x / P.cluster) {
+    const long long r0 = kRows > 1 ? static_cast<long long>(blockIdx.x) * kRows + threadIdx.y : blockIdx.x / P.cluster;
+    const long long step = kRows > 1 ? static_cast<long long>(gridDim.x) * kRows : gridDim.x / P.cluster;
+    for (long long r = r0; r < P.rows; r += step) {
         const Row<T> row(static_cast<const T*>(P.logits) + r * P.pitch, P.vocab);
         const int share = (row.units + P.cluster - 1) / P.cluster;
         const int u0 = min(row.units, rank * share), u1 = min(row.units, u0 + share);
@@ -462,18 +506,25 @@ __global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const Forward
         };
         const int f0 = max(u0, row.full0), f1 = min(u1, row.full1);
         int u = f0 + tid;
-        for (; u + kThreads < f1; u += 2 * kThreads) {
-            uint32_t a[8], b[8];
-            load_unit(row.at(u), a);
-            load_unit(row.at(u + kThreads), b);
-            take(u, a);
-            take(u + kThreads, b);
+        long long target = tid == 0 ? load_index(P.targets + r) : -1;
+        for (; u + (kFlight - 1) * kThreads < f1; u += kFlight * kThreads) {
+            uint32_t v[kFlight][8];
+#pragma unroll
+            for (int e = 0; e < kFlight; ++e) load_unit(row.at(u + e * kThreads), v[e]);
+#pragma unroll
+            for (int e = 0; e < kFlight; ++e) take(u + e * kThreads, v[e]);
         }
         if (u < f1) {
-            uint32_t a[8];
-            load_unit(row.at(u), a);
-            take(u, a);
+            uint32_t v[kFlight - 1][8];
+#pragma unroll
+            for (int e = 0; e < kFlight - 1; ++e)
+                if (u + e * kThreads < f1) load_unit(row.at(u + e * kThreads), v[e]);
+#pragma unroll
+            for (int e = 0; e < kFlight - 1; ++e)
+                if (u + e * kThreads < f1) take(u + e * kThreads, v[e]);
         }
+        // (asked for before the sums are exchanged, needed behind them)
+        const float of_target = target >= 0 && target < P.vocab ? Elements<T>::load(static_cast<const T*>(P.logits) + r * P.pitch + target) : 0.f;
         // the first and the last unit, where they have gaps
         if (tid < 2) {
             const int e = tid == 0 ? 0 : row.units - 1;
@@ -494,8 +545,6 @@ __global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const Forward
             block_sync<kThreads>();
             search<T, kThreads>(row, u0, u1 - u0, P.top, maxima, sh);
         }
-        uint32_t key = 0;
-        int index = 0;
         if (P.cluster > 1) {
             cg::cluster_group cluster = cg::this_cluster();
             if (tid == 0) sh.block = a;
@@ -504,38 +553,24 @@ __global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const Forward
                 if (tid < 32) a = merge_lanes<T>(*cluster.map_shared_rank(&sh.block, tid % P.cluster), P.cluster);
                 if (P.top) {
                     const int count = P.cluster * P.top;
-                    for (int e = tid; e < count; e += kThreads) {
-                        sh.candidate_key[e] = cluster.map_shared_rank(sh.key, e / P.top)[e % P.top];
-                        sh.candidate_index[e] = cluster.map_shared_rank(sh.index, e / P.top)[e % P.top];
-                    }
+                    for (int e = tid; e < count; e += kThreads) sh.candidate[e] = cluster.map_shared_rank(sh.best, e / P.top)[e % P.top];
                     __syncthreads();
-                    place<kThreads>(sh.candidate_key, sh.candidate_index, count, P.top, sh.key, sh.index);
+                    place<kThreads>(sh.candidate, count, P.top, sh.best);
                     __syncthreads();
                 }
             }
-        }
-        if (P.top && tid < P.top) {
-            key = sh.key[tid];
-            index = sh.index[tid];
         }
         if (rank == 0 && tid < 32) {
             const bool dead = a.m == -INFINITY, bad = !(a.m < INFINITY);  // nothing but -inf; a NaN or +inf
             const float off = extreme<T>(a.m) ? 0.f : fmaf(a.m, kLog2e, -reference<T>(a.m));  // of the reference, from m log2 e
             const float log_sum = dead ? 0.f : bad ? NAN : logf(a.s) - off * kLn2;
             if (tid < P.top) {
-                P.top_indices[r * P.top + tid] = index;
-                P.top_log_probs[r * P.top + tid] = dead ? -INFINITY : (key_value(key) - a.m) - log_sum;
+                const uint64_t c = sh.best[tid];
+                P.top_indices[r * P.top + tid] = index_of(c);
+                P.top_log_probs[r * P.top + tid] = dead ? -INFINITY : (value_of(c) - a.m) - log_sum;
             }
             if (tid == 0) {
-                const long long target = load_index(P.targets + r);
-                float lp = 0.f;
-                if (target >= P.vocab) {
-                    lp = NAN;
-                } else if (target >= 0) {
-                    const float x = Elements<T>::load(static_cast<const T*>(P.logits) + r * P.pitch + target);
-                    lp = dead ? -INFINITY : (x - a.m) - log_sum;
-                }
-                P.log_probs[r] = lp;
+                P.log_probs[r] = target < 0 ? 0.f : target >= P.vocab ? NAN : dead ? -INFINITY : (of_target - a.m) - log_sum;
                 P.entropy[r] = dead ? 0.f : bad ? NAN : logf(a.s) - kLn2 * (a.t / a.s);
                 P.stats[2 * r] = a.m;
                 P.stats[2 * r + 1] = log_sum;
@@ -555,13 +590,14 @@ struct BackwardParams {
     bool together;  // rows of the logits and of the result start at the same place of a unit
 };
 
-// A block to a run of a row's units.
-template <typename T>
+// A block to a run of a row's units, or to several short rows (blockDim.y).
+template <typename T, bool kShort>
 __global__ void __launch_bounds__(256) token_log_probs_backward_kernel(const BackwardParams P) {
     pdl_enter();
     constexpr int N = Elements<T>::N;
-    const long long r = blockIdx.x / P.blocks_per_row;
-    const int part = static_cast<int>(blockIdx.x % P.blocks_per_row);
+    const long long r = kShort ? static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y : blockIdx.x / P.blocks_per_row;
+    if (kShort && r >= P.rows) return;
+    const int part = kShort ? 0 : static_cast<int>(blockIdx.x % P.blocks_per_row);
     const Row<T> row(static_cast<const T*>(P.logits) + r * P.pitch, P.vocab);
     T* const out = static_cast<T*>(P.out) + r * P.out_pitch;
     const float m = load_global(P.stats + 2 * r), log_sum = load_global(P.stats + 2 * r + 1);
@@ -576,7 +612,7 @@ __global__ void __launch_bounds__(256) token_log_probs_backward_kernel(const Bac
     const float slope = -gh * kLn2, level = -fmaf(gh, h, g);
     const uint64_t slope2 = pack2(slope, slope), level2 = pack2(level, level);
     const bool entropy = P.d_entropy != nullptr;
-    for (int u = part * blockDim.x + threadIdx.x; u < row.units; u += P.blocks_per_row * blockDim.x) {
+    for (int u = part * blockDim.x + threadIdx.x; u < row.units; u += (kShort ? 1 : P.blocks_per_row) * blockDim.x) {
         const bool full = u >= row.full0 && u < row.full1;
         uint32_t v[8];
         if (full) load_unit(row.at(u), v); else row.load_broken(u, v);
@@ -621,7 +657,8 @@ __global__ void __launch_bounds__(256) token_log_probs_backward_kernel(const Bac
 }
 
 struct ForwardPlan {
-    int threads = 0, cluster = 1;
+    int threads = 0, cluster = 1, flight = 2;
+    int share = 0;
     size_t smem = 0;
     bool ok = false;
 };
@@ -629,18 +666,23 @@ static ForwardPlan forward_plan(long long rows, int vocab, int dtype, int top) {
     const int n = dtype == NML_F16 ? Elements<__half>::N : Elements<float>::N;
     const int units = static_cast<int>((static_cast<long long>(vocab) + 2 * n - 2) / n);  // at the worst start of a row
     ForwardPlan p;
+    // A warp to a short row, four to others, eight to the longest; these over several blocks where there are few rows.
     p.threads = units <= 128 ? 32 : units <= 4096 ? 128 : 256;
-    while (p.cluster < kMaxCluster && p.threads == 256 && (rows * p.cluster < 148 || (top && (units + p.cluster - 1) / p.cluster > kMaxUnits))) p.cluster *= 2;
-    const int share = (units + p.cluster - 1) / p.cluster;
-    p.ok = !top || share <= kMaxUnits;
-    p.smem = top ? sizeof(uint32_t) * static_cast<size_t>(share) : 0;
+    if (units > 1024 && rows < 74) p.threads = 256;
+    while (p.cluster < kMaxCluster && p.threads == 256 && ((rows * p.cluster < 148 && units > 512 * p.cluster) || (top && (units + p.cluster - 1) / p.cluster > kMaxUnits))) p.cluster *= 2;
+    if (rows * p.cluster <= 148) p.flight = 4;
+    p.share = (units + p.cluster - 1) / p.cluster;
+    p.ok = !top || p.share <= kMaxUnits;
+    p.smem = top ? sizeof(uint32_t) * p.share * (p.threads == 32 ? kWarpRows : 1) : 0;
     return p;
 }
 typedef void (*ForwardKernel)(const ForwardParams);
-static ForwardKernel forward_kernel(int dtype, int threads) {
-    if (dtype == NML_F16) return threads == 32 ? token_log_probs_kernel<__half, 32> : threads == 128 ? token_log_probs_kernel<__half, 128> : token_log_probs_kernel<__half, 256>;
-    return threads == 32 ? token_log_probs_kernel<float, 32> : threads == 128 ? token_log_probs_kernel<float, 128> : token_log_probs_kernel<float, 256>;
+template <typename T>
+static ForwardKernel forward_kernel_of(const ForwardPlan& p) {
+    return p.threads == 32 ? token_log_probs_kernel<T, 32, 4> : p.threads == 128 ? token_log_probs_kernel<T, 128, 2>
+           : p.flight == 4 ? token_log_probs_kernel<T, 256, 4> : token_log_probs_kernel<T, 256, 2>;
 }
+static ForwardKernel forward_kernel(int dtype, const ForwardPlan& p) { return dtype == NML_F16 ? forward_kernel_of<__half>(p) : forward_kernel_of<float>(p); }
 
 static bool shape_ok(const void* logits, int dtype, long long rows, int vocab, long long pitch) {
     if (!logits || (dtype != NML_F16 && dtype != NML_F32) || rows <= 0 || vocab <= 0 || pitch < vocab) return false;
@@ -658,10 +700,17 @@ using namespace nml_logits;
 int nml::prepare_logits_kernels() {
     for (int dtype : {NML_F32, NML_F16})
         for (int threads : {32, 128, 256})
-            NMLG_CUDA(cudaFuncSetAttribute(forward_kernel(dtype, threads), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxUnits * 4));
+            for (int flight : {2, 4}) {
+                ForwardPlan p;
+                p.threads = threads;
+                p.flight = flight;
+                NMLG_CUDA(cudaFuncSetAttribute(forward_kernel(dtype, p), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxUnits * 4));
+            }
     cudaFuncAttributes a;
-    NMLG_CUDA(cudaFuncGetAttributes(&a, token_log_probs_backward_kernel<float>));
-    NMLG_CUDA(cudaFuncGetAttributes(&a, token_log_probs_backward_kernel<__half>));
+    NMLG_CUDA(cudaFuncGetAttributes(&a, token_log_probs_backward_kernel<float, true>));
+    NMLG_CUDA(cudaFuncGetAttributes(&a, token_log_probs_backward_kernel<float, false>));
+    NMLG_CUDA(cudaFuncGetAttributes(&a, token_log_probs_backward_kernel<__half, true>));
+    NMLG_CUDA(cudaFuncGetAttributes(&a, token_log_probs_backward_kernel<__half, false>));
     return NML_OK;
 }
 
@@ -677,10 +726,12 @@ int nml_token_log_probs(const void* logits, int dtype, long long rows, int vocab
     int* status;
     int sms;
     if (const int rc = nml::current_device(&status, &sms)) return rc;
-    const ForwardParams P = {logits, targets, rows, pitch, vocab, top, plan.cluster, log_probs, entropy, stats, top_log_probs, top_indices};
-    const long long blocks = rows * plan.cluster, most = static_cast<long long>(sms) * 32 / plan.cluster * plan.cluster;
+    const ForwardParams P = {logits, targets, rows, pitch, vocab, top, plan.cluster, plan.share, log_probs, entropy, stats, top_log_probs, top_indices};
+    const bool warps = plan.threads == 32;
+    const long long blocks = warps ? (rows + kWarpRows - 1) / kWarpRows : rows * plan.cluster, most = static_cast<long long>(sms) * 32 / plan.cluster * plan.cluster;
     const int grid = static_cast<int>(blocks < most ? blocks : most);
-    nml::launch_with(nml::overlaps(grid, nml::kSms), plan.cluster, forward_kernel(dtype, plan.threads), grid, plan.threads, plan.smem,
+    nml::launch_with(nml::overlaps(grid, nml::kSms), plan.cluster, forward_kernel(dtype, plan), grid, warps ? dim3(32, kWarpRows) : dim3(plan.threads),
+                     plan.smem,
                      static_cast<cudaStream_t>(stream), P);
     NMLG_CUDA(cudaGetLastError());
     nml::count_launches(1);
@@ -705,9 +756,14 @@ int nml_token_log_probs_backward(const void* logits, int dtype, long long rows, 
                           (pitch - d_pitch) * size % kUnitBytes == 0;
     const BackwardParams P = {logits, targets, stats, entropy, d_log_probs, d_entropy, d_logits, rows, pitch, d_pitch, vocab,
                               static_cast<int>(per_row), together};
-    const int threads = units >= 256 ? 256 : static_cast<int>((units + 31) / 32 * 32);
-    nml::launch(dtype == NML_F16 ? token_log_probs_backward_kernel<__half> : token_log_probs_backward_kernel<float>,
-                static_cast<unsigned>(rows * per_row), threads, 0, static_cast<cudaStream_t>(stream), P);
+    // A power of two of threads to a row, up to two units each where it is short, 256 to a block.
+    int threads = 8;
+    while (threads < 256 && 2 * threads < units) threads *= 2;
+    const dim3 block(threads, 256 / threads);
+    const long long blocks = (rows + block.y - 1) / block.y * per_row;
+    nml::launch(dtype == NML_F16 ? (threads < 256 ? token_log_probs_backward_kernel<__half, true> : token_log_probs_backward_kernel<__half, false>)
+                                 : (threads < 256 ? token_log_probs_backward_kernel<float, true> : token_log_probs_backward_kernel<float, false>),
+                static_cast<unsigned>(blocks), block, 0, static_cast<cudaStream_t>(stream), P);
     NMLG_CUDA(cudaGetLastError());
     nml::count_launches(1);
     return NML_OK;
