@@ -305,7 +305,7 @@ typedef struct nml_matrix {
     long long in_row, in_col, out_row, out_col; /* strides */
 } nml_matrix;
 int nml_orthogonalize_workspace_size(const nml_matrix* matrices, int count, int math, int steps, size_t* bytes);
-int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int out_dtype, int math, int steps, const float* coefficients,
+int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int out_dtype, int math, int steps, const double* coefficients,
                       float eps, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Optimizer step with such updates, in place on dense fp32 parameters:
@@ -323,7 +323,7 @@ typedef struct nml_muon_param {
     float scale;
 } nml_muon_param;
 int nml_muon_workspace_size(const nml_muon_param* params, int count, int math, int steps, size_t* bytes);
-int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, const float* coefficients, float eps, float lr, float momentum,
+int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, const double* coefficients, float eps, float lr, float momentum,
                   int nesterov, float weight_decay, float inv_scale, const int* found_inf, void* workspace, size_t workspace_bytes, void* stream);
 long long nml_layers_launch_count(void);
 

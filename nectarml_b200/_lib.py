@@ -83,9 +83,9 @@ SYMBOLS = {
     "nml_grads_check": (_I, [_VP, _SZ, C.c_float, _VP, _VP]),
     "nml_sgd_momentum_step": (_I, [_VP, _VP, _VP, _VP, _SZ, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, _VP, _VP]),
     "nml_orthogonalize_workspace_size": (_I, [C.POINTER(Matrix), _I, _I, _I, C.POINTER(_SZ)]),
-    "nml_orthogonalize": (_I, [C.POINTER(Matrix), _I, _I, _I, _I, _I, C.POINTER(C.c_float), C.c_float, _VP, _SZ, _VP]),
+    "nml_orthogonalize": (_I, [C.POINTER(Matrix), _I, _I, _I, _I, _I, C.POINTER(C.c_double), C.c_float, _VP, _SZ, _VP]),
     "nml_muon_workspace_size": (_I, [C.POINTER(MuonParam), _I, _I, _I, C.POINTER(_SZ)]),
-    "nml_muon_step": (_I, [C.POINTER(MuonParam), _I, _I, _I, C.POINTER(C.c_float), C.c_float, C.c_float, C.c_float, _I, C.c_float, C.c_float,
+    "nml_muon_step": (_I, [C.POINTER(MuonParam), _I, _I, _I, C.POINTER(C.c_double), C.c_float, C.c_float, C.c_float, _I, C.c_float, C.c_float,
                            _VP, _VP, _SZ, _VP]),
     "nml_profile_begin": (_I, [_I]),
     "nml_profile_end": (_I, [C.POINTER(C.c_float), _I, C.POINTER(_I)]),

@@ -38,6 +38,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -1002,6 +1003,10 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
     }
 }
 
+}  // namespace nml_ortho
+#include "nml_ortho_small.cuh"
+namespace nml_ortho {
+
 // ---------------------------------------------------------------- parameters that are no matrices --
 constexpr int kVectors = 128;
 struct Vector {
@@ -1057,7 +1062,7 @@ struct Polynomial {
 static int exponent_below(double bound) {  // largest e with bound * 2^e <= 2^15
     return std::max(-24, std::min(24, static_cast<int>(floor(log2(32768.0 / std::max(bound, 1e-6))))));
 }
-static bool polynomial(const float* coefficients, int steps, bool chained, Polynomial* p) {
+static bool polynomial(const double* coefficients, int steps, bool chained, Polynomial* p) {
     constexpr int kPoints = 128;        // singular values, at which the matrices' eigenvalues are followed
     constexpr double kBetween = 1.01;   // and what lies between two of them
     double l = kBetween, lambda[kPoints + 1], q[kPoints + 1], growth = 1.0;
@@ -1243,16 +1248,70 @@ static void launch_pack(const PackParams<kMaxRounds>& all, const Call& call, int
 }
 constexpr int kFewRounds = 20;
 
+// Whether a group goes through double precision: see nml_ortho_small.cuh.
+static bool all_small(const Work* w, int count) {
+    return std::all_of(w, w + count, [](const Work& v) { return v.s.m <= kSmall; });
+}
+struct SmallPlan {
+    int partials = 0, chunks = 0;
+    size_t sums_at = 0, q_at = 0, bytes = 0;
+};
+static SmallPlan plan_small(Work* w, int count) {
+    SmallPlan p;
+    for (int k = 0; k < count; ++k) {
+        const int chunks = (w[k].s.n + 63) / 64, most = std::min(chunks, kSmallPartials), per = (chunks + most - 1) / most;
+        w[k].first_sum = p.partials;
+        w[k].sums = (chunks + per - 1) / per;
+        p.partials += w[k].sums;
+        w[k].first_half = p.chunks;
+        p.chunks += chunks;
+    }
+    p.sums_at = round_up(sizeof(Work) * kGroup, 256);
+    p.q_at = p.sums_at + sizeof(double) * kSmall * kSmall * p.partials;
+    p.bytes = p.q_at + sizeof(double) * kSmall * kSmall * count;
+    return p;
+}
+constexpr size_t kSmallStepsSmem = 5 * sizeof(double) * kSmall * kSmallPitch, kSmallResultSmem = 2 * sizeof(double) * kSmall * kSmallPitch;
+
 // The polynomials of the two classes.
 struct Steps {
     Polynomial of[kClasses];
 };
-static bool steps_of(const float* coefficients, int steps, Steps* s) {
+static bool steps_of(const double* coefficients, int steps, Steps* s) {
     return polynomial(coefficients, steps, true, &s->of[0]) && polynomial(coefficients, steps, false, &s->of[1]);
+}
+
+static int run_small(Work* w, int count, const Call& call, const Polynomial& poly, void* workspace, size_t bytes, cudaStream_t st) {
+    int* err;
+    int sms;
+    if (const int rc = nml::current_device(&err, &sms)) return rc;  // (sets the device up)
+    const SmallPlan p = plan_small(w, count);
+    uint8_t* const base = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<uintptr_t>(workspace), 1024));
+    if (!workspace || base + p.bytes > static_cast<uint8_t*>(workspace) + bytes) return NML_ERR_WORKSPACE;
+    const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), nullptr, nullptr, nullptr, call.skip, count};
+    double* const q = reinterpret_cast<double*>(base + p.q_at);
+    const bool half = call.in_dtype == NML_F16;
+    auto gram = [&](auto n) {
+        constexpr int N = decltype(n)::value;
+        Group<N> g;
+        std::copy(w, w + count, g.w);
+        nml::launch(half ? small_gram_kernel<N, __half> : small_gram_kernel<N, float>, p.partials, 256, 0, st, g, c, call.mo);
+    };
+    if (count <= 8) gram(std::integral_constant<int, 8>());
+    else gram(std::integral_constant<int, kGroup>());
+    SmallSteps s = {c, q, call.eps, poly.steps, {}, {}, {}};
+    for (int k = 0; k < poly.steps; ++k) s.a[k] = poly.step[k].a, s.b[k] = poly.step[k].b, s.k[k] = poly.step[k].c;
+    nml::launch(small_steps_kernel, count, 256, kSmallStepsSmem, st, s);
+    const SmallResult r = {c, q, call.mo, call.out_dtype == NML_F16, call.apply, call.keep, call.rate};
+    nml::launch(half ? small_result_kernel<__half> : small_result_kernel<float>, p.chunks, 256, kSmallResultSmem, st, r);
+    NMLO_CUDA(cudaGetLastError());
+    nml::count_launches(3);
+    return NML_OK;
 }
 
 // One group: three launches.
 static int run_group(Work* w, int count, const Call& call, const Steps& steps, void* workspace, size_t bytes, cudaStream_t st) {
+    if (all_small(w, count)) return run_small(w, count, call, steps.of[1], workspace, bytes, st);
     int* err;
     int sms;
     if (const int rc = nml::current_device(&err, &sms)) return rc;
@@ -1357,7 +1416,7 @@ static int workspace_of(int count, int math, int steps, F&& size, size_t* bytes)
     int sms = nml::usable_sms(), filled = 0;
     for (int k = 0; k <= count; ++k) {
         if (filled == kGroup || (k == count && filled > 0)) {
-            *bytes = std::max(*bytes, plan_group(w, filled, math, steps, sms).bytes + 1024);
+            *bytes = std::max(*bytes, (all_small(w, filled) ? plan_small(w, filled).bytes : plan_group(w, filled, math, steps, sms).bytes) + 1024);
             filled = 0;
         }
         if (k < count) {
@@ -1380,7 +1439,11 @@ int nml::prepare_ortho_kernels() {
         NMLO_CUDA(cudaFuncGetAttributes(&a, f));
         if (a.numRegs != kLaunchRegs) return NML_ERR_UNSUPPORTED;  // (a build whose register split would not hold)
     }
-    const void* others[] = {(const void*)ortho_sums_kernel<8, float>, (const void*)ortho_sums_kernel<8, __half>,
+    NMLO_CUDA(cudaFuncSetAttribute(small_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmallStepsSmem)));
+    NMLO_CUDA(cudaFuncSetAttribute(small_result_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmallResultSmem)));
+    NMLO_CUDA(cudaFuncSetAttribute(small_result_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmallResultSmem)));
+    const void* others[] = {(const void*)small_gram_kernel<8, float>, (const void*)small_gram_kernel<8, __half>,
+                            (const void*)small_gram_kernel<kGroup, float>, (const void*)small_gram_kernel<kGroup, __half>, (const void*)ortho_sums_kernel<8, float>, (const void*)ortho_sums_kernel<8, __half>,
                             (const void*)ortho_sums_kernel<kGroup, float>, (const void*)ortho_sums_kernel<kGroup, __half>,
                             (const void*)ortho_pack_kernel<kFewRounds, float>, (const void*)ortho_pack_kernel<kFewRounds, __half>,
                             (const void*)ortho_pack_kernel<kMaxRounds, float>, (const void*)ortho_pack_kernel<kMaxRounds, __half>,
@@ -1398,7 +1461,7 @@ int nml_orthogonalize_workspace_size(const nml_matrix* matrices, int count, int 
     return workspace_of(count, math, steps, [&](int k, Source& s) { return set_sizes(s, matrices[k].rows, matrices[k].cols), true; }, bytes);
 }
 
-int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int out_dtype, int math, int steps, const float* coefficients,
+int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int out_dtype, int math, int steps, const double* coefficients,
                       float eps, void* workspace, size_t workspace_bytes, void* stream) {
     size_t need = 0;
     if (const int rc = nml_orthogonalize_workspace_size(matrices, count, math, steps, &need)) return rc;
@@ -1442,7 +1505,7 @@ int nml_muon_workspace_size(const nml_muon_param* params, int count, int math, i
     return workspace_of(count, math, steps, [&](int k, Source& s) { return params[k].rows > 0 && (set_sizes(s, params[k].rows, params[k].cols), true); }, bytes);
 }
 
-int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, const float* coefficients, float eps, float lr, float momentum,
+int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, const double* coefficients, float eps, float lr, float momentum,
                   int nesterov, float weight_decay, float inv_scale, const int* found_inf, void* workspace, size_t workspace_bytes, void* stream) {
     size_t need = 0;
     if (const int rc = nml_muon_workspace_size(params, count, math, steps, &need)) return rc;

@@ -1101,10 +1101,10 @@ struct Items {
     PyObject* operator[](Py_ssize_t k) const { return PySequence_Fast_GET_ITEM(fast, k); }
 };
 // The polynomial's coefficients: a flat sequence of three numbers for each step.
-std::vector<float> coefficients_of(PyObject* o) {
+std::vector<double> coefficients_of(PyObject* o) {
     const Items items(o, "coefficients: a sequence of numbers");
-    std::vector<float> c;
-    for (Py_ssize_t k = 0; k < items.size(); ++k) c.push_back(static_cast<float>(as_double(items[k])));
+    std::vector<double> c;
+    for (Py_ssize_t k = 0; k < items.size(); ++k) c.push_back(as_double(items[k]));
     require(!c.empty() && c.size() % 3 == 0, "three coefficients for each step");
     return c;
 }
@@ -1130,7 +1130,7 @@ PyObject* py_orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Items in(a[0], "matrices: a sequence of tensors");
         const long out_code = as_int(a[2]);
         const int math = static_cast<int>(as_int(a[3]));
-        const std::vector<float> c = coefficients_of(a[4]);
+        const std::vector<double> c = coefficients_of(a[4]);
         const float eps = static_cast<float>(as_double(a[5]));
         const char* const kStrides = "matrices with one dense dimension";
         std::vector<nml_matrix> list;
@@ -1202,7 +1202,7 @@ PyObject* py_muon_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 "one gradient, momentum and half copy for each parameter");
         const long scaling = as_int(a[4]);
         const int math = static_cast<int>(as_int(a[5]));
-        const std::vector<float> c = coefficients_of(a[6]);
+        const std::vector<double> c = coefficients_of(a[6]);
         const float eps = static_cast<float>(as_double(a[7])), lr = static_cast<float>(as_double(a[8]));
         const float momentum = static_cast<float>(as_double(a[9])), decay = static_cast<float>(as_double(a[11]));
         const float inv_scale = static_cast<float>(as_double(a[12]));

@@ -44,7 +44,7 @@ def test_workspace_size(lib):
 def _call(lib, inp=P, out=P, rows=4, cols=6, in_row=6, in_col=1, out_row=6, out_col=1, in_dtype=0, out_dtype=0, math=_lib.NML_MATH_3XF16,
           steps=5, coef=COEF * 5, eps=1e-7, ws=None, ws_bytes=0):
     m = _lib.Matrix(inp, out, rows, cols, in_row, in_col, out_row, out_col)
-    c = None if coef is None else (C.c_float * len(coef))(*coef)
+    c = None if coef is None else (C.c_double * len(coef))(*coef)
     return lib.nml_orthogonalize(C.byref(m), 1, in_dtype, out_dtype, math, steps, c, eps, ws, ws_bytes, None)
 
 
@@ -68,7 +68,7 @@ def test_missing_workspace(lib):
 
 def _muon(lib, params, steps=5, coef=COEF * 5, eps=1e-7, found=None):
     p = (_lib.MuonParam * len(params))(*[_lib.MuonParam(*v) for v in params])
-    c = None if coef is None else (C.c_float * len(coef))(*coef)
+    c = None if coef is None else (C.c_double * len(coef))(*coef)
     return lib.nml_muon_step(p, len(params), _lib.NML_MATH_3XF16, steps, c, eps, 0.1, 0.9, 1, 0.0, 1.0, found, None, 0, None)
 
 
