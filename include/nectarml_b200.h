@@ -297,7 +297,8 @@ int nml_sgd_momentum_step(float* params, const float* grads, float* velocity, vo
  *  NML_MATH_F16    operands rounded to fp16, except X where it is carried to the next step: 2 to 3e-3 of the result's norm
  * Zeros stay zeros; a matrix with a NaN or an infinity becomes NaN.  Matrices may be views: one of the strides (in elements) is 1, the other at least
  * the length of the dense run; a result may lie where its matrix does but must not overlap another one.  Coefficients under which a singular value could
- * grow beyond 64 are NML_ERR_UNSUPPORTED.  Results are bitwise repeatable and do not depend on the group. */
+ * grow beyond 64 are NML_ERR_UNSUPPORTED.  Results are bitwise repeatable; the
+ * order of sums, and whether a short side up to 64 is taken in double, follow from the group's sizes and the SMs in use. */
 typedef struct nml_matrix {
     const void* in;
     void* out;

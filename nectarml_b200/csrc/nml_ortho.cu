@@ -58,7 +58,7 @@ using nml::pdl_enter;
         if (e_ != cudaSuccess) return nml::cuda_failed(static_cast<int>(e_), #expr); \
     } while (0)
 
-constexpr int kGroup = 128;            // matrices of one run of launches
+constexpr int kGroup = 64;             // matrices of one run of launches
 constexpr int kMaxSteps = 32;
 constexpr int kBlock = 128;            // rows and columns of a block
 constexpr uint32_t kHalf = 16384;      // bytes of one half of a block
@@ -75,7 +75,8 @@ enum {
     POLY = 0,    // symmetric: A = D f0, and P = D f1 + d1 I beside it
     PLAIN = 1,   // symmetric: D f0 + d1 I
     ITERATE = 2, // X = D f1
-    RESULT = 3   // D f1 in the caller's layout, or the parameters' update
+    RESULT = 3,  // D f1 in the caller's layout, or the parameters' update
+    SUM = 4      // POLY of a matrix's partial products X X^T, which POLY left in fp32 where K is in several parts
 };
 struct Symmetric {  // buffers of one symmetric product
     int left, right, out;
@@ -89,11 +90,11 @@ struct Op {
     float f1, d1;
     int left;                  // ITERATE, RESULT: the symmetric factor
     uint32_t identity;         // "f16": block of this step's a I
-    int symmetric_before, wide_before;  // symmetric products and products Q X of the class in front of this one
+    int gram_before, symmetric_before, wide_before, sum_before;  // what of the class is in front of this one
 };
 // Matrices whose steps are chained and those whose steps are single run different products; a round is one product of each.
 constexpr int kClasses = 2;
-constexpr int kMaxRounds = 4 * kMaxSteps;
+constexpr int kMaxRounds = 5 * kMaxSteps;
 struct Round {
     int first, of_first;       // tiles of all rounds in front, of the first class in this one
     Op op[kClasses];
@@ -112,11 +113,13 @@ struct Source {
 // and as the launches after the first find it in the workspace.
 struct alignas(16) Work {
     Source s;
-    uint32_t x[2], sym;                 // first blocks of X's two copies and of the symmetric matrices, in blocks of two planes
+    uint32_t x[2], sym, partial;        // first blocks of X's two copies, the symmetric matrices and partial products, in blocks of two planes
     int mb, nb;                         // blocks along m and n
     int first_sum, sums;                // its partial sums of squares
-    int first_half, first_gram, first_update;  // its halves of X, tiles of the symmetric products, tiles of the update
-    int wide;                           // blocks of n to a tile of the update: 1 or 2
+    int first_half;                     // its halves of X
+    int first_gram, first_symmetric, first_update, first_parts;  // its tiles: of X X^T, symmetric products, Q X, SUM
+    int wide;                           // 64-column groups to a tile of Q X: 1, 2 or 4
+    int fine, parts;                    // tiles to a block of a symmetric product, 1 or 2; parts of K of X X^T
     float sx;                           // X is stored times this
     int chained;
 };
@@ -410,6 +413,12 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__
 }
 
 // ---------------------------------------------------------------- products --
+// What another block of the same grid has written: past the SM's own cache.
+__device__ __forceinline__ float4 load_shared_by_blocks(const float4* p) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(__cvta_generic_to_global(p)) : "memory");
+    return v;
+}
 __device__ __forceinline__ long long load_wide(const long long* p) {
     long long v;
     asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(__cvta_generic_to_global(p)));
@@ -484,8 +493,8 @@ constexpr int kQueue = 4;            // tiles that the producer may be ahead
 // (One product of halves, of 2^-12, does not need it.)
 
 struct Info {        // of a matrix
-    int m, n, nb, wide;
-    uint32_t x[2], sym;
+    int m, n, nb, wide, fine, parts;
+    uint32_t x[2], sym, partial;
     float sx;
 };
 // Thirty-two rows and columns of a result, from a warp's room in shared memory.
@@ -513,10 +522,11 @@ struct Tile {
     int k;           // matrix of the group; -1: no more tiles
     int i, j;        // its block row; its (first) block column
     int job;
-    int groups;      // 64-column groups of it
-    int slices;      // of 64 along K
+    int column;      // its first 64-column group in that block: 0 or 1
+    int groups;      // 64-column groups of it; 0: none that is in use
+    int part, from;  // of K, and its first slice
+    int slices;      // of 64 along K; 0: no product
     int extra;       // "f16" update: slices of a I times X's low half behind them
-    int unused;
     Info w;
     Op op;
 };
@@ -535,7 +545,7 @@ __device__ __forceinline__ int load_acquire(const int* p) {
 __device__ __forceinline__ void add_release(int* p, int v) {
     asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(__cvta_generic_to_global(p)), "r"(v) : "memory");
 }
-// Both directions, shared and global memory: what generic loads and stores did is seen by bulk copies, and the other way round.
+// What other blocks stored and this thread has acquired is seen by its bulk copies.
 __device__ __forceinline__ void fence_proxies() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
 template <int kPlanes>
@@ -545,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
         drain_bar;
     __shared__ __align__(8) int abort_state[4];
     __shared__ uint32_t tmem_base;
-    __shared__ int first_gram[kGroup], first_update[kGroup];
+    __shared__ int first[4][kGroup];  // of X X^T, symmetric products, Q X, SUM
     __shared__ __align__(16) Tile queue[kQueue];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -575,8 +585,10 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
     const bool skip = skipped(P.c.skip);
     const int count = P.c.count;
     for (int i = tid; i < count; i += kThreads) {
-        first_update[i] = load_global(&P.c.table[i].first_update);
-        first_gram[i] = load_global(&P.c.table[i].first_gram);
+        first[0][i] = load_global(&P.c.table[i].first_gram);
+        first[1][i] = load_global(&P.c.table[i].first_symmetric);
+        first[2][i] = load_global(&P.c.table[i].first_update);
+        first[3][i] = load_global(&P.c.table[i].first_parts);
     }
     nml::tc_fence_before();
     __syncthreads();
@@ -618,64 +630,64 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 const int word = lane < kOpWords ? load_global(words + lane) : 0;
                 const int kind = __shfl_sync(0xffffffffu, word, offsetof(Op, kind) / 4), jobs = __shfl_sync(0xffffffffu, word, offsetof(Op, jobs) / 4);
                 const int gram = __shfl_sync(0xffffffffu, word, offsetof(Op, gram) / 4);
-                const bool is_wide = kind >= ITERATE;
+                const bool is_wide = kind == ITERATE || kind == RESULT, whole = kind == POLY && gram;
                 // (matrices of the first class come first, and their tiles count from 0; those of the second behind all of the first)
                 const int n0 = P.first_class;
                 const int lo = cls ? n0 : 0, hi = cls ? count : n0;
-                const int* const first = is_wide ? first_update : first_gram;
-                const int base = first[lo], per_job = is_wide ? 1 : jobs;
+                const int* const starts = first[is_wide ? 2 : kind == SUM ? 3 : whole ? 0 : 1];
+                const int base = starts[lo], per_job = is_wide ? 1 : jobs;
                 int a = lo, b = hi - 1;
                 while (a < b) {
                     const int mid = (a + b + 1) / 2;
-                    if ((first[mid] - base) * per_job <= t) a = mid; else b = mid - 1;
+                    if ((starts[mid] - base) * per_job <= t) a = mid; else b = mid - 1;
                 }
                 tile.k = a;
-                t -= (first[a] - base) * per_job;
+                t -= (starts[a] - base) * per_job;
                 Info w;
                 {
                     const Work* const from = P.c.table + a;
                     auto word = [](const uint32_t* p) { return static_cast<uint32_t>(load_global(reinterpret_cast<const int*>(p))); };
-                    w = {load_global(&from->s.m), load_global(&from->s.n), load_global(&from->nb), load_global(&from->wide),
-                         {word(&from->x[0]), word(&from->x[1])}, word(&from->sym), load_global(&from->sx)};
+                    w = {load_global(&from->s.m), load_global(&from->s.n), load_global(&from->nb), load_global(&from->wide), load_global(&from->fine),
+                         load_global(&from->parts), {word(&from->x[0]), word(&from->x[1])}, word(&from->sym), word(&from->partial), load_global(&from->sx)};
                 }
                 const int mb = (w.m + kBlock - 1) / kBlock;
-                tile.extra = tile.job = 0;
+                const int blocks = lower(mb, 0), symmetric_tiles = blocks * w.fine, wide_groups = (w.n + 63) / 64, per_row = (wide_groups + w.wide - 1) / w.wide;
+                tile.extra = tile.job = tile.column = tile.part = tile.from = 0;
                 if (is_wide) {
-                    const int per = (w.nb + w.wide - 1) / w.wide;
-                    tile.i = t / per;
-                    tile.j = t % per * w.wide;
-                    tile.groups = min(2 * w.wide, (w.n - tile.j * kBlock + 63) / 64);
+                    tile.i = t / per_row;
+                    const int group = t % per_row * w.wide;
+                    tile.j = group >> 1;
+                    tile.column = group & 1;
+                    tile.groups = min(w.wide, wide_groups - group);
                     tile.slices = (w.m + 63) / 64;
                     if (kPlanes == 1) tile.extra = min(2, tile.slices - 2 * tile.i);
                 } else {
-                    if (t >= lower(mb, 0)) t -= lower(mb, 0), tile.job = 1;
+                    const int fine = kind == SUM ? 2 : w.fine;
+                    if (whole) {
+                        tile.part = t / symmetric_tiles;
+                        t %= symmetric_tiles;
+                    } else if (kind != SUM && t >= symmetric_tiles) {
+                        t -= symmetric_tiles;
+                        tile.job = 1;
+                    }
+                    if (fine == 2) {
+                        tile.column = t & 1;
+                        t >>= 1;
+                    }
                     tile.i = static_cast<int>((sqrtf(8.f * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
                     while (lower(tile.i, 0) > t) --tile.i;
                     while (lower(tile.i + 1, 0) <= t) ++tile.i;
                     tile.j = t - lower(tile.i, 0);
-                    tile.groups = min(2, (w.m - tile.j * kBlock + 63) / 64);
-                    tile.slices = ((gram ? w.n : w.m) + 63) / 64;
+                    tile.groups = max(0, min(3 - fine, (w.m - tile.j * kBlock + 63) / 64 - tile.column));
+                    const int all = ((whole ? w.n : w.m) + 63) / 64, share = whole ? (all + w.parts - 1) / w.parts : all;
+                    tile.from = tile.part * share;
+                    tile.slices = kind == SUM || tile.groups == 0 ? 0 : min(share, all - tile.from);
                 }
-                // pass it on
-                if (!wait(&qempty_bar[slot], qparity ^ 1, nml::ERR_WAIT_EMPTY)) {
-                    ok = false;
-                    break;
-                }
-                if (lane < kOpWords) reinterpret_cast<int*>(&queue[slot].op)[lane] = word;
-                if (lane == 0) {
-                    queue[slot].k = tile.k, queue[slot].i = tile.i, queue[slot].j = tile.j, queue[slot].job = tile.job;
-                    queue[slot].groups = tile.groups, queue[slot].slices = tile.slices, queue[slot].extra = tile.extra;
-                    queue[slot].w = w;
-                }
-                __syncwarp();
-                if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qfull_bar[slot]));
-                const Op& op = queue[slot].op;  // (the producer's own copy stays until it comes round to the slot again)
-                if (++slot == kQueue) slot = 0, qparity ^= 1;
-
-                // the matrix's earlier products
-                const int tiles_gram = lower(mb, 0), tiles_update = mb * ((w.nb + w.wide - 1) / w.wide);
-                const int need = kEpilogueWarps * (op.symmetric_before * tiles_gram + op.wide_before * tiles_update);
-                if (need > 0) {
+                // the matrix's earlier products: to be waited for before its copies are issued, or, where there are none, before it is passed on
+                auto wait_for_matrix = [&](const Op& op) {
+                    const int need = kEpilogueWarps * (op.gram_before * symmetric_tiles * w.parts + op.symmetric_before * symmetric_tiles +
+                                                       op.wide_before * mb * per_row + op.sum_before * (w.parts > 1 ? 2 * blocks : 0));
+                    if (need == 0) return true;
                     int gave_up = 0;
                     if (lane == 0) {
                         const int* const done = P.c.done + 1 + tile.k;
@@ -693,11 +705,33 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                             }
                         }
                     }
-                    if (__shfl_sync(0xffffffffu, gave_up, 0)) {
-                        ok = false;
-                        break;
-                    }
+                    if (__shfl_sync(0xffffffffu, gave_up, 0)) return false;
                     fence_proxies();
+                    return true;
+                };
+                // pass it on
+                if (!wait(&qempty_bar[slot], qparity ^ 1, nml::ERR_WAIT_EMPTY)) {
+                    ok = false;
+                    break;
+                }
+                if (lane < kOpWords) reinterpret_cast<int*>(&queue[slot].op)[lane] = word;
+                if (lane == 0) {
+                    queue[slot].k = tile.k, queue[slot].i = tile.i, queue[slot].j = tile.j, queue[slot].job = tile.job, queue[slot].column = tile.column;
+                    queue[slot].groups = tile.groups, queue[slot].part = tile.part, queue[slot].slices = tile.slices, queue[slot].extra = tile.extra;
+                    queue[slot].w = w;
+                }
+                __syncwarp();
+                const Op& op = queue[slot].op;  // (the producer's own copy stays until it comes round to the slot again)
+                if (tile.slices == 0 && !wait_for_matrix(op)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qfull_bar[slot]));
+                if (++slot == kQueue) slot = 0, qparity ^= 1;
+                if (tile.slices == 0) continue;
+                if (!wait_for_matrix(op)) {
+                    ok = false;
+                    break;
                 }
 
                 // its K slices; a ring of stages of the other size only begins when the last one's are free
@@ -711,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                     now_stage = stage_bytes;
                     stages = kRing / stage_bytes;
                 }
-                const bool same = gram && tile.i == tile.j;
+                const bool same = whole && tile.i == tile.j;
                 const int b_pieces = same ? 0 : tile.groups, pieces = kPlanes * (2 + b_pieces);
                 const bool is_a = lane < 2 * kPlanes;
                 const int at = is_a ? lane : lane - 2 * kPlanes, per = is_a ? 2 : max(1, b_pieces);
@@ -731,19 +765,20 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                     __syncwarp();
                     if (lane < pieces) {
                         const bool low = q >= tile.slices;  // a I times X's low half
-                        const int kq = low ? 2 * tile.i + q - tile.slices : q, kb = kq >> 1, h = kq & 1;
+                        const int kq = low ? 2 * tile.i + q - tile.slices : tile.from + q, kb = kq >> 1, h = kq & 1;
+                        const int group = is_a ? piece : piece + tile.column;
                         const uint8_t* from;
-                        const uint32_t straight = (h * 2 + piece) * kPiece, across = (piece * 2 + h) * kPiece;  // K-major; MN-major
+                        const uint32_t straight = (h * 2 + group) * kPiece, across = (group * 2 + h) * kPiece;  // K-major; MN-major
                         auto symmetric = [&](int row) {
                             return kb <= row ? block_at(P.c.blocks, buffer, lower(row, kb)) + straight : block_at(P.c.blocks, buffer, lower(kb, row)) + across;
                         };
                         if (!is_wide) {
                             const int row = is_a ? tile.i : tile.j;
-                            from = gram ? block_at(P.c.blocks, x, row * w.nb + kb) + straight : symmetric(row);
+                            from = whole ? block_at(P.c.blocks, x, row * w.nb + kb) + straight : symmetric(row);
                         } else if (is_a) {
                             from = low ? block_at(P.c.blocks, op.identity, 0) + straight : symmetric(tile.i);
                         } else {  // X's rows along K: two 64-column groups to a block
-                            from = block_at(P.c.blocks, x, kb * w.nb + tile.j + (piece >> 1)) + (low ? kPlane : 0) + ((piece & 1) * 2 + h) * kPiece;
+                            from = block_at(P.c.blocks, x, kb * w.nb + tile.j + (group >> 1)) + (low ? kPlane : 0) + ((group & 1) * 2 + h) * kPiece;
                         }
                         nml::bulk_load(to, from + plane * kPlane, kPiece, bar);
                     }
@@ -785,12 +820,13 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 break;
             }
             const int k = queue[slot].k, row = queue[slot].i, column = queue[slot].j, groups = queue[slot].groups, real = queue[slot].slices;
-            const int slices = real + queue[slot].extra;
-            const bool is_wide = queue[slot].op.kind >= ITERATE, gram = queue[slot].op.gram != 0;
+            const int slices = real + queue[slot].extra, kind = queue[slot].op.kind, in_block = queue[slot].column;
+            const bool is_wide = kind == ITERATE || kind == RESULT, gram = queue[slot].op.gram != 0;
             if (k < 0) break;
             __syncwarp();
             if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qempty_bar[slot]));
             if (++slot == kQueue) slot = 0, qparity ^= 1;
+            if (slices == 0) continue;
             const uint32_t stage_bytes = is_wide ? kWideStage : kNarrow, b_bytes = is_wide ? 2 * kHalf : kHalf;
             if (now_stage != stage_bytes) {
                 s = 0;
@@ -816,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 const int a_mn = !gram && !low && kb > row;
                 const int b_mn = is_wide ? 1 : !gram && kb > column;
                 const uint32_t idesc = nml::make_instr_desc(0, a_mn, b_mn, 128, groups * 64);
-                const uint32_t sa = ring + s * stage_bytes, sb = same ? sa : sa + kPlanes * kHalf, bp = same ? kHalf : b_bytes;
+                const uint32_t sa = ring + s * stage_bytes, sb = same ? sa + in_block * kPiece : sa + kPlanes * kHalf, bp = same ? kHalf : b_bytes;
                 if (nml::elect_one()) {
                     const uint64_t a0 = nml::make_smem_desc(sa, kPiece, 1024, 2), b0 = nml::make_smem_desc(sb, kPiece, 1024, 2);
                     const uint32_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
@@ -858,7 +894,6 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
         // A tile is reported when its stores are visible, which takes a while: where the next one is there already, its first slice comes first.
         auto report = [&]() {
             if (pending >= 0) {
-                fence_proxies();
                 __syncwarp();
                 if (lane == 0) add_release(P.c.done + 1 + pending, 1);
                 pending = -1;
@@ -868,6 +903,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
             if (!__all_sync(0xffffffffu, nml::mbar_test(nml::smem_u32(&qfull_bar[slot]), qparity))) report();
             if (!wait(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL)) break;
             const int k = queue[slot].k, tile_i = queue[slot].i, tile_j = queue[slot].j, groups = queue[slot].groups, slices = queue[slot].slices;
+            const int in_block = queue[slot].column, part = queue[slot].part;
             const int kind = queue[slot].op.kind, gram = queue[slot].op.gram, from_x = queue[slot].op.from;
             const Symmetric job = queue[slot].op.job[queue[slot].job];
             const float op_f1 = queue[slot].op.f1, op_d1 = queue[slot].op.d1;
@@ -876,8 +912,8 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
             __syncwarp();
             if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qempty_bar[slot]));
             if (++slot == kQueue) slot = 0, qparity ^= 1;
-            const int mine = groups * 2, g0 = side * mine;  // this thread's columns in sixteens; the first
-            const int chunks = kPlanes == 2 ? slices : 1;
+            const int mine = groups * 2, g0 = side * mine + 4 * in_block;  // this thread's columns in sixteens; the first one in its block
+            const int chunks = kPlanes == 2 ? slices : min(1, slices);
             float acc[8][16];
 #pragma unroll
             for (int c = 0; c < 8; ++c)
@@ -891,7 +927,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                     break;
                 }
                 nml::tc_fence_after();
-                const uint32_t from = tmem + buf * 256 + g0 * 16 + (static_cast<uint32_t>(quarter * 32) << 16);
+                const uint32_t from = tmem + buf * 256 + side * mine * 16 + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
                 for (int c = 0; c < 8; c += 2) {
                     if (c < mine) {
@@ -982,7 +1018,33 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 // (of a last block of 64 rows or fewer, half is never read: K slices and columns end at a multiple of 64, and what the other rows of an
                 // operand hold, which may be anything, ends in rows and columns that are not stored either)
                 const bool in_use = tile_i * kBlock + (quarter & 2) * 32 < w.m;
-                const int matrices = in_use ? kind == POLY ? 2 : 1 : 0;
+                // X X^T in several parts of K: the sums go to memory as they are, [sixteen columns][four of them][row], and come from there in order
+                const int mb = (w.m + kBlock - 1) / kBlock;
+                const bool partial = kind == POLY && gram && w.parts > 1;
+                if (partial && in_use) {
+                    float4* const out = reinterpret_cast<float4*>(block_at(P.c.blocks, w.partial, part * lower(mb, 0) + block));
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (c < mine)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                out[((g0 + c) * 4 + q) * kBlock + row] = make_float4(acc[c][4 * q], acc[c][4 * q + 1], acc[c][4 * q + 2], acc[c][4 * q + 3]);
+                }
+                if (kind == SUM && in_use) {
+                    const float4* const from = reinterpret_cast<const float4*>(block_at(P.c.blocks, w.partial, block));
+                    const size_t step = static_cast<size_t>(lower(mb, 0)) * (2 * kPlane / sizeof(float4));
+#pragma unroll 2
+                    for (int p = 0; p < w.parts; ++p)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            if (c < mine)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    const float4 v = load_shared_by_blocks(from + p * step + ((g0 + c) * 4 + q) * kBlock + row);
+                                    acc[c][4 * q] += v.x, acc[c][4 * q + 1] += v.y, acc[c][4 * q + 2] += v.z, acc[c][4 * q + 3] += v.w;
+                                }
+                }
+                const int matrices = !in_use || partial || groups == 0 ? 0 : kind == POLY || kind == SUM ? 2 : 1;
 #pragma unroll 1
                 for (int e = 0; e < matrices; ++e) {  // (A and P: f0 is a power of two)
                     scale(e ? op_f1 / job.f0 : (iterate ? op_f1 : job.f0) * over);
@@ -1113,46 +1175,57 @@ static bool chained(const Source& s, int math) { return math == NML_MATH_3XF16 &
 
 struct Plan {
     int sums = 0, halves = 0, first_class = 0;
-    int gram_tiles[kClasses] = {0, 0}, update_tiles[kClasses] = {0, 0};
+    int gram_tiles[kClasses] = {0, 0}, symmetric_tiles[kClasses] = {0, 0}, update_tiles[kClasses] = {0, 0}, sum_tiles[kClasses] = {0, 0};
     uint32_t blocks = 0, identity = 0;
     size_t sums_at = 0, rounds_at = 0, done_at = 0, blocks_at = 0, bytes = 0;
 };
 // Lays a group of at most kGroup matrices out, chained ones first, longer ones first; the sources are set.
 static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
     Plan p;
-    long long wide_tiles = 0;
+    long long blocks = 0, wide_tiles[3] = {0, 0, 0};
     for (int k = 0; k < count; ++k) {
         w[k].chained = steps > 1 && chained(w[k].s, math);
         w[k].mb = (w[k].s.m + kBlock - 1) / kBlock;
         w[k].nb = (w[k].s.n + kBlock - 1) / kBlock;
-        wide_tiles += static_cast<long long>(w[k].mb) * ((w[k].nb + 1) / 2);
+        blocks += w[k].mb * (w[k].mb + 1) / 2;
+        for (int e = 0; e < 3; ++e) wide_tiles[e] += static_cast<long long>(w[k].mb) * (((w[k].s.n + 63) / 64 + (1 << e) - 1) >> e);
     }
+    // Where a round has few tiles: two to a block, narrow ones of Q X, and X X^T with its long K in parts, at least eight slices each (XXX).
+    const int fine = 2 * blocks <= sms ? 2 : 1, spare = static_cast<int>(std::max<long long>(1, sms / (blocks * fine)));
+    const int wide = wide_tiles[0] <= sms ? 1 : wide_tiles[1] <= sms ? 2 : 4;
     std::sort(w, w + count, [](const Work& a, const Work& b) {
         if (a.chained != b.chained) return a.chained > b.chained;
         if (a.s.m != b.s.m) return a.s.m > b.s.m;
         return a.s.n != b.s.n ? a.s.n > b.s.n : a.s.in < b.s.in;
     });
-    int gram = 0, update = 0;
+    int gram = 0, symmetric = 0, update = 0, sum = 0;
     for (int k = 0; k < count; ++k) {
         Work& v = w[k];
-        const int c = v.chained ? 0 : 1, tiles = v.mb * (v.mb + 1) / 2;
+        const int c = v.chained ? 0 : 1, own = v.mb * (v.mb + 1) / 2, slices = (v.s.n + 63) / 64;
         if (v.chained) p.first_class = k + 1;
         v.first_sum = p.sums;
         v.sums = static_cast<int>((static_cast<long long>(v.s.m) * v.s.n + kSumElements - 1) / kSumElements);
         p.sums += v.sums;
         v.first_half = p.halves;
         p.halves += v.mb * v.nb * 2;
-        v.first_gram = gram;
-        gram += tiles;
-        p.gram_tiles[c] += tiles;
-        v.wide = wide_tiles >= sms ? 2 : 1;
-        v.first_update = update;
-        const int updates = v.mb * ((v.nb + v.wide - 1) / v.wide);
-        update += updates;
-        p.update_tiles[c] += updates;
+        v.fine = fine;
+        const int most = std::max(1, std::min(spare, slices / 8)), share = (slices + most - 1) / most;
+        v.parts = (slices + share - 1) / share;
+        v.wide = wide;
+        auto tiles = [&](int* first, int* all, int* of_class, int n) {
+            *first = *all;
+            *all += n;
+            *of_class += n;
+        };
+        tiles(&v.first_gram, &gram, &p.gram_tiles[c], own * fine * v.parts);
+        tiles(&v.first_symmetric, &symmetric, &p.symmetric_tiles[c], own * fine);
+        tiles(&v.first_update, &update, &p.update_tiles[c], v.mb * ((slices + wide - 1) / wide));
+        tiles(&v.first_parts, &sum, &p.sum_tiles[c], v.parts > 1 ? 2 * own : 0);
         for (uint32_t* at : {&v.x[0], &v.x[1]}) *at = p.blocks, p.blocks += v.mb * v.nb;
         v.sym = p.blocks;
-        p.blocks += (v.chained ? 7 : 3) * tiles;
+        p.blocks += (v.chained ? 7 : 3) * own;
+        v.partial = p.blocks;
+        if (v.parts > 1) p.blocks += v.parts * own;
     }
     p.identity = p.blocks;
     if (math == NML_MATH_F16) p.blocks += steps;
@@ -1166,13 +1239,18 @@ static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
 }
 
 // The products of a class, in order; their number.
-static int build_ops(const Polynomial& poly, uint32_t identity, Op* ops) {
-    int n = 0, from = 0, symmetric_before = 0, wide_before = 0;
+static int build_ops(const Polynomial& poly, uint32_t identity, bool in_parts, Op* ops) {
+    int n = 0, from = 0, gram_before = 0, symmetric_before = 0, wide_before = 0, sum_before = 0;
     auto add = [&](Op op) {
         op.jobs = std::max(op.jobs, 1);
+        op.gram_before = gram_before;
         op.symmetric_before = symmetric_before;
         op.wide_before = wide_before;
-        if (op.kind >= ITERATE) ++wide_before; else symmetric_before += op.jobs;
+        op.sum_before = sum_before;
+        if (op.kind == SUM) ++sum_before;
+        else if (op.kind == ITERATE || op.kind == RESULT) ++wide_before;
+        else if (op.kind == POLY && op.gram) ++gram_before;
+        else symmetric_before += op.jobs;
         ops[n++] = op;
     };
     // a product of two symmetric matrices stored times 2^el and 2^er, to be stored times 2^eo, + d on the diagonal
@@ -1192,6 +1270,10 @@ static int build_ops(const Polynomial& poly, uint32_t identity, Op* ops) {
         a.f1 = static_cast<float>(ldexp(s.c, s.ep - (s.starts ? 0 : eu_last + poly.step[k - 1].et)));
         a.d1 = static_cast<float>(ldexp(s.b, s.ep));
         add(a);
+        if (s.starts && in_parts) {
+            a.kind = SUM;
+            add(a);
+        }
         u = s.starts || u != kUpdate ? kUpdate : kUpdate2;
         if (s.starts) q = u, eq = s.eu;
         Op b = {};             // U
@@ -1246,7 +1328,7 @@ static void launch_pack(const PackParams<kMaxRounds>& all, const Call& call, int
     std::copy(all.round, all.round + std::min(N, all.rounds), q.round);
     nml::launch(call.in_dtype == NML_F16 ? ortho_pack_kernel<N, __half> : ortho_pack_kernel<N, float>, blocks, 256, 0, st, q);
 }
-constexpr int kFewRounds = 20;
+constexpr int kFewRounds = 22;
 
 // Whether a group goes through double precision: see nml_ortho_small.cuh.
 static bool all_small(const Work* w, int count) {
@@ -1301,7 +1383,7 @@ static int run_small(Work* w, int count, const Call& call, const Polynomial& pol
     else gram(std::integral_constant<int, kGroup>());
     SmallSteps s = {c, q, call.eps, poly.steps, {}, {}, {}};
     for (int k = 0; k < poly.steps; ++k) s.a[k] = poly.step[k].a, s.b[k] = poly.step[k].b, s.k[k] = poly.step[k].c;
-    nml::launch(small_steps_kernel, count, 256, kSmallStepsSmem, st, s);
+    nml::launch(small_steps_kernel, count, 32 * kStepsWarps, kSmallStepsSmem, st, s);
     const SmallResult r = {c, q, call.mo, call.out_dtype == NML_F16, call.apply, call.keep, call.rate};
     nml::launch(half ? small_result_kernel<__half> : small_result_kernel<float>, p.chunks, 256, kSmallResultSmem, st, r);
     NMLO_CUDA(cudaGetLastError());
@@ -1330,7 +1412,7 @@ static int run_group(Work* w, int count, const Call& call, const Steps& steps, v
     PackParams<kMaxRounds> pack = {c, call.mo, call.eps, p.halves, 0, p.identity, call.math == NML_MATH_F16 ? steps.of[1].steps : 0, {}, {}};
     Op ops[kClasses][kMaxRounds];
     int number[kClasses];
-    for (int cls = 0; cls < kClasses; ++cls) number[cls] = build_ops(steps.of[cls], p.identity, ops[cls]);
+    for (int cls = 0; cls < kClasses; ++cls) number[cls] = build_ops(steps.of[cls], p.identity, p.sum_tiles[cls] > 0, ops[cls]);
     if (p.first_class == 0) number[0] = 0;
     if (p.first_class == count) number[1] = 0;
     pack.rounds = std::max(number[0], number[1]);
@@ -1342,7 +1424,9 @@ static int run_group(Work* w, int count, const Call& call, const Steps& steps, v
         for (int cls = 0; cls < kClasses; ++cls) {
             if (r >= number[cls]) continue;
             const Op& op = round.op[cls] = ops[cls][r];
-            const long long n = op.kind >= ITERATE ? p.update_tiles[cls] : static_cast<long long>(op.jobs) * p.gram_tiles[cls];
+            const long long n = op.kind == ITERATE || op.kind == RESULT ? p.update_tiles[cls]
+                                : op.kind == SUM ? p.sum_tiles[cls] : op.kind == POLY && op.gram ? p.gram_tiles[cls]
+                                : static_cast<long long>(op.jobs) * p.symmetric_tiles[cls];
             if (cls == 0) round.of_first = static_cast<int>(n);
             tiles += n;
         }
@@ -1353,7 +1437,7 @@ static int run_group(Work* w, int count, const Call& call, const Steps& steps, v
     double slices = 0.0;
     for (int k = 0; k < count; ++k) {
         const double m = w[k].s.m / 64 + 1, n = w[k].s.n / 64 + 1, t = w[k].mb * (w[k].mb + 1) / 2;
-        slices += steps.of[1].steps * (t * n + 3 * t * m + w[k].mb * (w[k].nb / w[k].wide + 1.0) * (m + 2));
+        slices += steps.of[1].steps * 2 * (t * n + 3 * t * m + w[k].mb * n * (m + 2));
     }
 
     if (count <= 8) launch_sums<8>(w, c, call, p.sums, st);

@@ -56,30 +56,30 @@ __device__ __forceinline__ void multiply8(const double (*l)[kSmallPitch], const 
     const double a = l[lane >> 2][k + (lane & 3)], b = r[lane >> 2][k + (lane & 3)];
     asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
 }
-constexpr int kSmallTiles = 5;  // of the 36 lower ones, to a warp
-// The lower 8 x 8 tiles of l r^T, t = warp, warp + 8, ... to a warp.
-__device__ __forceinline__ void multiply_lower(const double (*l)[kSmallPitch], const double (*r)[kSmallPitch], int tiles, int depth, double (&d)[kSmallTiles][2]) {
+// The lower 8 x 8 tiles of l r^T, t = warp, warp + kWarps, ... to a warp; kTiles x kWarps are at least 36.
+template <int kWarps, int kTiles>
+__device__ __forceinline__ void multiply_lower(const double (*l)[kSmallPitch], const double (*r)[kSmallPitch], int tiles, int depth, double (&d)[kTiles][2]) {
     const int warp = threadIdx.x >> 5;
-    int row[kSmallTiles], column[kSmallTiles];
+    int row[kTiles], column[kTiles];
 #pragma unroll
-    for (int e = 0; e < kSmallTiles; ++e) {
-        const int t = warp + 8 * e;
+    for (int e = 0; e < kTiles; ++e) {
+        const int t = warp + kWarps * e;
         row[e] = static_cast<int>((sqrtf(8.f * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
         column[e] = t - row[e] * (row[e] + 1) / 2;
     }
 #pragma unroll 2
     for (int k = 0; k < depth; k += 4)
 #pragma unroll
-        for (int e = 0; e < kSmallTiles; ++e)
-            if (warp + 8 * e < tiles) multiply8(l + 8 * row[e], r + 8 * column[e], k, d[e]);
+        for (int e = 0; e < kTiles; ++e)
+            if (warp + kWarps * e < tiles) multiply8(l + 8 * row[e], r + 8 * column[e], k, d[e]);
 }
 // f(value, i, j) for this lane's elements of them.
-template <class F>
-__device__ __forceinline__ void each_lower(int tiles, const double (&d)[kSmallTiles][2], F&& f) {
+template <int kWarps, int kTiles, class F>
+__device__ __forceinline__ void each_lower(int tiles, const double (&d)[kTiles][2], F&& f) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-    for (int e = 0; e < kSmallTiles; ++e) {
-        const int t = warp + 8 * e;
+    for (int e = 0; e < kTiles; ++e) {
+        const int t = warp + kWarps * e;
         if (t >= tiles) continue;
         const int row = static_cast<int>((sqrtf(8.f * static_cast<float>(t) + 1.f) - 1.f) * 0.5f), column = t - row * (row + 1) / 2;
         const int i = 8 * row + (lane >> 2), j = 8 * column + 2 * (lane & 3);
@@ -105,15 +105,15 @@ __global__ void __launch_bounds__(256) small_gram_kernel(const __grid_constant__
     }
     const Work& w = group.w[lo];
     const int part = blockIdx.x - w.first_sum, tiles = small_lower(small_side(w.s.m)), chunks = (w.s.n + 63) / 64, per = (chunks + w.sums - 1) / w.sums;
-    double d[kSmallTiles][2] = {};
+    double d[5][2] = {};
     for (int e = part * per; e < min(chunks, (part + 1) * per); ++e) {
         __syncthreads();
         load_columns<T, false>(w.s, mo, e * 64, true, x);
         __syncthreads();
-        multiply_lower(x, x, tiles, min(64, (w.s.n - e * 64 + 3) & ~3), d);
+        multiply_lower<8>(x, x, tiles, min(64, (w.s.n - e * 64 + 3) & ~3), d);
     }
     double* const out = c.sums + static_cast<size_t>(blockIdx.x) * kSmall * kSmall;
-    each_lower(tiles, d, [&](double v, int i, int j) { out[i * kSmall + j] = v; });
+    each_lower<8>(tiles, d, [&](double v, int i, int j) { out[i * kSmall + j] = v; });
 }
 
 struct SmallSteps {
@@ -124,7 +124,8 @@ struct SmallSteps {
     double a[kMaxSteps], b[kMaxSteps], k[kMaxSteps];  // coefficients
 };
 // The steps, a block to a matrix.
-__global__ void __launch_bounds__(256) small_steps_kernel(const __grid_constant__ SmallSteps P) {
+constexpr int kStepsWarps = 16;
+__global__ void __launch_bounds__(32 * kStepsWarps) small_steps_kernel(const __grid_constant__ SmallSteps P) {
     pdl_enter();
     if (skipped(P.c.skip)) return;
     extern __shared__ double room[];
@@ -137,11 +138,11 @@ __global__ void __launch_bounds__(256) small_steps_kernel(const __grid_constant_
     const int m = small_side(w.s.m), tiles = small_lower(m), tid = threadIdx.x, i0 = tid >> 6, j0 = tid & 63;
     auto each = [&](auto&& f) {  // all elements
         if (j0 < m)
-            for (int i = i0; i < m; i += 4) f(i, j0);
+            for (int i = i0; i < m; i += kStepsWarps / 2) f(i, j0);
     };
     // the sum of the partial ones, in a fixed order; the lower blocks, mirrored
 #pragma unroll 2
-    for (int i = i0; i < m; i += 4) {
+    for (int i = i0; i < m; i += kStepsWarps / 2) {
         if (j0 > i) continue;
         const double* from = P.c.sums + static_cast<size_t>(w.first_sum) * kSmall * kSmall + i * kSmall + j0;
         double s = 0.0;
@@ -163,9 +164,9 @@ __global__ void __launch_bounds__(256) small_steps_kernel(const __grid_constant_
     __syncthreads();
     // out = f(l r, i, j) of two symmetric matrices, both triangles
     auto product = [&](Matrix l, Matrix r, Matrix out, auto&& f) {
-        double d[kSmallTiles][2] = {};
-        multiply_lower(l, r, tiles, m, d);
-        each_lower(tiles, d, [&](double v, int i, int j) {
+        double d[3][2] = {};
+        multiply_lower<kStepsWarps>(l, r, tiles, m, d);
+        each_lower<kStepsWarps>(tiles, d, [&](double v, int i, int j) {
             if (i >= j) out[i][j] = out[j][i] = f(v, i, j);
         });
     };

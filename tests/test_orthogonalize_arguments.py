@@ -31,8 +31,8 @@ def test_workspace_size(lib):
     chained = _need(lib, [(256, 512)])[1]       # two iterates of eight blocks, seven symmetric matrices of three
     assert 37 * block <= chained <= 37 * block + tables
     assert _need(lib, [(256, 512)], steps=1)[1] == chained - 12 * block
-    group = _need(lib, [(128, 256)] * 128)[1]
-    assert group >= 128 * 7 * block and _need(lib, [(128, 256)] * 1000)[1] == group   # one group at a time
+    group = _need(lib, [(128, 256)] * 64)[1]
+    assert group >= 64 * 7 * block and _need(lib, [(128, 256)] * 1000)[1] == group   # one group at a time
     assert _need(lib, [(1, (1 << 24) + 1)])[0] == INVALID
     for bad in ([(0, 4)], [(4, 0)], [(-1, 4)], [(1 << 30, 1 << 30)]):
         assert _need(lib, bad)[0] == INVALID
