@@ -334,10 +334,11 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__
     }
     for (int i = tid; i < P.c.count; i += 256) first[i] = load_global(&P.c.table[i].first_half);
     __syncthreads();
-    const int k = owner_of(first, P.c.count, blockIdx.x);
+    // (from the last one to the first: the sums have read the matrices in the other order, so the last ones are in L2)
+    const int at_half = P.halves - 1 - blockIdx.x, k = owner_of(first, P.c.count, at_half);
     const Work w = load_work(P.c.table + k);
     const Source& s = w.s;
-    const int half = blockIdx.x - first[k], i0 = half / (2 * w.nb) * kBlock, j0 = half % (2 * w.nb) * 64;
+    const int half = at_half - first[k], i0 = half / (2 * w.nb) * kBlock, j0 = half % (2 * w.nb) * 64;
     uint8_t* const out = block_at(P.c.blocks, w.x[0], half / 2) + (half & 1) * kHalf;
     if (j0 >= w.nb * kBlock) return;
     // the norm, from the partial sums in a fixed order
@@ -551,7 +552,7 @@ __device__ __forceinline__ void fence_proxies() { asm volatile("fence.proxy.asyn
 template <int kPlanes>
 __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid_constant__ ProductParams P) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tfull_bar[2], tempty_bar[2], qfull_bar[kQueue], qempty_bar[kQueue],
+    __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tfull_bar[4], tempty_bar[4], qfull_bar[kQueue], qempty_bar[kQueue],
         drain_bar;
     __shared__ __align__(8) int abort_state[4];
     __shared__ uint32_t tmem_base;
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
             nml::mbar_init(nml::smem_u32(&full_bar[s]), 1);
             nml::mbar_init(nml::smem_u32(&empty_bar[s]), 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 4; ++b) {
             nml::mbar_init(nml::smem_u32(&tfull_bar[b]), 1);
             nml::mbar_init(nml::smem_u32(&tempty_bar[b]), kEpilogueWarps);
         }
@@ -810,8 +811,8 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA
-        int slot = 0, s = 0, stages = 0, buf = 0;
-        uint32_t qparity = 0, parity = 0, tparity = 0, now_stage = 0;
+        int slot = 0, s = 0, stages = 0, unit = 0;
+        uint32_t qparity = 0, parity = 0, tparity = 0, pairs = 0, now_stage = 0;  // pairs: of units whose last use was by both
         bool ok = true;
         const uint32_t ring = nml::smem_u32(smem);
         while (ok) {
@@ -836,10 +837,13 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
             const bool same = gram && row == column;
             for (int q = 0; q < slices; ++q) {
                 if (kPlanes == 2 || q == 0) {
-                    if (!wait(&tempty_bar[buf], tparity ^ 1, nml::ERR_WAIT_TMEM_EMPTY)) {
-                        ok = false;
-                        break;
-                    }
+                    // TMEM is four units of 128 columns, each with its barriers; a wide tile takes two, and the first one's barriers
+                    if (is_wide && (unit & 1)) unit = (unit + 1) & 3;
+                    const int pair = unit >> 1;
+                    auto drained = [&](int u) { return wait(&tempty_bar[u], (tparity >> u & 1) ^ 1, nml::ERR_WAIT_TMEM_EMPTY); };
+                    ok = drained(unit) && (!is_wide || drained(unit + 1)) && (is_wide || !(unit & 1) || !(pairs >> pair & 1) || drained(unit - 1));
+                    if (!ok) break;
+                    if (is_wide) pairs |= 1u << pair; else pairs &= ~(1u << pair);
                     nml::tc_fence_after();
                 }
                 if (!wait(&full_bar[s], parity >> s & 1, nml::ERR_WAIT_FULL)) {
@@ -861,15 +865,18 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                         uint64_t ad = a0 + (p == 2 ? kHalf >> 4 : 0), bd = b0 + (p == 1 ? bp >> 4 : 0);
 #pragma unroll
                         for (int e = 0; e < 4; ++e, ad += a_step, bd += b_step)
-                            nml::umma_f16(tmem + buf * 256, ad, bd, idesc, kPlanes == 2 ? e > 0 || p < 2 : e > 0 || q > 0);
+                            nml::umma_f16(tmem + unit * 128, ad, bd, idesc, kPlanes == 2 ? e > 0 || p < 2 : e > 0 || q > 0);
                     }
                     nml::umma_commit(nml::smem_u32(&empty_bar[s]));
-                    if (last) nml::umma_commit(nml::smem_u32(&tfull_bar[buf]));
+                    if (last) nml::umma_commit(nml::smem_u32(&tfull_bar[unit]));
                 }
                 __syncwarp();
                 parity ^= 1u << s;
                 if (++s == stages) s = 0;
-                if (last && ++buf == 2) buf = 0, tparity ^= 1;
+                if (last) {
+                    tparity ^= 1u << unit;
+                    unit = (unit + (is_wide ? 2 : 1)) & 3;
+                }
             }
         }
         if (!ok) {  // the products issued so far still read shared memory and write TMEM
@@ -887,7 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         // ------------------------------------------------------------ epilogue: a thread to a row and half of the columns of the tile
-        int slot = 0, buf = 0, pending = -1;  // pending: matrix of a tile that is stored but not reported
+        int slot = 0, unit = 0, pending = -1;  // pending: matrix of a tile that is stored but not reported
         uint32_t qparity = 0, tparity = 0;
         const int quarter = warp & 3, row = quarter * 32 + lane, side = (warp - 4) >> 2;
         uint8_t* const staging = smem + kRing + (warp - 4) * kStaging;
@@ -914,6 +921,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
             if (++slot == kQueue) slot = 0, qparity ^= 1;
             const int mine = groups * 2, g0 = side * mine + 4 * in_block;  // this thread's columns in sixteens; the first one in its block
             const int chunks = kPlanes == 2 ? slices : min(1, slices);
+            const bool is_wide = kind == ITERATE || kind == RESULT;
             float acc[8][16];
 #pragma unroll
             for (int c = 0; c < 8; ++c)
@@ -921,13 +929,14 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 for (int e = 0; e < 16; ++e) acc[c][e] = 0.f;
             bool ok = true;
             for (int q = 0; q < chunks; ++q) {
-                if (q == 0 && !__all_sync(0xffffffffu, nml::mbar_test(nml::smem_u32(&tfull_bar[buf]), tparity))) report();
-                if (!wait(&tfull_bar[buf], tparity, nml::ERR_WAIT_TMEM_FULL)) {
+                if (is_wide && (unit & 1)) unit = (unit + 1) & 3;
+                if (q == 0 && !__all_sync(0xffffffffu, nml::mbar_test(nml::smem_u32(&tfull_bar[unit]), tparity >> unit & 1))) report();
+                if (!wait(&tfull_bar[unit], tparity >> unit & 1, nml::ERR_WAIT_TMEM_FULL)) {
                     ok = false;
                     break;
                 }
                 nml::tc_fence_after();
-                const uint32_t from = tmem + buf * 256 + side * mine * 16 + (static_cast<uint32_t>(quarter * 32) << 16);
+                const uint32_t from = tmem + unit * 128 + side * mine * 16 + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
                 for (int c = 0; c < 8; c += 2) {
                     if (c < mine) {
@@ -940,8 +949,9 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 }
                 nml::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) nml::mbar_arrive(nml::smem_u32(&tempty_bar[buf]));
-                if (++buf == 2) buf = 0, tparity ^= 1;
+                if (lane == 0) nml::mbar_arrive(nml::smem_u32(&tempty_bar[unit]));
+                tparity ^= 1u << unit;
+                unit = (unit + (is_wide ? 2 : 1)) & 3;
             }
             if (!ok) break;
             report();
