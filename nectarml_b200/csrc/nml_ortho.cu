@@ -425,7 +425,9 @@ __device__ __forceinline__ long long load_wide(const long long* p) {
     asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(__cvta_generic_to_global(p)));
     return v;
 }
+constexpr int kMapRow = 512;   // bytes of a row of the map
 struct ProductParams {
+    CUtensorMap map;           // pairs: the blocks, a copy to a box
     Common c;
     int* err;
     unsigned long long limit_ns;  // of a wait
@@ -549,7 +551,25 @@ __device__ __forceinline__ void add_release(int* p, int v) {
 // What other blocks stored and this thread has acquired is seen by its bulk copies.
 __device__ __forceinline__ void fence_proxies() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
-template <int kPlanes>
+// A lane to a word of the other block's shared memory.
+__device__ __forceinline__ void store_remote(uint32_t cluster_addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+// Tiles of symmetric products: the blocks on and below the diagonal, or, for pairs of block rows, those of both rows up to the lower one's diagonal
+// (the upper one's last is above it, and not stored).
+template <bool kPair>
+__host__ __device__ __forceinline__ int symmetric_count(int mb) {
+    const int pairs = (mb + 1) / 2;
+    return kPair ? pairs * (pairs + 1) - (mb & 1) : mb * (mb + 1) / 2;
+}
+
+// kPair: a cluster of two blocks takes a tile of two block rows with cta_group::2 products, 256 x 128 or 256 x 256.  An SM then holds its own 128 rows and
+// half of the columns of a slice, so shared memory, which paces the tiles of one block (a slice of 128 x 128 in three products reads 128 KB and takes
+// in 64: 1250 clocks, where the tensor core needs 768; 128 x 256 1875 for 1536), has a quarter (a third) less to deliver, and a stage is as much smaller.
+// The first block takes the tiles and passes them to the other one; each loads its own operands, whose arrival the first one's barrier counts, and
+// stores its own row.  What the accumulators' readers of the other block tell the first one is a barrier's arrival without a fence: with one, behind
+// which the stores of the last tile had to be visible, the pair was slower than two blocks (2048 x 8192 1331 us; without 970; two blocks 1197).
+template <int kPlanes, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid_constant__ ProductParams P) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tfull_bar[4], tempty_bar[4], qfull_bar[kQueue], qempty_bar[kQueue],
@@ -561,22 +581,29 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     volatile int* const abort_flag = abort_state;
-    // A stage holds a K slice of both operands: 128 rows of the left one and 128 columns (symmetric products) or 256 (X) of the right one.
-    constexpr uint32_t kNarrow = kPlanes * 2 * kHalf, kWideStage = kPlanes * 3 * kHalf;
+    // A stage holds a K slice of both operands: 128 rows of the left one and 128 columns (symmetric products) or 256 (X) of the right one, of a pair
+    // half of them in each block.
+    constexpr uint32_t kNarrowB = kPair ? kPiece : kHalf, kWideB = kPair ? kHalf : 2 * kHalf;  // of a plane of the right one
+    constexpr uint32_t kNarrow = kPlanes * (kHalf + kNarrowB), kWideStage = kPlanes * (kHalf + kWideB);
+    constexpr int kBoth = kPair ? 2 : 1, kReports = kBoth * kEpilogueWarps;
+    const uint32_t rank = kPair ? nml::cluster_ctarank() : 0;
+    const bool leader = rank == 0;
 
-    if (warp == 0) nml::tmem_alloc(nml::smem_u32(&tmem_base), 512);
+    if (warp == 0) {
+        if (kPair) nml::tmem_alloc_pair(nml::smem_u32(&tmem_base), 512); else nml::tmem_alloc(nml::smem_u32(&tmem_base), 512);
+    }
     if (tid == 32) {
         for (int s = 0; s < kMaxStages; ++s) {
-            nml::mbar_init(nml::smem_u32(&full_bar[s]), 1);
+            nml::mbar_init(nml::smem_u32(&full_bar[s]), 1);  // (of a pair the first block's counts both blocks' copies)
             nml::mbar_init(nml::smem_u32(&empty_bar[s]), 1);
         }
         for (int b = 0; b < 4; ++b) {
             nml::mbar_init(nml::smem_u32(&tfull_bar[b]), 1);
-            nml::mbar_init(nml::smem_u32(&tempty_bar[b]), kEpilogueWarps);
+            nml::mbar_init(nml::smem_u32(&tempty_bar[b]), kReports);
         }
         for (int q = 0; q < kQueue; ++q) {
             nml::mbar_init(nml::smem_u32(&qfull_bar[q]), 1);
-            nml::mbar_init(nml::smem_u32(&qempty_bar[q]), 1 + kEpilogueWarps);
+            nml::mbar_init(nml::smem_u32(&qempty_bar[q]), (kPair && leader ? 2 : 1) + kEpilogueWarps);  // (the other block's users are one)
         }
         nml::mbar_init(nml::smem_u32(&drain_bar), 1);
         nml::fence_mbar_init();
@@ -593,101 +620,156 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
     }
     nml::tc_fence_before();
     __syncthreads();
+    if (kPair) nml::cluster_sync_all();  // (barriers are there before the other block arrives on them)
     nml::tc_fence_after();
     const uint32_t tmem = tmem_base;
     auto symmetric_first = [&](const Info& w, int buffer) { return w.sym + buffer * lower((w.m + kBlock - 1) / kBlock, 0); };
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, nml::mbar_wait(nml::smem_u32(bar), parity, abort_flag, P.err, code)) != 0;
     };
+    // for what the other block of a pair has arrived with
+    auto wait_other = [&](uint64_t* bar, uint32_t parity, int code) {
+        return __all_sync(0xffffffffu, nml::mbar_wait<false, kPair>(nml::smem_u32(bar), parity, abort_flag, P.err, code)) != 0;
+    };
 
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
-    if (warp == 0) {
-        // ------------------------------------------------------------ producer: takes tiles, then a lane to a copy of 8 KB
-        const int tiles = skip ? 0 : P.tiles;
-        const Round* const rounds = P.c.rounds;
-        int slot = 0, s = 0, stages = 0;
-        uint32_t qparity = 0, parity = 0, used = 0;  // bits of parity: phase of each stage's next use; of used: stages not known to be free
-        uint32_t now_stage = 0;
-        bool ok = true;
-        int round = 0;
-        int next_first = tiles ? load_global(&rounds[min(1, P.rounds - 1)].first) : 0;
-        while (ok) {
-            // (not before the last tile's copies are issued: a block that held a second tile of a product would make that product twice as long)
-            int t = 0;
-            if (lane == 0) t = claim(P.c.done);
-            t = __shfl_sync(0xffffffffu, t, 0);
-            Tile tile;
-            tile.k = -1;
-            if (t < tiles) {
-                while (round + 1 < P.rounds && t >= next_first) {
-                    ++round;
-                    next_first = load_global(&rounds[min(round + 1, P.rounds - 1)].first);
-                }
-                t -= load_global(&rounds[round].first);
-                const int of_first = load_global(&rounds[round].of_first), cls = t >= of_first;
-                if (cls) t -= of_first;
-                const int* const words = reinterpret_cast<const int*>(&rounds[round].op[cls]);
-                const int word = lane < kOpWords ? load_global(words + lane) : 0;
-                const int kind = __shfl_sync(0xffffffffu, word, offsetof(Op, kind) / 4), jobs = __shfl_sync(0xffffffffu, word, offsetof(Op, jobs) / 4);
-                const int gram = __shfl_sync(0xffffffffu, word, offsetof(Op, gram) / 4);
-                const bool is_wide = kind == ITERATE || kind == RESULT, whole = kind == POLY && gram;
-                // (matrices of the first class come first, and their tiles count from 0; those of the second behind all of the first)
-                const int n0 = P.first_class;
-                const int lo = cls ? n0 : 0, hi = cls ? count : n0;
-                const int* const starts = first[is_wide ? 2 : kind == SUM ? 3 : whole ? 0 : 1];
-                const int base = starts[lo], per_job = is_wide ? 1 : jobs;
-                int a = lo, b = hi - 1;
-                while (a < b) {
-                    const int mid = (a + b + 1) / 2;
-                    if ((starts[mid] - base) * per_job <= t) a = mid; else b = mid - 1;
-                }
-                tile.k = a;
-                t -= (starts[a] - base) * per_job;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+        if (warp == 0) {
+            // ------------------------------------------------------------ producer: takes tiles, then a lane to a copy of 8 KB
+            const int tiles = skip ? 0 : P.tiles;
+            const Round* const rounds = P.c.rounds;
+            int slot = 0, s = 0, stages = 0;
+            uint32_t qparity = 0, parity = 0, used = 0;  // bits of parity: phase of each stage's next use; of used: stages not known to be free
+            uint32_t now_stage = 0;
+            bool ok = true;
+            int round = 0;
+            int next_first = tiles ? load_global(&rounds[min(1, P.rounds - 1)].first) : 0;
+            while (ok) {
+                Tile tile;
                 Info w;
-                {
-                    const Work* const from = P.c.table + a;
-                    auto word = [](const uint32_t* p) { return static_cast<uint32_t>(load_global(reinterpret_cast<const int*>(p))); };
-                    w = {load_global(&from->s.m), load_global(&from->s.n), load_global(&from->nb), load_global(&from->wide), load_global(&from->fine),
-                         load_global(&from->parts), {word(&from->x[0]), word(&from->x[1])}, word(&from->sym), word(&from->partial), load_global(&from->sx)};
-                }
-                const int mb = (w.m + kBlock - 1) / kBlock;
-                const int blocks = lower(mb, 0), symmetric_tiles = blocks * w.fine, wide_groups = (w.n + 63) / 64, per_row = (wide_groups + w.wide - 1) / w.wide;
-                tile.extra = tile.job = tile.column = tile.part = tile.from = 0;
-                if (is_wide) {
-                    tile.i = t / per_row;
-                    const int group = t % per_row * w.wide;
-                    tile.j = group >> 1;
-                    tile.column = group & 1;
-                    tile.groups = min(w.wide, wide_groups - group);
-                    tile.slices = (w.m + 63) / 64;
-                    if (kPlanes == 1) tile.extra = min(2, tile.slices - 2 * tile.i);
+                int mb, symmetric_tiles, per_row, whole;
+                bool is_wide;
+                const int now = slot;
+                if (leader) {
+                    // (not before the last tile's copies are issued: a block that held a second tile of a product would make that product twice as long)
+                    int t = 0;
+                    if (lane == 0) t = claim(P.c.done);
+                    t = __shfl_sync(0xffffffffu, t, 0);
+                    tile.k = -1;
+                    if (t < tiles) {
+                        while (round + 1 < P.rounds && t >= next_first) {
+                            ++round;
+                            next_first = load_global(&rounds[min(round + 1, P.rounds - 1)].first);
+                        }
+                        t -= load_global(&rounds[round].first);
+                        const int of_first = load_global(&rounds[round].of_first), cls = t >= of_first;
+                        if (cls) t -= of_first;
+                        const int* const words = reinterpret_cast<const int*>(&rounds[round].op[cls]);
+                        const int word = lane < kOpWords ? load_global(words + lane) : 0;
+                        const int kind = __shfl_sync(0xffffffffu, word, offsetof(Op, kind) / 4), jobs = __shfl_sync(0xffffffffu, word, offsetof(Op, jobs) / 4);
+                        const int gram = __shfl_sync(0xffffffffu, word, offsetof(Op, gram) / 4);
+                        is_wide = kind == ITERATE || kind == RESULT;
+                        whole = kind == POLY && gram;
+                        // (matrices of the first class come first, and their tiles count from 0; those of the second behind all of the first)
+                        const int n0 = P.first_class;
+                        const int lo = cls ? n0 : 0, hi = cls ? count : n0;
+                        const int* const starts = first[is_wide ? 2 : kind == SUM ? 3 : whole ? 0 : 1];
+                        const int base = starts[lo], per_job = is_wide ? 1 : jobs;
+                        int a = lo, b = hi - 1;
+                        while (a < b) {
+                            const int mid = (a + b + 1) / 2;
+                            if ((starts[mid] - base) * per_job <= t) a = mid; else b = mid - 1;
+                        }
+                        tile.k = a;
+                        t -= (starts[a] - base) * per_job;
+                        {
+                            const Work* const from = P.c.table + a;
+                            auto word = [](const uint32_t* p) { return static_cast<uint32_t>(load_global(reinterpret_cast<const int*>(p))); };
+                            w = {load_global(&from->s.m), load_global(&from->s.n), load_global(&from->nb), load_global(&from->wide), load_global(&from->fine),
+                                 load_global(&from->parts), {word(&from->x[0]), word(&from->x[1])}, word(&from->sym), word(&from->partial), load_global(&from->sx)};
+                        }
+                        mb = (w.m + kBlock - 1) / kBlock;
+                        symmetric_tiles = symmetric_count<kPair>(mb) * w.fine;
+                        const int wide_groups = (w.n + 63) / 64;
+                        per_row = (wide_groups + w.wide - 1) / w.wide;
+                        tile.extra = tile.job = tile.column = tile.part = tile.from = 0;
+                        if (is_wide) {
+                            tile.i = t / per_row;
+                            const int group = t % per_row * w.wide;
+                            tile.j = group >> 1;
+                            tile.column = group & 1;
+                            tile.groups = min(w.wide, wide_groups - group);
+                            tile.slices = (w.m + 63) / 64;
+                            if (kPlanes == 1) tile.extra = min(2, tile.slices - 2 * tile.i);
+                        } else {
+                            const int fine = kind == SUM ? 2 : w.fine;
+                            if (whole) {
+                                tile.part = t / symmetric_tiles;
+                                t %= symmetric_tiles;
+                            } else if (kind != SUM && t >= symmetric_tiles) {
+                                t -= symmetric_tiles;
+                                tile.job = 1;
+                            }
+                            if (fine == 2) {
+                                tile.column = t & 1;
+                                t >>= 1;
+                            }
+                            // the row: of row i there are i (i + 1) / 2 tiles in front, of pair i twice as many
+                            auto in_front = [](int i) { return kBoth * (i * (i + 1) / 2); };
+                            tile.i = static_cast<int>((sqrtf(8.f / kBoth * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
+                            while (in_front(tile.i) > t) --tile.i;
+                            while (in_front(tile.i + 1) <= t) ++tile.i;
+                            tile.j = t - in_front(tile.i);
+                            tile.groups = max(0, min(3 - fine, (w.m - tile.j * kBlock + 63) / 64 - tile.column));
+                            const int all = ((whole ? w.n : w.m) + 63) / 64, share = whole ? (all + w.parts - 1) / w.parts : all;
+                            tile.from = tile.part * share;
+                            tile.slices = kind == SUM || tile.groups == 0 ? 0 : min(share, all - tile.from);
+                        }
+                        // pass it on
+                        if (!wait_other(&qempty_bar[slot], qparity ^ 1, nml::ERR_WAIT_EMPTY)) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane < kOpWords) reinterpret_cast<int*>(&queue[slot].op)[lane] = word;
+                        if (lane == 0) {
+                            queue[slot].k = tile.k, queue[slot].i = tile.i, queue[slot].j = tile.j, queue[slot].job = tile.job, queue[slot].column = tile.column;
+                            queue[slot].groups = tile.groups, queue[slot].part = tile.part, queue[slot].from = tile.from, queue[slot].slices = tile.slices, queue[slot].extra = tile.extra;
+                            queue[slot].w = w;
+                        }
+                        __syncwarp();
+                    } else {
+                        if (!wait_other(&qempty_bar[slot], qparity ^ 1, nml::ERR_WAIT_EMPTY)) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) queue[slot].k = -1;
+                        __syncwarp();
+                    }
+                    if (kPair) {  // to the other block
+                        const uint32_t to = nml::map_to_cta(nml::smem_u32(&queue[slot]), 1);
+                        const uint32_t* const words = reinterpret_cast<const uint32_t*>(&queue[slot]);
+                        for (int e = lane; e < static_cast<int>(sizeof(Tile) / 4); e += 32) store_remote(to + 4 * e, words[e]);
+                        __syncwarp();
+                    }
                 } else {
-                    const int fine = kind == SUM ? 2 : w.fine;
-                    if (whole) {
-                        tile.part = t / symmetric_tiles;
-                        t %= symmetric_tiles;
-                    } else if (kind != SUM && t >= symmetric_tiles) {
-                        t -= symmetric_tiles;
-                        tile.job = 1;
+                    if (!wait_other(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL)) {
+                        ok = false;
+                        break;
                     }
-                    if (fine == 2) {
-                        tile.column = t & 1;
-                        t >>= 1;
-                    }
-                    tile.i = static_cast<int>((sqrtf(8.f * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
-                    while (lower(tile.i, 0) > t) --tile.i;
-                    while (lower(tile.i + 1, 0) <= t) ++tile.i;
-                    tile.j = t - lower(tile.i, 0);
-                    tile.groups = max(0, min(3 - fine, (w.m - tile.j * kBlock + 63) / 64 - tile.column));
-                    const int all = ((whole ? w.n : w.m) + 63) / 64, share = whole ? (all + w.parts - 1) / w.parts : all;
-                    tile.from = tile.part * share;
-                    tile.slices = kind == SUM || tile.groups == 0 ? 0 : min(share, all - tile.from);
+                    tile = queue[slot];
+                    if (tile.k < 0) break;
+                    w = tile.w;
+                    is_wide = tile.op.kind == ITERATE || tile.op.kind == RESULT;
+                    whole = tile.op.kind == POLY && tile.op.gram;
+                    mb = (w.m + kBlock - 1) / kBlock;
+                    symmetric_tiles = symmetric_count<kPair>(mb) * w.fine;
+                    per_row = ((w.n + 63) / 64 + w.wide - 1) / w.wide;
                 }
+                const Op& op = queue[now].op;  // (the producer's own copy stays until it comes round to the slot again; the other block's until it is given back)
                 // the matrix's earlier products: to be waited for before its copies are issued, or, where there are none, before it is passed on
                 auto wait_for_matrix = [&](const Op& op) {
-                    const int need = kEpilogueWarps * (op.gram_before * symmetric_tiles * w.parts + op.symmetric_before * symmetric_tiles +
-                                                       op.wide_before * mb * per_row + op.sum_before * (w.parts > 1 ? 2 * blocks : 0));
+                    const int need = kReports * (op.gram_before * symmetric_tiles * w.parts + op.symmetric_before * symmetric_tiles +
+                                                       op.wide_before * ((mb + kBoth - 1) / kBoth) * per_row + op.sum_before * (w.parts > 1 ? 2 * lower(mb, 0) : 0));
                     if (need == 0) return true;
                     int gave_up = 0;
                     if (lane == 0) {
@@ -710,98 +792,191 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                     fence_proxies();
                     return true;
                 };
-                // pass it on
-                if (!wait(&qempty_bar[slot], qparity ^ 1, nml::ERR_WAIT_EMPTY)) {
-                    ok = false;
-                    break;
+                if (leader) {
+                    if (tile.k >= 0 && tile.slices == 0 && !wait_for_matrix(op)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        nml::mbar_arrive(nml::smem_u32(&qfull_bar[now]));
+                        if (kPair) nml::mbar_arrive_cluster(nml::map_to_cta(nml::smem_u32(&qfull_bar[now]), 1));
+                    }
                 }
-                if (lane < kOpWords) reinterpret_cast<int*>(&queue[slot].op)[lane] = word;
-                if (lane == 0) {
-                    queue[slot].k = tile.k, queue[slot].i = tile.i, queue[slot].j = tile.j, queue[slot].job = tile.job, queue[slot].column = tile.column;
-                    queue[slot].groups = tile.groups, queue[slot].part = tile.part, queue[slot].slices = tile.slices, queue[slot].extra = tile.extra;
-                    queue[slot].w = w;
-                }
-                __syncwarp();
-                const Op& op = queue[slot].op;  // (the producer's own copy stays until it comes round to the slot again)
-                if (tile.slices == 0 && !wait_for_matrix(op)) {
-                    ok = false;
-                    break;
-                }
-                if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qfull_bar[slot]));
                 if (++slot == kQueue) slot = 0, qparity ^= 1;
-                if (tile.slices == 0) continue;
-                if (!wait_for_matrix(op)) {
-                    ok = false;
-                    break;
+                if (tile.k < 0) break;
+                if (tile.slices > 0) {
+                    if (!wait_for_matrix(op)) {
+                        ok = false;
+                        break;
+                    }
+                    // its K slices; a ring of stages of the other size only begins when the last one's are free
+                    const uint32_t stage_bytes = is_wide ? kWideStage : kNarrow, b_bytes = is_wide ? kWideB : kNarrowB;
+                    if (now_stage != stage_bytes) {
+                        for (int e = 0; ok && e < stages; ++e)
+                            if (used >> e & 1) ok = wait(&empty_bar[e], (parity >> e & 1) ^ 1, nml::ERR_WAIT_EMPTY);
+                        if (!ok) break;
+                        used = 0;
+                        s = 0;
+                        now_stage = stage_bytes;
+                        stages = min(kMaxStages, static_cast<int>(kRing / stage_bytes));
+                    }
+                    const bool same = !kPair && whole && tile.i == tile.j;
+                    const int b_pieces = kPair ? (is_wide ? 2 : 1) : same ? 0 : tile.groups, pieces = kPlanes * (2 + b_pieces);
+                    const bool is_a = lane < 2 * kPlanes;
+                    const int at = is_a ? lane : lane - 2 * kPlanes, per = is_a ? 2 : max(1, b_pieces);
+                    const int plane = at / per, piece = at % per;
+                    const uint32_t dst = (is_a ? plane * kHalf : kPlanes * kHalf + plane * b_bytes) + piece * kPiece;
+                    const uint32_t buffer = symmetric_first(w, is_wide ? op.left : is_a ? op.job[tile.job].left : op.job[tile.job].right);
+                    const uint32_t x = op.from ? w.x[1] : w.x[0];
+                    // block row of the left operand; a pair that is one row short has its last one twice.  K-major up to `turn`, for both rows alike
+                    const int left_row = min(kBoth * tile.i + static_cast<int>(rank), mb - 1), turn = is_a ? kBoth * tile.i : tile.j;
+                    const int last_group = (w.n + 63) / 64 - 1 - 2 * tile.j;
+                    for (int q = 0; q < tile.slices + tile.extra; ++q) {
+                        if (used >> s & 1) {
+                            if (!wait(&empty_bar[s], (parity >> s & 1) ^ 1, nml::ERR_WAIT_EMPTY)) {
+                                ok = false;
+                                break;
+                            }
+                        }
+                        const uint32_t bar = nml::smem_u32(&full_bar[s]), to = nml::smem_u32(smem) + s * stage_bytes + dst;
+                        if (lane == 0 && leader) nml::mbar_arrive_expect_tx(bar, kBoth * pieces * kPiece);
+                        __syncwarp();
+                        if (lane < pieces) {
+                            const bool low = q >= tile.slices;  // a I times X's low half
+                            const int kq = low ? 2 * tile.i + q - tile.slices : tile.from + q, kb = kq >> 1, h = kq & 1;
+                            const int group = is_a ? piece : !kPair ? piece + tile.column : is_wide ? min(2 * static_cast<int>(rank) + piece, last_group) : static_cast<int>(rank);
+                            const uint8_t* from;
+                            const uint32_t straight = (h * 2 + group) * kPiece, across = (group * 2 + h) * kPiece;  // K-major; MN-major
+                            auto symmetric = [&](int row) {
+                                return kb <= turn ? block_at(P.c.blocks, buffer, lower(row, kb)) + straight : block_at(P.c.blocks, buffer, lower(kb, row)) + across;
+                            };
+                            if (!is_wide) {
+                                const int row = is_a ? left_row : tile.j;
+                                from = whole ? block_at(P.c.blocks, x, row * w.nb + kb) + straight : symmetric(row);
+                            } else if (is_a) {
+                                from = low ? block_at(P.c.blocks, op.identity, 0) + straight : symmetric(left_row);
+                            } else {  // X's rows along K: two 64-column groups to a block
+                                from = block_at(P.c.blocks, x, kb * w.nb + tile.j + (group >> 1)) + (low ? kPlane : 0) + ((group & 1) * 2 + h) * kPiece;
+                            }
+                            from += plane * kPlane;
+                            if (kPair) nml::tma_load_2d_pair(to, &P.map, nml::map_to_cta(bar, 0), 0, static_cast<int>((from - P.c.blocks) / kMapRow));
+                            else nml::bulk_load(to, from, kPiece, bar);
+                        }
+                        __syncwarp();
+                        used |= 1u << s;
+                        parity ^= 1u << s;
+                        if (++s == stages) s = 0;
+                    }
                 }
-
-                // its K slices; a ring of stages of the other size only begins when the last one's are free
-                const uint32_t stage_bytes = is_wide ? kWideStage : kNarrow, b_bytes = is_wide ? 2 * kHalf : kHalf;
-                if (now_stage != stage_bytes) {
-                    for (int e = 0; ok && e < stages; ++e)
-                        if (used >> e & 1) ok = wait(&empty_bar[e], (parity >> e & 1) ^ 1, nml::ERR_WAIT_EMPTY);
-                    if (!ok) break;
-                    used = 0;
-                    s = 0;
-                    now_stage = stage_bytes;
-                    stages = kRing / stage_bytes;
+                if (!ok) break;
+                if (kPair && !leader) {
+                    __syncwarp();
+                    if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qempty_bar[now]));
                 }
-                const bool same = whole && tile.i == tile.j;
-                const int b_pieces = same ? 0 : tile.groups, pieces = kPlanes * (2 + b_pieces);
-                const bool is_a = lane < 2 * kPlanes;
-                const int at = is_a ? lane : lane - 2 * kPlanes, per = is_a ? 2 : max(1, b_pieces);
-                const int plane = at / per, piece = at % per;
-                const uint32_t dst = (is_a ? plane * kHalf : kPlanes * kHalf + plane * b_bytes) + piece * kPiece;
-                const uint32_t buffer = symmetric_first(w, is_wide ? op.left : is_a ? op.job[tile.job].left : op.job[tile.job].right);
-                const uint32_t x = op.from ? w.x[1] : w.x[0];
-                for (int q = 0; q < tile.slices + tile.extra; ++q) {
-                    if (used >> s & 1) {
-                        if (!wait(&empty_bar[s], (parity >> s & 1) ^ 1, nml::ERR_WAIT_EMPTY)) {
-                            ok = false;
+            }
+            if (leader && (!ok || *abort_flag)) {  // no copy may be in flight when the block's shared memory goes away
+                for (int e = 0; e < stages; ++e) {
+                    if (!(used >> e & 1)) continue;
+                    const uint64_t t0 = nml::globaltimer_ns();
+                    while (!nml::mbar_try_wait(nml::smem_u32(&full_bar[e]), (parity >> e & 1) ^ 1)) {
+                        if (nml::globaltimer_ns() - t0 > 2000000ull) {
+                            if (lane == 0) atomicCAS(P.err, 0, nml::ERR_WAIT_DRAIN);
                             break;
                         }
                     }
-                    const uint32_t bar = nml::smem_u32(&full_bar[s]), to = nml::smem_u32(smem) + s * stage_bytes + dst;
-                    if (lane == 0) nml::mbar_arrive_expect_tx(bar, pieces * kPiece);
-                    __syncwarp();
-                    if (lane < pieces) {
-                        const bool low = q >= tile.slices;  // a I times X's low half
-                        const int kq = low ? 2 * tile.i + q - tile.slices : tile.from + q, kb = kq >> 1, h = kq & 1;
-                        const int group = is_a ? piece : piece + tile.column;
-                        const uint8_t* from;
-                        const uint32_t straight = (h * 2 + group) * kPiece, across = (group * 2 + h) * kPiece;  // K-major; MN-major
-                        auto symmetric = [&](int row) {
-                            return kb <= row ? block_at(P.c.blocks, buffer, lower(row, kb)) + straight : block_at(P.c.blocks, buffer, lower(kb, row)) + across;
-                        };
-                        if (!is_wide) {
-                            const int row = is_a ? tile.i : tile.j;
-                            from = whole ? block_at(P.c.blocks, x, row * w.nb + kb) + straight : symmetric(row);
-                        } else if (is_a) {
-                            from = low ? block_at(P.c.blocks, op.identity, 0) + straight : symmetric(tile.i);
-                        } else {  // X's rows along K: two 64-column groups to a block
-                            from = block_at(P.c.blocks, x, kb * w.nb + tile.j + (group >> 1)) + (low ? kPlane : 0) + ((group & 1) * 2 + h) * kPiece;
+                }
+            }
+        } else if (kPair && warp == 1 && !leader) {
+            // ------------------------------------------------------------ tells the first block which tiles this one is through with
+            int slot = 0;
+            uint32_t qparity = 0;
+            while (true) {
+                if (!wait_other(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL) || queue[slot].k < 0) break;
+                if (!wait(&qempty_bar[slot], qparity, nml::ERR_WAIT_EMPTY)) break;
+                if (lane == 0) nml::mbar_arrive_cluster(nml::map_to_cta(nml::smem_u32(&qempty_bar[slot]), 0));
+                __syncwarp();
+                if (++slot == kQueue) slot = 0, qparity ^= 1;
+            }
+        } else if (warp == 1) {
+            // ------------------------------------------------------------ MMA
+            int slot = 0, s = 0, stages = 0, unit = 0;
+            uint32_t qparity = 0, parity = 0, tparity = 0, pairs = 0, now_stage = 0;  // pairs: of units whose last use was by both
+            bool ok = true;
+            const uint32_t ring = nml::smem_u32(smem);
+            auto commit = [&](uint64_t* bar) {  // (of a pair in both blocks)
+                if (kPair) nml::umma_commit_pair(nml::smem_u32(bar)); else nml::umma_commit(nml::smem_u32(bar));
+            };
+            while (ok) {
+                if (!wait(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL)) {
+                    ok = false;
+                    break;
+                }
+                const int k = queue[slot].k, row = queue[slot].i, column = queue[slot].j, groups = queue[slot].groups, real = queue[slot].slices;
+                const int slices = real + queue[slot].extra, kind = queue[slot].op.kind, in_block = queue[slot].column;
+                const bool is_wide = kind == ITERATE || kind == RESULT, gram = queue[slot].op.gram != 0;
+                if (k < 0) break;
+                __syncwarp();
+                if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qempty_bar[slot]));
+                if (++slot == kQueue) slot = 0, qparity ^= 1;
+                if (slices == 0) continue;
+                const uint32_t stage_bytes = is_wide ? kWideStage : kNarrow, b_bytes = is_wide ? kWideB : kNarrowB;
+                if (now_stage != stage_bytes) {
+                    s = 0;
+                    now_stage = stage_bytes;
+                    stages = min(kMaxStages, static_cast<int>(kRing / stage_bytes));
+                }
+                const bool same = !kPair && gram && row == column;
+                for (int q = 0; q < slices; ++q) {
+                    if (kPlanes == 2 || q == 0) {
+                        // TMEM is four units of 128 columns, each with its barriers; a wide tile takes two, and the first one's barriers
+                        if (is_wide && (unit & 1)) unit = (unit + 1) & 3;
+                        const int pair = unit >> 1;
+                        auto drained = [&](int u) { return wait(&tempty_bar[u], (tparity >> u & 1) ^ 1, nml::ERR_WAIT_TMEM_EMPTY); };
+                        ok = drained(unit) && (!is_wide || drained(unit + 1)) && (is_wide || !(unit & 1) || !(pairs >> pair & 1) || drained(unit - 1));
+                        if (!ok) break;
+                        if (is_wide) pairs |= 1u << pair; else pairs &= ~(1u << pair);
+                        nml::tc_fence_after();
+                    }
+                    if (!wait(&full_bar[s], parity >> s & 1, nml::ERR_WAIT_FULL)) {
+                        ok = false;
+                        break;
+                    }
+                    nml::tc_fence_after();
+                    const bool low = q >= real, last = kPlanes == 2 || q + 1 == slices;
+                    const int kb = q >> 1;
+                    const int a_mn = !gram && !low && kb > kBoth * row;
+                    const int b_mn = is_wide ? 1 : !gram && kb > column;
+                    const uint32_t idesc = nml::make_instr_desc(0, a_mn, b_mn, kBoth * 128, kPair ? (is_wide ? 256 : 128) : groups * 64);
+                    const uint32_t sa = ring + s * stage_bytes, sb = same ? sa + in_block * kPiece : sa + kPlanes * kHalf, bp = same ? kHalf : b_bytes;
+                    if (nml::elect_one()) {
+                        const uint64_t a0 = nml::make_smem_desc(sa, kPiece, 1024, 2), b0 = nml::make_smem_desc(sb, kPiece, 1024, 2);
+                        const uint32_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
+#pragma unroll
+                        for (int p = kPlanes == 2 ? 2 : 0; p >= 0; --p) {  // low x high, high x low, high x high
+                            uint64_t ad = a0 + (p == 2 ? kHalf >> 4 : 0), bd = b0 + (p == 1 ? bp >> 4 : 0);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e, ad += a_step, bd += b_step) {
+                                const bool add = kPlanes == 2 ? e > 0 || p < 2 : e > 0 || q > 0;
+                                if (kPair) nml::umma_f16_pair(tmem + unit * 128, ad, bd, idesc, add); else nml::umma_f16(tmem + unit * 128, ad, bd, idesc, add);
+                            }
                         }
-                        nml::bulk_load(to, from + plane * kPlane, kPiece, bar);
+                        commit(&empty_bar[s]);
+                        if (last) commit(&tfull_bar[unit]);
                     }
                     __syncwarp();
-                    used |= 1u << s;
                     parity ^= 1u << s;
                     if (++s == stages) s = 0;
+                    if (last) {
+                        tparity ^= 1u << unit;
+                        unit = (unit + (is_wide ? 2 : 1)) & 3;
+                    }
                 }
-            } else {
-                if (!wait(&qempty_bar[slot], qparity ^ 1, nml::ERR_WAIT_EMPTY)) ok = false;
-                if (ok && lane == 0) {
-                    queue[slot].k = -1;
-                    nml::mbar_arrive(nml::smem_u32(&qfull_bar[slot]));
-                }
-                break;
             }
-        }
-        if (!ok || *abort_flag) {  // no copy may be in flight when the block's shared memory goes away
-            for (int e = 0; e < stages; ++e) {
-                if (!(used >> e & 1)) continue;
+            if (!ok) {  // the products issued so far still read shared memory and write TMEM
+                if (nml::elect_one()) commit(&drain_bar);
+                __syncwarp();
                 const uint64_t t0 = nml::globaltimer_ns();
-                while (!nml::mbar_try_wait(nml::smem_u32(&full_bar[e]), (parity >> e & 1) ^ 1)) {
+                while (!nml::mbar_try_wait(nml::smem_u32(&drain_bar), 0)) {
                     if (nml::globaltimer_ns() - t0 > 2000000ull) {
                         if (lane == 0) atomicCAS(P.err, 0, nml::ERR_WAIT_DRAIN);
                         break;
@@ -809,88 +984,6 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 }
             }
         }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA
-        int slot = 0, s = 0, stages = 0, unit = 0;
-        uint32_t qparity = 0, parity = 0, tparity = 0, pairs = 0, now_stage = 0;  // pairs: of units whose last use was by both
-        bool ok = true;
-        const uint32_t ring = nml::smem_u32(smem);
-        while (ok) {
-            if (!wait(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL)) {
-                ok = false;
-                break;
-            }
-            const int k = queue[slot].k, row = queue[slot].i, column = queue[slot].j, groups = queue[slot].groups, real = queue[slot].slices;
-            const int slices = real + queue[slot].extra, kind = queue[slot].op.kind, in_block = queue[slot].column;
-            const bool is_wide = kind == ITERATE || kind == RESULT, gram = queue[slot].op.gram != 0;
-            if (k < 0) break;
-            __syncwarp();
-            if (lane == 0) nml::mbar_arrive(nml::smem_u32(&qempty_bar[slot]));
-            if (++slot == kQueue) slot = 0, qparity ^= 1;
-            if (slices == 0) continue;
-            const uint32_t stage_bytes = is_wide ? kWideStage : kNarrow, b_bytes = is_wide ? 2 * kHalf : kHalf;
-            if (now_stage != stage_bytes) {
-                s = 0;
-                now_stage = stage_bytes;
-                stages = kRing / stage_bytes;
-            }
-            const bool same = gram && row == column;
-            for (int q = 0; q < slices; ++q) {
-                if (kPlanes == 2 || q == 0) {
-                    // TMEM is four units of 128 columns, each with its barriers; a wide tile takes two, and the first one's barriers
-                    if (is_wide && (unit & 1)) unit = (unit + 1) & 3;
-                    const int pair = unit >> 1;
-                    auto drained = [&](int u) { return wait(&tempty_bar[u], (tparity >> u & 1) ^ 1, nml::ERR_WAIT_TMEM_EMPTY); };
-                    ok = drained(unit) && (!is_wide || drained(unit + 1)) && (is_wide || !(unit & 1) || !(pairs >> pair & 1) || drained(unit - 1));
-                    if (!ok) break;
-                    if (is_wide) pairs |= 1u << pair; else pairs &= ~(1u << pair);
-                    nml::tc_fence_after();
-                }
-                if (!wait(&full_bar[s], parity >> s & 1, nml::ERR_WAIT_FULL)) {
-                    ok = false;
-                    break;
-                }
-                nml::tc_fence_after();
-                const bool low = q >= real, last = kPlanes == 2 || q + 1 == slices;
-                const int kb = q >> 1;
-                const int a_mn = !gram && !low && kb > row;
-                const int b_mn = is_wide ? 1 : !gram && kb > column;
-                const uint32_t idesc = nml::make_instr_desc(0, a_mn, b_mn, 128, groups * 64);
-                const uint32_t sa = ring + s * stage_bytes, sb = same ? sa + in_block * kPiece : sa + kPlanes * kHalf, bp = same ? kHalf : b_bytes;
-                if (nml::elect_one()) {
-                    const uint64_t a0 = nml::make_smem_desc(sa, kPiece, 1024, 2), b0 = nml::make_smem_desc(sb, kPiece, 1024, 2);
-                    const uint32_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
-#pragma unroll
-                    for (int p = kPlanes == 2 ? 2 : 0; p >= 0; --p) {  // low x high, high x low, high x high
-                        uint64_t ad = a0 + (p == 2 ? kHalf >> 4 : 0), bd = b0 + (p == 1 ? bp >> 4 : 0);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e, ad += a_step, bd += b_step)
-                            nml::umma_f16(tmem + unit * 128, ad, bd, idesc, kPlanes == 2 ? e > 0 || p < 2 : e > 0 || q > 0);
-                    }
-                    nml::umma_commit(nml::smem_u32(&empty_bar[s]));
-                    if (last) nml::umma_commit(nml::smem_u32(&tfull_bar[unit]));
-                }
-                __syncwarp();
-                parity ^= 1u << s;
-                if (++s == stages) s = 0;
-                if (last) {
-                    tparity ^= 1u << unit;
-                    unit = (unit + (is_wide ? 2 : 1)) & 3;
-                }
-            }
-        }
-        if (!ok) {  // the products issued so far still read shared memory and write TMEM
-            if (nml::elect_one()) nml::umma_commit(nml::smem_u32(&drain_bar));
-            __syncwarp();
-            const uint64_t t0 = nml::globaltimer_ns();
-            while (!nml::mbar_try_wait(nml::smem_u32(&drain_bar), 0)) {
-                if (nml::globaltimer_ns() - t0 > 2000000ull) {
-                    if (lane == 0) atomicCAS(P.err, 0, nml::ERR_WAIT_DRAIN);
-                    break;
-                }
-            }
-        }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         // ------------------------------------------------------------ epilogue: a thread to a row and half of the columns of the tile
@@ -908,8 +1001,8 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
         };
         while (true) {
             if (!__all_sync(0xffffffffu, nml::mbar_test(nml::smem_u32(&qfull_bar[slot]), qparity))) report();
-            if (!wait(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL)) break;
-            const int k = queue[slot].k, tile_i = queue[slot].i, tile_j = queue[slot].j, groups = queue[slot].groups, slices = queue[slot].slices;
+            if (!wait_other(&qfull_bar[slot], qparity, nml::ERR_WAIT_FULL)) break;
+            const int k = queue[slot].k, tile_i = kBoth * queue[slot].i + static_cast<int>(rank), tile_j = queue[slot].j, groups = queue[slot].groups, slices = queue[slot].slices;
             const int in_block = queue[slot].column, part = queue[slot].part;
             const int kind = queue[slot].op.kind, gram = queue[slot].op.gram, from_x = queue[slot].op.from;
             const Symmetric job = queue[slot].op.job[queue[slot].job];
@@ -949,7 +1042,10 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 }
                 nml::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) nml::mbar_arrive(nml::smem_u32(&tempty_bar[unit]));
+                if (lane == 0) {
+                    if (kPair) nml::mbar_arrive_remote(nml::map_to_cta(nml::smem_u32(&tempty_bar[unit]), 0));
+                    else nml::mbar_arrive(nml::smem_u32(&tempty_bar[unit]));
+                }
                 tparity ^= 1u << unit;
                 unit = (unit + (is_wide ? 2 : 1)) & 3;
             }
@@ -1054,7 +1150,8 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                                     acc[c][4 * q] += v.x, acc[c][4 * q + 1] += v.y, acc[c][4 * q + 2] += v.z, acc[c][4 * q + 3] += v.w;
                                 }
                 }
-                const int matrices = !in_use || partial || groups == 0 ? 0 : kind == POLY || kind == SUM ? 2 : 1;
+                const bool above = kPair && !iterate && tile_j > tile_i;  // the diagonal
+                const int matrices = !in_use || above || partial || groups == 0 ? 0 : kind == POLY || kind == SUM ? 2 : 1;
 #pragma unroll 1
                 for (int e = 0; e < matrices; ++e) {  // (A and P: f0 is a power of two)
                     scale(e ? op_f1 / job.f0 : (iterate ? op_f1 : job.f0) * over);
@@ -1068,10 +1165,16 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
     }
     nml::tc_fence_before();
     __syncthreads();
+    if (kPair) nml::cluster_sync_all();  // (neither block leaves while the other may still reach it)
     nml::tc_fence_after();
     if (warp == 0) {
-        nml::tmem_relinquish();
-        nml::tmem_dealloc(tmem, 512);
+        if (kPair) {
+            nml::tmem_relinquish_pair();
+            nml::tmem_dealloc_pair(tmem, 512);
+        } else {
+            nml::tmem_relinquish();
+            nml::tmem_dealloc(tmem, 512);
+        }
     }
 }
 
@@ -1187,22 +1290,34 @@ struct Plan {
     int sums = 0, halves = 0, first_class = 0;
     int gram_tiles[kClasses] = {0, 0}, symmetric_tiles[kClasses] = {0, 0}, update_tiles[kClasses] = {0, 0}, sum_tiles[kClasses] = {0, 0};
     uint32_t blocks = 0, identity = 0;
+    bool pair = false;
     size_t sums_at = 0, rounds_at = 0, done_at = 0, blocks_at = 0, bytes = 0;
 };
 // Lays a group of at most kGroup matrices out, chained ones first, longer ones first; the sources are set.
 static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
     Plan p;
     long long blocks = 0, wide_tiles[3] = {0, 0, 0};
+    double single = 0.0, paired = 0.0;
     for (int k = 0; k < count; ++k) {
         w[k].chained = steps > 1 && chained(w[k].s, math);
         w[k].mb = (w[k].s.m + kBlock - 1) / kBlock;
         w[k].nb = (w[k].s.n + kBlock - 1) / kBlock;
         blocks += w[k].mb * (w[k].mb + 1) / 2;
+        // its work in K slices of narrow tiles, one of Q X as 1.5 of them
+        const double mk = 2.0 * w[k].mb, nk = 2.0 * w[k].nb, across = 0.375 * nk * mk, pairs = (w[k].mb + 1) / 2;
+        single += w[k].mb * (w[k].mb + 1) / 2 * (nk + 2 * mk) + w[k].mb * across;
+        paired += 2 * symmetric_count<true>(w[k].mb) * (nk + 2 * mk) + 2 * pairs * across;
         for (int e = 0; e < 3; ++e) wide_tiles[e] += static_cast<long long>(w[k].mb) * (((w[k].s.n + 63) / 64 + (1 << e) - 1) >> e);
     }
-    // Where a round has few tiles: two to a block, narrow ones of Q X, and X X^T with its long K in parts, at least eight slices each (XXX).
+    // Where a round has few tiles: two to a block, narrow ones of Q X, and X X^T with its long K in parts, at least eight slices each
+    // (together: 1024 x 4096 384 us instead of 484, 128 x 2048 175 / 205, 512 x 512 185 / 217).
     const int fine = 2 * blocks <= sms ? 2 : 1, spare = static_cast<int>(std::max<long long>(1, sms / (blocks * fine)));
     const int wide = wide_tiles[0] <= sms ? 1 : wide_tiles[1] <= sms ? 2 : 4;
+    // Pairs of blocks (see the kernel), where every round has tiles for all SMs and little of a pair's work is lost above the diagonal or for an
+    // odd row: 4096 x 4096 3.5 ms instead of 4.5, 2048 x 8192 970 us / 1197, 8 of 512 x 2048 345 / 386, 30 of 256 x 1024 261 / 278; against it 30 of
+    // 640 x 640, five rows each, 843 / 685 (pairs do 1.38 times the work), four of 512 x 2048 among 60 of 128 x 1152 425 / 378.  "f16" would
+    // gain nothing (4096 x 4096 2.5 ms / 2.35): its slices are so short that the copies' issue paces them.
+    p.pair = math == NML_MATH_3XF16 && fine == 1 && spare == 1 && wide == 4 && sms >= 2 && paired <= 1.2 * single;
     std::sort(w, w + count, [](const Work& a, const Work& b) {
         if (a.chained != b.chained) return a.chained > b.chained;
         if (a.s.m != b.s.m) return a.s.m > b.s.m;
@@ -1211,7 +1326,7 @@ static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
     int gram = 0, symmetric = 0, update = 0, sum = 0;
     for (int k = 0; k < count; ++k) {
         Work& v = w[k];
-        const int c = v.chained ? 0 : 1, own = v.mb * (v.mb + 1) / 2, slices = (v.s.n + 63) / 64;
+        const int c = v.chained ? 0 : 1, own = v.mb * (v.mb + 1) / 2, tiles_of = p.pair ? symmetric_count<true>(v.mb) : own, slices = (v.s.n + 63) / 64;
         if (v.chained) p.first_class = k + 1;
         v.first_sum = p.sums;
         v.sums = static_cast<int>((static_cast<long long>(v.s.m) * v.s.n + kSumElements - 1) / kSumElements);
@@ -1227,9 +1342,9 @@ static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
             *all += n;
             *of_class += n;
         };
-        tiles(&v.first_gram, &gram, &p.gram_tiles[c], own * fine * v.parts);
-        tiles(&v.first_symmetric, &symmetric, &p.symmetric_tiles[c], own * fine);
-        tiles(&v.first_update, &update, &p.update_tiles[c], v.mb * ((slices + wide - 1) / wide));
+        tiles(&v.first_gram, &gram, &p.gram_tiles[c], tiles_of * fine * v.parts);
+        tiles(&v.first_symmetric, &symmetric, &p.symmetric_tiles[c], tiles_of * fine);
+        tiles(&v.first_update, &update, &p.update_tiles[c], (p.pair ? (v.mb + 1) / 2 : v.mb) * ((slices + wide - 1) / wide));
         tiles(&v.first_parts, &sum, &p.sum_tiles[c], v.parts > 1 ? 2 * own : 0);
         for (uint32_t* at : {&v.x[0], &v.x[1]}) *at = p.blocks, p.blocks += v.mb * v.nb;
         v.sym = p.blocks;
@@ -1456,12 +1571,15 @@ static int run_group(Work* w, int count, const Call& call, const Steps& steps, v
     const int blocks = p.halves + 2 * pack.identities + 1;
     if (pack.rounds <= kFewRounds) launch_pack<kFewRounds>(pack, call, blocks, st);
     else launch_pack<kMaxRounds>(pack, call, blocks, st);
-    const ProductParams q = {c, err, static_cast<unsigned long long>(1.5e9 + 2e3 * slices), pack.rounds, static_cast<int>(tiles), p.first_class,
+    ProductParams q = {{}, c, err, static_cast<unsigned long long>(1.5e9 + 2e3 * slices), pack.rounds, static_cast<int>(tiles), p.first_class,
                              call.out_dtype == NML_F16, call.apply, call.keep, call.rate};
+    if (p.pair)
+        if (const int rc = nml::encode_rows(&q.map, c.blocks, kMapRow / 2, static_cast<size_t>(p.blocks) * (2 * kPlane / kMapRow), kPiece / kMapRow)) return rc;
     // (no more blocks than a round has tiles)
-    const int grid = static_cast<int>(std::min<long long>(widest, sms));
-    if (call.math == NML_MATH_F16) nml::launch(ortho_product_kernel<1>, grid, kThreads, kProductSmem, st, q);
-    else nml::launch(ortho_product_kernel<2>, grid, kThreads, kProductSmem, st, q);
+    const int each = p.pair ? 2 : 1, grid = each * static_cast<int>(std::min<long long>(widest, sms / each));
+    nml::launch_with(nml::overlaps(grid, nml::kSms), each,
+                     call.math == NML_MATH_F16 ? ortho_product_kernel<1, false> : p.pair ? ortho_product_kernel<2, true> : ortho_product_kernel<2, false>,
+                     grid, kThreads, kProductSmem, st, q);
     NMLO_CUDA(cudaGetLastError());
     nml::count_launches(3);
     return NML_OK;
@@ -1526,10 +1644,9 @@ static int workspace_of(int count, int math, int steps, F&& size, size_t* bytes)
 using namespace nml_ortho;
 
 int nml::prepare_ortho_kernels() {
-    NMLO_CUDA(cudaFuncSetAttribute(ortho_product_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem)));
-    NMLO_CUDA(cudaFuncSetAttribute(ortho_product_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem)));
     cudaFuncAttributes a;
-    for (auto f : {ortho_product_kernel<1>, ortho_product_kernel<2>}) {
+    for (auto f : {ortho_product_kernel<1, false>, ortho_product_kernel<2, false>, ortho_product_kernel<2, true>}) {
+        NMLO_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem)));
         NMLO_CUDA(cudaFuncGetAttributes(&a, f));
         if (a.numRegs != kLaunchRegs) return NML_ERR_UNSUPPORTED;  // (a build whose register split would not hold)
     }

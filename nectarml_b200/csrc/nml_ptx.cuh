@@ -130,15 +130,30 @@ __device__ __forceinline__ void abort_state_init(volatile int* abort_state, unsi
     *reinterpret_cast<volatile unsigned long long*>(abort_state + 2) = limit_ns ? limit_ns : NML_WAIT_LIMIT_NS;
 }
 
+// The same, and what the other block of a cluster has arrived with is visible.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kTryWaitHintNs)
+        : "memory");
+    return ok != 0;
+}
+
 // Bounded wait.  `abort_flag` points at the CTA's abort state (above); the others see a raised flag
 // within ~16 polls and leave too.  Returns false when the wait was abandoned.
-template <bool kPollFirst = false>
+template <bool kPollFirst = false, bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           int* err_word, int err_code) {
-    if (kPollFirst ? mbar_poll(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    if (kCluster ? mbar_try_wait_cluster(bar, parity) : kPollFirst ? mbar_poll(bar, parity) : mbar_try_wait(bar, parity)) return true;
     uint64_t t0 = 0;
     for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
         if ((it & 0xF) == 0) {
             if (*abort_flag) return false;
             uint64_t now = globaltimer_ns();
@@ -239,6 +254,11 @@ __device__ __forceinline__ void cluster_sync_all() {
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The same without ordering this thread's stores: for what the tensor core and the accumulators' readers pass to one another (tcgen05 fences order
+// that), while stores to memory are in flight.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // TMA loads whose completion may be signalled on the partner CTA's mbarrier
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1) {

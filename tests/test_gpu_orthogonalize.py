@@ -74,6 +74,19 @@ def test_half_precision(rows, cols):
 
 
 @MODES
+@pytest.mark.parametrize("shapes", [[(1601, 1700)], [(2000, 1537)], [(1550, 2600)], [(1100, 1100), (700, 2000), (65, 300), (1, 5), (900, 640)],
+                                    [(384, 1024)] * 15 + [(129, 4000), (300, 257)]], ids=str)
+def test_many_tiles(shapes, mode):
+    """Two blocks to a tile: an odd and an even number of block rows, one alone, ragged ends, beside matrices of one block row."""
+    gs = [gradient(r, c, seed=r + k) for k, (r, c) in enumerate(shapes)]
+    ys = ops.orthogonalize(gs, math=mode)
+    ops.device_status()
+    for g, y in zip(gs, ys):
+        assert off(y, plain(g)) <= TOL[mode], g.shape
+    assert all(torch.equal(a, b) for a, b in zip(ys, ops.orthogonalize(gs, math=mode)))
+
+
+@MODES
 def test_singular_values_and_vectors(mode):
     """What the operator is for: singular values near 1, the same singular vectors."""
     g = gradient(96, 250, seed=5)
