@@ -90,6 +90,28 @@ def test_sizes(rows, vocab, top, dtype):
     check_forward(logits((rows, vocab), dtype, vocab), tokens((rows,), vocab), top)
 
 
+@pytest.mark.parametrize("offset", [1e3, 1e6, 9e6, 1.1e7, 1e8, 1e10, 1e15, 1e20, 1e29, 1e31, 1e38])
+def test_large_offsets(offset):
+    """Only distances count, however far the logits lie from 0: the gradient too."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    for sign in (1, -1):
+        x = sign * offset * (1 + 1e-3 * torch.rand(40, 1, device=DEV, generator=g)) + logits((40, 777), torch.float32, 4)
+        x[3, 5:] = -math.inf
+        x[4, 5:] = torch.finfo(torch.float32).min
+        t = tokens((40,), 777)
+        t[3:5] = 2
+        r = check_forward(x, t, 3)
+        d, dh = logits((40,), torch.float32, 5), logits((40,), torch.float32, 6)
+        lp, _, h, _ = plain(x, t)
+        p = lp.exp()
+        want = -d[:, None] * p * (t >= 0)[:, None] - dh[:, None] * p * torch.where(p > 0, lp + h[:, None], 0.0)
+        want[torch.arange(40, device=DEV), t.clamp(min=0)] += torch.where(t >= 0, d, 0.0)
+        got = ops.token_log_probs_backward(x, t, r.stats, r.entropy, d, dh).double()
+        # y = log2 p is good to 2 u of x log2 e - M, whose size is that of M's rounding (up to 1 where it is not 0) and of y, and as log s is
+        size = (d.abs().max() + dh.abs().max() * 16).item()
+        assert bool(((got - want).abs() <= 2 * size * (8 + chain(777, torch.float32)) * U).all())
+
+
 @DTYPES
 def test_more_rows_than_blocks(dtype):
     check_forward(logits((10000, 257), dtype, 1), tokens((10000,), 257), 3)
