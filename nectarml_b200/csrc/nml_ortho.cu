@@ -27,8 +27,8 @@
 //           directions, 512 x 512: 1.0e-3; with X rounded 5.9e-3; all of U X in two products 1.2e-3.)
 //
 // Storage.  Every matrix between the products lies in blocks of 128 x 128, a block as two halves of 64 columns, each 128
-// rows of 128 bytes in the 128-byte swizzle that tcgen05.mma reads: a tile of an operand is contiguous, an untiled bulk copy brings it, no
-// tensor map is needed and ragged sizes are zeros in the blocks.  Such a half serves as K-major (its rows are the M or
+// rows of 128 bytes in the 128-byte swizzle that tcgen05.mma reads: a tile of an operand is contiguous, an untiled bulk copy brings it (a
+// tiled one where two blocks work together and the copy signals the other one's barrier) and ragged sizes are zeros in the blocks.  Such a half serves as K-major (its rows are the M or
 // N index) and as MN-major operand (its columns are), so X is read both ways, and a block of a symmetric matrix
 // stands for its mirror image too.
 #include <cuda_fp16.h>

@@ -6,7 +6,7 @@
 // (all of them polynomials of the first A, so symmetric; |G|^2 is the trace of G G^T).  The steps square the condition number and
 // amplify the error of A by up to a^2 = 11.9 each, so this is done in double: 2^-53 a^10 = 2e-11, and the result is rounded once.
 // With tiles of 128 in three products of halves a matrix of 64 x 147 took 116 us, 15 products of one tile, 7 us each: loads, flags and
-// stores.  Here it takes three launches: partial Gram matrices of 64 columns a block; the steps, a block to a matrix; Q G, 64 columns a block.
+// stores.  Here it takes 59 us in three launches: partial Gram matrices of 64 columns a block; the steps, a block to a matrix; Q G, 64 columns a block.
 // Bound by the double-precision pipe: 64 FMAs a clock and SM, from registers or by mma.sync alike (both measured), so the lower blocks of a
 // product of 64 x 64 matrices take 2304 clocks; mma.sync needs a quarter of the shared-memory reads.
 #pragma once

@@ -230,18 +230,16 @@ def _polynomial(steps: int, coefficients) -> Sequence[float]:
 
 
 def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps: int = 5, coefficients=ORTHOGONALIZE_COEFFICIENTS,
-                  eps: float = 1e-7, math: Optional[str] = None, out_dtype: Optional[torch.dtype] = None, out=None,
+                  eps: float = 1e-7, math: str = "3xf16", out_dtype: Optional[torch.dtype] = None, out=None,
                   ws: Optional[Workspace] = None) -> Union[torch.Tensor, List[torch.Tensor]]:
     """Orthogonalised matrices: ``steps`` of X <- (a I + b A + c A^2) X with A = X X^T, from G / (|G| + eps).
 
     ``g``: a matrix, a batch [n, rows, cols], or a sequence of such of any sizes, float32 or float16 (all of one), which go through
     the kernels together.  One dimension of a matrix is dense; transposed ones and slices of rows or columns are read in place.  ``math``: "3xf16"
-    (float32's default, as accurate as float32 products) or "f16" (float16's, 2 to 3e-3 of the result's norm).  ``out`` may be ``g``
+    (as accurate as float32 products) or "f16" (faster, good to 2 to 3e-3 of the result's norm).  ``out`` may be ``g``
     itself.  ``coefficients``: (a, b, c), or a row for each step."""
     single = isinstance(g, torch.Tensor)
     items = [g] if single else g
-    if math is None:
-        math = "f16" if len(items) and items[0].dtype == torch.float16 else "3xf16"
     if math not in _ORTHO_MATH:
         raise _lib.NectarB200Error(f"math: 'f16' or '3xf16', got {math!r}")
     r = _native.orthogonalize(items, out if out is None or not single else [out], _out_dtype(out_dtype), _ORTHO_MATH[math],
