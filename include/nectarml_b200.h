@@ -296,7 +296,7 @@ int nml_sgd_momentum_step(float* params, const float* grads, float* velocity, vo
  *                  fits fp16's range, which fp32 operands in general do not)
  *  NML_MATH_F16    operands rounded to fp16, except X where it is carried to the next step: 2 to 3e-3 of the result's norm
  * Zeros stay zeros; a matrix with a NaN or an infinity becomes NaN.  Matrices may be views: one of the strides (in elements) is 1, the other at least
- * the length of the dense run; a result may lie where its matrix does but must not overlap another one.  Coefficients under which a singular value could
+ * the length of the dense run; a result may lie where its matrix does (with its strides and type) but must not overlap another one.  Coefficients under which a singular value could
  * grow beyond 64 are NML_ERR_UNSUPPORTED.  Results are bitwise repeatable; the
  * order of sums, and whether a short side up to 64 is taken in double, follow from the group's sizes and the SMs in use. */
 typedef struct nml_matrix {
@@ -314,7 +314,7 @@ int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int o
  *   p = p (1 - lr weight_decay) - lr scale orthogonalize(u)     (rows > 0: a rows x cols matrix)
  *   p = p (1 - lr weight_decay) - lr u                          (rows = 0: a vector of cols values)
  * and, where param_f16 is set, the fp16 copy of p.  Nothing at all is changed when *found_inf (device int, see nml_grads_check;
- * may be NULL) is set.  No parameter, momentum or copy may overlap another.  Beside nml_sgd_momentum_step. */
+ * may be NULL) is set.  No parameter, momentum or copy may overlap another or a gradient.  Beside nml_sgd_momentum_step. */
 typedef struct nml_muon_param {
     float* param;
     const float* grad;

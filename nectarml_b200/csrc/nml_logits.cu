@@ -792,6 +792,7 @@ int nml_token_log_probs_backward(const void* logits, int dtype, long long rows, 
                                  long long d_pitch, void* stream) {
     if (!shape_ok(logits, dtype, rows, vocab, pitch) || !shape_ok(d_logits, dtype, rows, vocab, d_pitch)) return NML_ERR_INVALID;
     if (!targets || !stats || !d_log_probs || (d_entropy && !entropy)) return NML_ERR_INVALID;
+    if (d_logits == logits && d_pitch != pitch && rows > 1) return NML_ERR_INVALID;
     if (!aligned(4, stats, entropy, d_log_probs, d_entropy) || !aligned(8, targets)) return NML_ERR_INVALID;
     int* status;
     int sms;

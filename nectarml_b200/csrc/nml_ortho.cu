@@ -38,6 +38,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <iterator>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -1596,7 +1597,8 @@ static void set_sizes(Source& s, int rows, int cols) {
 }
 static bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// Whether what a step writes is in one place each: a parameter that is listed twice would be updated by two blocks at a time.
+// Whether what a step writes is in one place each: a parameter that is listed twice would be updated by two blocks at a time.  Gradients may be shared,
+// but lie apart from all that.
 static bool apart(const nml_muon_param* params, int count) {
     typedef std::pair<uintptr_t, uintptr_t> Range;
     try {
@@ -1614,7 +1616,25 @@ static bool apart(const nml_muon_param* params, int count) {
         std::sort(r.begin(), r.end());
         for (size_t k = 1; k < r.size(); ++k)
             if (r[k].first < r[k - 1].second) return false;
+        for (int k = 0; k < count; ++k) {
+            const uintptr_t from = reinterpret_cast<uintptr_t>(params[k].grad);
+            const uintptr_t to = from + 4 * static_cast<uintptr_t>(std::max(params[k].rows, 1)) * params[k].cols;
+            const auto next = std::lower_bound(r.begin(), r.end(), Range(to, 0));  // the first one that begins at its end or behind
+            if (next != r.begin() && std::prev(next)->second > from) return false;
+        }
         return true;
+    } catch (...) {
+        return false;
+    }
+}
+// Whether every result has a place of its own.
+static bool apart(const nml_matrix* matrices, int count) {
+    try {
+        std::vector<const void*> out;
+        out.reserve(count);
+        for (int k = 0; k < count; ++k) out.push_back(matrices[k].out);
+        std::sort(out.begin(), out.end());
+        return std::adjacent_find(out.begin(), out.end()) == out.end();
     } catch (...) {
         return false;
     }
@@ -1684,7 +1704,10 @@ int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int o
             return (c == 1 && r >= x.cols) || (r == 1 && c >= x.rows) || (x.rows == 1 && c == 1) || (x.cols == 1 && r == 1);
         };
         if (!dense(x.in_row, x.in_col) || !dense(x.out_row, x.out_col)) return NML_ERR_INVALID;
+        // in place: element by element
+        if (x.in == x.out && (in_dtype != out_dtype || x.in_row != x.out_row || x.in_col != x.out_col)) return NML_ERR_INVALID;
     }
+    if (!apart(matrices, count)) return NML_ERR_INVALID;
     Steps poly;
     if (!steps_of(coefficients, steps, &poly)) return NML_ERR_UNSUPPORTED;
     if (count > 0 && (!workspace || workspace_bytes < need)) return NML_ERR_WORKSPACE;

@@ -24,6 +24,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 import torch.distributed as dist
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from .ops import ConvGeometry
@@ -59,6 +60,7 @@ class ParamStore:
 
     def __init__(self, device) -> None:
         self.device = torch.device(device)
+        self._muon_ws = ops.Workspace()   # of its own: a captured step keeps it
         self.shapes: List[Tuple[int, ...]] = []
         self.offsets: List[int] = []
         self.n = 0
@@ -199,11 +201,10 @@ class ParamStore:
             self._muon = [[self._view(buf, i) for i in every] for buf in (self.p32, self.grad, self.vel, self.p16)]
         _lib.check(lib.nml_grads_check(self.grad.data_ptr(), self.n, inv_scale, self.found_inf.data_ptr(), torch.cuda.current_stream().cuda_stream))
         ops.muon_step(*self._muon, lr=lr, momentum=momentum, weight_decay=weight_decay, inv_scale=inv_scale, found_inf=self.found_inf,
-                      ws=_muon_ws)
+                      ws=self._muon_ws)
 
 
 _bn_ws = ops.Workspace()
-_muon_ws = ops.Workspace()
 
 
 # ------------------------------------------------------------------ autograd nodes --
@@ -267,6 +268,7 @@ class _TokenLogProbsFn(torch.autograd.Function):
         return tuple(r)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_log_probs, d_entropy, *_):
         logits, targets, stats, entropy = ctx.saved_tensors
         if d_log_probs is None and d_entropy is None:

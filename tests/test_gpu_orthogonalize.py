@@ -88,6 +88,43 @@ def test_many_tiles(shapes, mode):
     assert all(torch.equal(a, b) for a, b in zip(ys, ops.orthogonalize(gs, math=mode)))
 
 
+def test_many_tiles_in_graphs_on_streams_and_few_sms():
+    """Two graphs with workspaces of their own, replayed side by side; any number of SMs; a NaN stays in its matrix."""
+    gs = [gradient(r, c, seed=r) for r, c in ((1600, 1800), (1700, 1601))]
+    want = [ops.orthogonalize(g) for g in gs]
+    streams, spaces = [torch.cuda.Stream() for _ in gs], [ops.Workspace() for _ in gs]
+    ins, outs, graphs = [torch.zeros_like(g) for g in gs], [torch.zeros_like(g) for g in gs], []
+    for x, y, ws, stream in zip(ins, outs, spaces, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            ops.orthogonalize(x, out=y, ws=ws)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            ops.orthogonalize(x, out=y, ws=ws)
+    for x, g in zip(ins, gs):
+        x.copy_(g)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    ops.device_status()
+    assert all(torch.equal(y, w) for y, w in zip(outs, want))
+    try:
+        for sms in (1, 2, 3, 37):
+            ops.set_sm_limit(sms)
+            assert off(ops.orthogonalize(gs[0]), plain(gs[0])) <= TOL["3xf16"], sms
+    finally:
+        ops.set_sm_limit(0)
+    group = [gradient(512, 2048, seed=k) for k in range(9)]
+    group[4][3, 5] = math.nan
+    ys = ops.orthogonalize(group)
+    assert bool(ys[4].isnan().all())
+    assert all(off(ys[k], plain(group[k])) <= TOL["3xf16"] for k in range(9) if k != 4)
+
+
 @MODES
 def test_singular_values_and_vectors(mode):
     """What the operator is for: singular values near 1, the same singular vectors."""

@@ -113,6 +113,26 @@ def test_large_offsets(offset):
 
 
 @DTYPES
+@pytest.mark.parametrize("step", [0.01, 0.5, 7.9, 8.1, 60.0])
+def test_rising_logits(step, dtype):
+    """Every unit has a new maximum: the sums move seldom, always or by nearly as much as leaves them where they are."""
+    v = torch.arange(2000, device=DEV, dtype=torch.float64) * step
+    x = (v - v[-1] / 2).clamp(-60000, 60000).to(dtype)
+    check_forward(torch.stack([x, x.flip(0), x.roll(1000)]), torch.tensor([1999, 1, 1000], device=DEV), 4)
+
+
+@DTYPES
+def test_ties(dtype):
+    """Few values, many of each: alternatives by index, however many units share their maximum."""
+    g = torch.Generator(device=DEV).manual_seed(8)
+    for vocab in (1000, 2000, 5000, 40000):
+        for values, top in ((1, 32), (3, 32), (40, 7), (40, 1)):
+            x = torch.randint(0, values, (70, vocab), device=DEV, generator=g).to(dtype)
+            got = ops.token_log_probs(x, tokens((70,), vocab), top=top).top_indices
+            assert torch.equal(got, x.float().sort(dim=-1, descending=True, stable=True).indices[:, :top]), (vocab, values)
+
+
+@DTYPES
 def test_more_rows_than_blocks(dtype):
     check_forward(logits((10000, 257), dtype, 1), tokens((10000,), 257), 3)
     check_forward(logits((5000, 5001), dtype, 2), tokens((5000,), 5001), 2)
@@ -353,6 +373,10 @@ def test_autograd(dtype):
         want = ops.token_log_probs_backward(x.detach(), t, plainly.stats, plainly.entropy, ones * (part == "log_probs"),
                                             ones if part == "entropy" else None)
         assert torch.equal(x.grad, want)
+    weight = ones.clone().requires_grad_(True)
+    g, = torch.autograd.grad((weight * train.token_log_probs(x, t).log_probs).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):   # (and not a second gradient that lacks a part)
+        g.square().sum().backward()
 
 
 def test_training_step_with_this_loss():

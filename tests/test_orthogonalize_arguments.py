@@ -92,6 +92,33 @@ def test_muon_refuses_a_parameter_listed_twice(lib):
     assert _muon(lib, [(0x10000, 0x20000, 0x10000, None, 0, 8, 1.0)]) == INVALID  # momentum is the parameter
 
 
+def test_muon_refuses_gradients_among_what_it_writes(lib):
+    good = (0x10000, 0x20000, 0x30000, 0x40000, 8, 8, 1.0)
+    beside = (0x10100, 0x20000, 0x31000, 0x41000, 8, 8, 1.0)
+    assert _muon(lib, [good, beside]) == WORKSPACE                 # one gradient for two parameters
+    for at in (0x10000, 0x100fc, 0x0ff04, 0x30000, 0x4007c, 0x310fc):
+        assert _muon(lib, [good, beside[:1] + (at,) + beside[2:]]) == INVALID, hex(at)
+    for at in (0x0ff00, 0x10200, 0x40080):                         # ends where one begins, begins where one ends
+        assert _muon(lib, [good, beside[:1] + (at,) + beside[2:]]) == WORKSPACE, hex(at)
+
+
+def test_results_in_places_of_their_own(lib):
+    def call(*m):
+        c = (C.c_double * 15)(*(COEF * 5))
+        return lib.nml_orthogonalize((_lib.Matrix * len(m))(*m), len(m), 0, 0, _lib.NML_MATH_3XF16, 5, c, 1e-7, None, 0, None)
+    a = _lib.Matrix(P, P, 4, 4, 4, 1, 4, 1)
+    assert call(a) == WORKSPACE
+    assert call(a, _lib.Matrix(P, 2 * P, 4, 4, 4, 1, 4, 1)) == WORKSPACE       # one matrix twice, two results
+    assert call(a, _lib.Matrix(2 * P, P, 4, 4, 4, 1, 4, 1)) == INVALID
+    assert call(_lib.Matrix(P, P, 4, 4, 4, 1, 1, 4)) == INVALID                # in place, turned
+    assert _call(lib, out_dtype=1) == INVALID                                  # in place, of another type
+
+
+def test_every_store_has_a_workspace_of_its_own():
+    """A captured step's stays where it is when another net's step needs a larger one."""
+    assert train.ParamStore("cpu")._muon_ws is not train.ParamStore("cpu")._muon_ws
+
+
 def test_tensor_level_refusals():
     e = _lib.NectarB200Error
     x = torch.zeros(4, 6)

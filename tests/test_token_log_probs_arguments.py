@@ -51,6 +51,6 @@ def _backward(lib, logits=P, dtype=0, rows=4, vocab=100, pitch=100, targets=P, s
 
 @pytest.mark.parametrize("bad", [
     dict(logits=None), dict(targets=None), dict(stats=None), dict(dlp=None), dict(out=None), dict(h=None), dict(dtype=3), dict(rows=0),
-    dict(vocab=0), dict(pitch=99), dict(d_pitch=99), dict(out=P + 2), dict(targets=P + 4), dict(dlp=P + 2), dict(dh=P + 3)], ids=str)
+    dict(vocab=0), dict(pitch=99), dict(d_pitch=99), dict(out=P + 2), dict(targets=P + 4), dict(dlp=P + 2), dict(dh=P + 3), dict(d_pitch=101)], ids=str)
 def test_backward_arguments(lib, bad):
     assert _backward(lib, **bad) == INVALID
