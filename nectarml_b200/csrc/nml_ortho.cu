@@ -439,11 +439,13 @@ struct ProductParams {
     float keep, rate;
 };
 
+// A parameter's element with its update.
+__device__ __forceinline__ float applied(const ProductParams& P, float param, float v, float rate) { return param * P.keep - rate * v; }
 // Results at elements e ... of the output, of which `have` exist.
 __device__ __forceinline__ void put1(const ProductParams& P, uint8_t* out, uint8_t* half, long long e, float v, float rate) {
     if (P.apply) {
         float* const p = reinterpret_cast<float*>(out) + e;
-        const float next = load_global(p) * P.keep - rate * v;
+        const float next = applied(P, load_global(p), v, rate);
         *p = next;
         if (half) reinterpret_cast<__half*>(half)[e] = __float2half_rn(next);
     } else if (P.out_half) {
@@ -465,7 +467,7 @@ __device__ __forceinline__ void put4(const ProductParams& P, uint8_t* out, uint8
     }
     if (P.apply) {
         const float4 w = load_global(reinterpret_cast<const float4*>(out + e * 4));
-        v = make_float4(w.x * P.keep - rate * v.x, w.y * P.keep - rate * v.y, w.z * P.keep - rate * v.z, w.w * P.keep - rate * v.w);
+        v = make_float4(applied(P, w.x, v.x, rate), applied(P, w.y, v.y, rate), applied(P, w.z, v.z, rate), applied(P, w.w, v.w, rate));
     }
     __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
     const uint2 h = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
@@ -508,6 +510,30 @@ __device__ __forceinline__ void write_columns(const ProductParams& P, const uint
     if (out_j == 1) {
         const int j = j0 + (lane & 7) * 4, have = n - j;
         if (have <= 0) return;
+        if (P.apply && have >= 4 && (reinterpret_cast<uintptr_t>(out) | out_i * 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(half) | out_i * 2) % 8 == 0) {
+            // (four loads in flight, from L2: two at a time, and from memory, the parameters' latency was 140 of 1560 us of a step over 34 million of them)
+            long long e = (i0 + lane / 8) * out_i + j;
+#pragma unroll 1
+            for (int q0 = 0; q0 < 8; q0 += 4) {
+                float4 w[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (i0 + (q0 + q) * 4 + lane / 8 < m) w[q] = load_global(reinterpret_cast<const float4*>(out + (e + q * 4 * out_i) * 4));
+#pragma unroll
+                for (int q = 0; q < 4; ++q, e += 4 * out_i) {
+                    const int r = (q0 + q) * 4 + lane / 8;
+                    if (i0 + r >= m) return;
+                    const float4 v = *reinterpret_cast<const float4*>(staging + swizzled(r, lane & 7));
+                    const float4 next = make_float4(applied(P, w[q].x, v.x, rate), applied(P, w[q].y, v.y, rate), applied(P, w[q].z, v.z, rate), applied(P, w[q].w, v.w, rate));
+                    *reinterpret_cast<float4*>(out + e * 4) = next;
+                    if (half) {
+                        const __half2 a = __floats2half2_rn(next.x, next.y), b = __floats2half2_rn(next.z, next.w);
+                        *reinterpret_cast<uint2*>(half + e * 2) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+                    }
+                }
+            }
+            return;
+        }
 #pragma unroll 2
         for (int q = 0; q < 8; ++q) {
             const int r = q * 4 + lane / 8;
@@ -515,9 +541,36 @@ __device__ __forceinline__ void write_columns(const ProductParams& P, const uint
         }
     } else if (i0 + lane < m) {
         long long e = (i0 + lane) * out_i + j0 * out_j;
+        if (P.apply && n - j0 >= 32) {
+#pragma unroll 1
+            for (int q0 = 0; q0 < 32; q0 += 4) {
+                float w[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) w[q] = load_global(reinterpret_cast<const float*>(out) + e + q * out_j);
+#pragma unroll
+                for (int q = 0; q < 4; ++q, e += out_j) {
+                    const float next = applied(P, w[q], *reinterpret_cast<const float*>(staging + swizzled(lane, (q0 + q) >> 2) + (q & 3) * 4), rate);
+                    reinterpret_cast<float*>(out)[e] = next;
+                    if (half) reinterpret_cast<__half*>(half)[e] = __float2half_rn(next);
+                }
+            }
+            return;
+        }
 #pragma unroll 2
         for (int q = 0; q < min(32, n - j0); ++q, e += out_j)
             put1(P, out, half, e, *reinterpret_cast<const float*>(staging + swizzled(lane, q >> 2) + (q & 3) * 4), rate);
+    }
+}
+// Brings the parameters of a warp's 32 rows and `columns` columns into L2, while the tile's products run.
+__device__ __forceinline__ void prefetch_columns(const uint8_t* out, long long out_i, long long out_j, int i0, int m, int j0, int n, int columns) {
+    const int lane = threadIdx.x & 31;
+    auto fetch = [&](long long e) { asm volatile("prefetch.global.L2 [%0];" ::"l"(__cvta_generic_to_global(out + e * 4))); };
+    const int end = min(n, j0 + columns);
+    if (out_j == 1) {
+        if (i0 + lane < m)
+            for (int j = j0; j < end; j += 32) fetch((i0 + lane) * out_i + j);
+    } else {
+        for (int j = j0 + lane; j < end; j += 32) fetch(i0 * out_i + j * out_j);
     }
 }
 
@@ -1016,6 +1069,11 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
             const int mine = groups * 2, g0 = side * mine + 4 * in_block;  // this thread's columns in sixteens; the first one in its block
             const int chunks = kPlanes == 2 ? slices : min(1, slices);
             const bool is_wide = kind == ITERATE || kind == RESULT;
+            if (kind == RESULT && P.apply) {
+                const Source* src = &P.c.table[k].s;
+                prefetch_columns(reinterpret_cast<const uint8_t*>(load_wide(reinterpret_cast<const long long*>(&src->out))), load_wide(&src->out_i), load_wide(&src->out_j),
+                                 tile_i * kBlock + quarter * 32, w.m, tile_j * kBlock + g0 * 16, w.n, mine * 16);
+            }
             float acc[8][16];
 #pragma unroll
             for (int c = 0; c < 8; ++c)
