@@ -542,91 +542,89 @@ __global__ void __launch_bounds__(kThreads == 32 ? 32 * kWarpRows : kThreads, kT
     uint32_t* const maxima = all_maxima + (kRows > 1 ? threadIdx.y * P.share : 0);
     const int rank = P.cluster > 1 ? static_cast<int>(blockIdx.x % P.cluster) : 0;
     const int tid = threadIdx.x;
-    const long long r0 = kRows > 1 ? static_cast<long long>(blockIdx.x) * kRows + threadIdx.y : blockIdx.x / P.cluster;
-    const long long step = kRows > 1 ? static_cast<long long>(gridDim.x) * kRows : gridDim.x / P.cluster;
-    for (long long r = r0; r < P.rows; r += step) {
-        const Row<T> row(static_cast<const T*>(P.logits) + r * P.pitch, P.vocab);
-        const int share = (row.units + P.cluster - 1) / P.cluster;
-        const int u0 = min(row.units, rank * share), u1 = min(row.units, u0 + share);
-        Running<T> run;
-        auto take = [&](int u, const uint32_t (&v)[8]) {
-            const float most = run.add(v);
-            if (P.top) maxima[u - u0] = order_key(most);
-        };
-        const int f0 = max(u0, row.full0), f1 = min(u1, row.full1);
-        int u = f0 + tid;
-        long long target = tid == 0 ? load_index(P.targets + r) : -1;
-        for (; u + (kFlight - 1) * kThreads < f1; u += kFlight * kThreads) {
-            uint32_t v[kFlight][8];
+    const long long r = kRows > 1 ? static_cast<long long>(blockIdx.x) * kRows + threadIdx.y : blockIdx.x / P.cluster;
+    if (kRows > 1 && r >= P.rows) return;
+    const Row<T> row(static_cast<const T*>(P.logits) + r * P.pitch, P.vocab);
+    const int share = (row.units + P.cluster - 1) / P.cluster;
+    const int u0 = min(row.units, rank * share), u1 = min(row.units, u0 + share);
+    Running<T> run;
+    auto take = [&](int u, const uint32_t (&v)[8]) {
+        const float most = run.add(v);
+        if (P.top) maxima[u - u0] = order_key(most);
+    };
+    const int f0 = max(u0, row.full0), f1 = min(u1, row.full1);
+    int u = f0 + tid;
+    long long target = tid == 0 ? load_index(P.targets + r) : -1;
+    for (; u + (kFlight - 1) * kThreads < f1; u += kFlight * kThreads) {
+        uint32_t v[kFlight][8];
 #pragma unroll
-            for (int e = 0; e < kFlight; ++e) load_unit(row.at(u + e * kThreads), v[e]);
+        for (int e = 0; e < kFlight; ++e) load_unit(row.at(u + e * kThreads), v[e]);
 #pragma unroll
-            for (int e = 0; e < kFlight; ++e) take(u + e * kThreads, v[e]);
-        }
-        if (u < f1) {
-            uint32_t v[kFlight - 1][8];
-#pragma unroll
-            for (int e = 0; e < kFlight - 1; ++e)
-                if (u + e * kThreads < f1) load_unit(row.at(u + e * kThreads), v[e]);
-#pragma unroll
-            for (int e = 0; e < kFlight - 1; ++e)
-                if (u + e * kThreads < f1) take(u + e * kThreads, v[e]);
-        }
-        // (asked for before the sums are exchanged, needed behind them)
-        const float of_target = target >= 0 && target < P.vocab ? Elements<T>::load(static_cast<const T*>(P.logits) + r * P.pitch + target) : 0.f;
-        // the first and the last unit, where they have gaps
-        if (tid < 2) {
-            const int e = tid == 0 ? 0 : row.units - 1;
-            const bool broken = tid == 0 ? row.full0 == 1 : row.full1 < row.units && !(row.full0 == 1 && row.units == 1);
-            if (broken && e >= u0 && e < u1) {
-                uint32_t a[8];
-                row.load_broken(e, a);
-                take(e, a);
-            }
-        }
-        Stats a = run.done();
-        if (kThreads > 32) {
-            if ((tid & 31) == 0) sh.warp[tid / 32] = a;
-            __syncthreads();
-            if (tid < 32) a = merge_lanes<T>(sh.warp[tid % (kThreads / 32)], kThreads / 32);
-        }
-        if (P.top) {
-            block_sync<kThreads>();
-            search<T, kThreads>(row, u0, u1 - u0, P.top, maxima, sh);
-        }
-        if (P.cluster > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            if (tid == 0) sh.block = a;
-            cluster.sync();
-            if (rank == 0) {
-                if (tid < 32) a = merge_lanes<T>(*cluster.map_shared_rank(&sh.block, tid % P.cluster), P.cluster);
-                if (P.top) {
-                    const int count = P.cluster * P.top;
-                    for (int e = tid; e < count; e += kThreads) sh.candidate[e] = cluster.map_shared_rank(sh.best, e / P.top)[e % P.top];
-                    __syncthreads();
-                    place<kThreads>(sh.candidate, count, P.top, sh.best);
-                    __syncthreads();
-                }
-            }
-        }
-        if (rank == 0 && tid < 32) {
-            const bool dead = a.m == -INFINITY, bad = !(a.m < INFINITY);  // nothing but -inf; a NaN or +inf
-            const float off = extreme<T>(a.m) ? 0.f : fmaf(a.m, kLog2e, -reference<T>(a.m));  // of the reference, from m log2 e
-            const float log_sum = dead ? 0.f : bad ? NAN : logf(a.s) - off * kLn2;
-            if (tid < P.top) {
-                const uint64_t c = sh.best[tid];
-                P.top_indices[r * P.top + tid] = index_of(c);
-                P.top_log_probs[r * P.top + tid] = dead ? -INFINITY : (value_of(c) - a.m) - log_sum;
-            }
-            if (tid == 0) {
-                P.log_probs[r] = target < 0 ? 0.f : target >= P.vocab ? NAN : dead ? -INFINITY : (of_target - a.m) - log_sum;
-                P.entropy[r] = dead ? 0.f : bad ? NAN : logf(a.s) - kLn2 * (a.t / a.s);
-                P.stats[2 * r] = a.m;
-                P.stats[2 * r + 1] = log_sum;
-            }
-        }
-        if (P.cluster > 1) cg::this_cluster().sync(); else block_sync<kThreads>();
+        for (int e = 0; e < kFlight; ++e) take(u + e * kThreads, v[e]);
     }
+    if (u < f1) {
+        uint32_t v[kFlight - 1][8];
+#pragma unroll
+        for (int e = 0; e < kFlight - 1; ++e)
+            if (u + e * kThreads < f1) load_unit(row.at(u + e * kThreads), v[e]);
+#pragma unroll
+        for (int e = 0; e < kFlight - 1; ++e)
+            if (u + e * kThreads < f1) take(u + e * kThreads, v[e]);
+    }
+    // (asked for before the sums are exchanged, needed behind them)
+    const float of_target = target >= 0 && target < P.vocab ? Elements<T>::load(static_cast<const T*>(P.logits) + r * P.pitch + target) : 0.f;
+    // the first and the last unit, where they have gaps
+    if (tid < 2) {
+        const int e = tid == 0 ? 0 : row.units - 1;
+        const bool broken = tid == 0 ? row.full0 == 1 : row.full1 < row.units && !(row.full0 == 1 && row.units == 1);
+        if (broken && e >= u0 && e < u1) {
+            uint32_t a[8];
+            row.load_broken(e, a);
+            take(e, a);
+        }
+    }
+    Stats a = run.done();
+    if (kThreads > 32) {
+        if ((tid & 31) == 0) sh.warp[tid / 32] = a;
+        __syncthreads();
+        if (tid < 32) a = merge_lanes<T>(sh.warp[tid % (kThreads / 32)], kThreads / 32);
+    }
+    if (P.top) {
+        block_sync<kThreads>();
+        search<T, kThreads>(row, u0, u1 - u0, P.top, maxima, sh);
+    }
+    if (P.cluster > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        if (tid == 0) sh.block = a;
+        cluster.sync();
+        if (rank == 0) {
+            if (tid < 32) a = merge_lanes<T>(*cluster.map_shared_rank(&sh.block, tid % P.cluster), P.cluster);
+            if (P.top) {
+                const int count = P.cluster * P.top;
+                for (int e = tid; e < count; e += kThreads) sh.candidate[e] = cluster.map_shared_rank(sh.best, e / P.top)[e % P.top];
+                __syncthreads();
+                place<kThreads>(sh.candidate, count, P.top, sh.best);
+                __syncthreads();
+            }
+        }
+    }
+    if (rank == 0 && tid < 32) {
+        const bool dead = a.m == -INFINITY, bad = !(a.m < INFINITY);  // nothing but -inf; a NaN or +inf
+        const float off = extreme<T>(a.m) ? 0.f : fmaf(a.m, kLog2e, -reference<T>(a.m));  // of the reference, from m log2 e
+        const float log_sum = dead ? 0.f : bad ? NAN : logf(a.s) - off * kLn2;
+        if (tid < P.top) {
+            const uint64_t c = sh.best[tid];
+            P.top_indices[r * P.top + tid] = index_of(c);
+            P.top_log_probs[r * P.top + tid] = dead ? -INFINITY : (value_of(c) - a.m) - log_sum;
+        }
+        if (tid == 0) {
+            P.log_probs[r] = target < 0 ? 0.f : target >= P.vocab ? NAN : dead ? -INFINITY : (of_target - a.m) - log_sum;
+            P.entropy[r] = dead ? 0.f : bad ? NAN : logf(a.s) - kLn2 * (a.t / a.s);
+            P.stats[2 * r] = a.m;
+            P.stats[2 * r + 1] = log_sum;
+        }
+    }
+    if (P.cluster > 1) cg::this_cluster().sync();  // (the first block has read the others' shared memory)
 }
 
 struct BackwardParams {
@@ -777,8 +775,10 @@ int nml_token_log_probs(const void* logits, int dtype, long long rows, int vocab
     if (const int rc = nml::current_device(&status, &sms)) return rc;
     const ForwardParams P = {logits, targets, rows, pitch, vocab, top, plan.cluster, plan.share, log_probs, entropy, stats, top_log_probs, top_indices};
     const bool warps = plan.threads == 32;
-    const long long blocks = warps ? (rows + kWarpRows - 1) / kWarpRows : rows * plan.cluster, most = static_cast<long long>(sms) * 32 / plan.cluster * plan.cluster;
-    const int grid = static_cast<int>(blocks < most ? blocks : most);
+    const long long blocks = warps ? (rows + kWarpRows - 1) / kWarpRows : rows * plan.cluster;
+    if (blocks > 0x7fffffff) return NML_ERR_UNSUPPORTED;
+    // (a row to a block however many there are: 16384 x 32768 fp16 188 us, 193 with 4736 blocks that take rows in turn, 199 with as many as fit the SMs)
+    const int grid = static_cast<int>(blocks);
     nml::launch_with(nml::overlaps(grid, nml::kSms), plan.cluster, forward_kernel(dtype, plan), grid, warps ? dim3(32, kWarpRows) : dim3(plan.threads),
                      plan.smem,
                      static_cast<cudaStream_t>(stream), P);
