@@ -341,10 +341,9 @@ int current_device(int** status_word, int* sms) {
 }
 int usable_sms() { return planning_sms(); }
 void count_launches(int n) { g_launches += n; }
-int encode_rows(CUtensorMap* map, const void* base, int width, size_t rows, int box) {
-    const uint64_t dims[2] = {static_cast<uint64_t>(width), rows};
-    const uint32_t boxes[2] = {static_cast<uint32_t>(width), static_cast<uint32_t>(box)}, one[2] = {1, 1};
-    return encode_map(map, base, 2, 2, dims, boxes, one, SWZ_NONE);
+int encode_box(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint32_t* box) {
+    const uint32_t one[5] = {1, 1, 1, 1, 1};
+    return encode_map(map, base, 2, rank, dims, box, one, SWZ_NONE);
 }
 int cuda_failed(int error, const char* what) {
     set_last_cuda_error(static_cast<cudaError_t>(error), what);

@@ -2,7 +2,7 @@
 // nml_api.cu), and each file's kernels for the one-time set-up of a device.
 #pragma once
 #include <cuda.h>
-#include <stddef.h>
+#include <stdint.h>
 
 #define NML_HIDDEN __attribute__((visibility("hidden")))
 
@@ -16,8 +16,8 @@ NML_HIDDEN void count_launches(int n);
 // Keeps the text of a CUDA error for nml_status_string; returns NML_ERR_CUDA.
 NML_HIDDEN int cuda_failed(int error, const char* what);
 
-// Tensor map of `rows` dense rows of `width` fp16 elements (at most 256), a box of `box` rows.  Returns a status.
-NML_HIDDEN int encode_rows(CUtensorMap* map, const void* base, int width, size_t rows, int box);
+// Tensor map of a dense tensor of fp16 elements, fastest dimension first, unswizzled.  Returns a status.
+NML_HIDDEN int encode_box(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint32_t* box);
 
 // Loads a file's kernels and raises their shared-memory limits on the current device (called once per device).
 NML_HIDDEN int prepare_logits_kernels();

@@ -426,9 +426,11 @@ __device__ __forceinline__ long long load_wide(const long long* p) {
     asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(__cvta_generic_to_global(p)));
     return v;
 }
-constexpr int kMapRow = 512;   // bytes of a row of the map
+// Pairs: the blocks as [plane][half][rows 0 to 63, 64 to 127][16][256 elements], so that one copy brings an operand's slice in both planes: both pieces of a
+// half, the same piece of both halves, or one piece.
+enum { MAP_HALF = 0, MAP_ACROSS = 1, MAP_PIECE = 2, kMaps = 3 };
 struct ProductParams {
-    CUtensorMap map;           // pairs: the blocks, a copy to a box
+    CUtensorMap map[kMaps];
     Common c;
     int* err;
     unsigned long long limit_ns;  // of a wait
@@ -874,17 +876,17 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                         now_stage = stage_bytes;
                         stages = min(kMaxStages, static_cast<int>(kRing / stage_bytes));
                     }
-                    const bool same = !kPair && whole && tile.i == tile.j;
-                    const int b_pieces = kPair ? (is_wide ? 2 : 1) : same ? 0 : tile.groups, pieces = kPlanes * (2 + b_pieces);
-                    const bool is_a = lane < 2 * kPlanes;
+                    const bool same = whole && tile.i == tile.j;
+                    const int b_pieces = same ? 0 : tile.groups, pieces = kPlanes * (2 + b_pieces);
+                    const bool is_a = lane < (kPair ? 1 : 2 * kPlanes);
                     const int at = is_a ? lane : lane - 2 * kPlanes, per = is_a ? 2 : max(1, b_pieces);
                     const int plane = at / per, piece = at % per;
-                    const uint32_t dst = (is_a ? plane * kHalf : kPlanes * kHalf + plane * b_bytes) + piece * kPiece;
+                    const uint32_t dst = kPair ? (is_a ? 0 : kPlanes * kHalf) : (is_a ? plane * kHalf : kPlanes * kHalf + plane * b_bytes) + piece * kPiece;
                     const uint32_t buffer = symmetric_first(w, is_wide ? op.left : is_a ? op.job[tile.job].left : op.job[tile.job].right);
                     const uint32_t x = op.from ? w.x[1] : w.x[0];
                     // block row of the left operand; a pair that is one row short has its last one twice.  K-major up to `turn`, for both rows alike
                     const int left_row = min(kBoth * tile.i + static_cast<int>(rank), mb - 1), turn = is_a ? kBoth * tile.i : tile.j;
-                    const int last_group = (w.n + 63) / 64 - 1 - 2 * tile.j;
+                    const int right_block = min(tile.j + static_cast<int>(rank), w.nb - 1);
                     for (int q = 0; q < tile.slices + tile.extra; ++q) {
                         if (used >> s & 1) {
                             if (!wait(&empty_bar[s], (parity >> s & 1) ^ 1, nml::ERR_WAIT_EMPTY)) {
@@ -893,12 +895,31 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                             }
                         }
                         const uint32_t bar = nml::smem_u32(&full_bar[s]), to = nml::smem_u32(smem) + s * stage_bytes + dst;
-                        if (lane == 0 && leader) nml::mbar_arrive_expect_tx(bar, kBoth * pieces * kPiece);
+                        if (lane == 0 && leader) nml::mbar_arrive_expect_tx(bar, kPair ? 2 * stage_bytes : pieces * kPiece);
                         __syncwarp();
-                        if (lane < pieces) {
+                        if (kPair && lane < 2) {  // a lane to an operand
+                            const int kq = tile.from + q, kb = kq >> 1, h = kq & 1;
+                            const bool own = lane == 0, both = own || is_wide;  // the left operand; both pieces of the right one
+                            const int row = own ? left_row : tile.j;
+                            bool straight = true;
+                            int block;
+                            if (whole) {
+                                block = static_cast<int>(x) + row * w.nb + kb;
+                            } else if (!own && is_wide) {
+                                block = static_cast<int>(x) + kb * w.nb + right_block;
+                                straight = false;
+                            } else {
+                                straight = kb <= turn;
+                                block = static_cast<int>(buffer) + (straight ? lower(row, kb) : lower(kb, row));
+                            }
+                            const int mine = both ? 0 : static_cast<int>(rank);
+                            nml::tma_load_5d_pair(to, &P.map[both ? (straight ? MAP_HALF : MAP_ACROSS) : MAP_PIECE], nml::map_to_cta(bar, 0), 0, 0, straight ? mine : h,
+                                                  straight ? h : mine, 2 * block);
+                        }
+                        if (!kPair && lane < pieces) {
                             const bool low = q >= tile.slices;  // a I times X's low half
                             const int kq = low ? 2 * tile.i + q - tile.slices : tile.from + q, kb = kq >> 1, h = kq & 1;
-                            const int group = is_a ? piece : !kPair ? piece + tile.column : is_wide ? min(2 * static_cast<int>(rank) + piece, last_group) : static_cast<int>(rank);
+                            const int group = is_a ? piece : piece + tile.column;
                             const uint8_t* from;
                             const uint32_t straight = (h * 2 + group) * kPiece, across = (group * 2 + h) * kPiece;  // K-major; MN-major
                             auto symmetric = [&](int row) {
@@ -913,8 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                                 from = block_at(P.c.blocks, x, kb * w.nb + tile.j + (group >> 1)) + (low ? kPlane : 0) + ((group & 1) * 2 + h) * kPiece;
                             }
                             from += plane * kPlane;
-                            if (kPair) nml::tma_load_2d_pair(to, &P.map, nml::map_to_cta(bar, 0), 0, static_cast<int>((from - P.c.blocks) / kMapRow));
-                            else nml::bulk_load(to, from, kPiece, bar);
+                            nml::bulk_load(to, from, kPiece, bar);
                         }
                         __syncwarp();
                         used |= 1u << s;
@@ -1633,7 +1653,11 @@ static int run_group(Work* w, int count, const Call& call, const Steps& steps, v
     ProductParams q = {{}, c, err, static_cast<unsigned long long>(1.5e9 + 2e3 * slices), pack.rounds, static_cast<int>(tiles), p.first_class,
                              call.out_dtype == NML_F16, call.apply, call.keep, call.rate};
     if (p.pair)
-        if (const int rc = nml::encode_rows(&q.map, c.blocks, kMapRow / 2, static_cast<size_t>(p.blocks) * (2 * kPlane / kMapRow), kPiece / kMapRow)) return rc;
+        for (int e = 0; e < kMaps; ++e) {
+            const uint64_t dims[5] = {256, 16, 2, 2, 2ull * p.blocks};
+            const uint32_t box[5] = {256, 16, e == MAP_HALF ? 2u : 1u, e == MAP_ACROSS ? 2u : 1u, 2};
+            if (const int rc = nml::encode_box(&q.map[e], c.blocks, 5, dims, box)) return rc;
+        }
     // (no more blocks than a round has tiles)
     const int each = p.pair ? 2 : 1, grid = each * static_cast<int>(std::min<long long>(widest, sms / each));
     nml::launch_with(nml::overlaps(grid, nml::kSms), each,
