@@ -482,6 +482,10 @@ __device__ __forceinline__ void put4(const ProductParams& P, uint8_t* out, uint8
 }
 
 
+// Two sums in one instruction.
+__device__ __forceinline__ void add2(float& a, float& b, uint32_t x, uint32_t y) {
+    asm("{\n\t.reg .b64 s, t;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\tadd.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}" : "+f"(a), "+f"(b) : "r"(x), "r"(y));
+}
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 // Registers: a thread of the epilogue holds 128 accumulators beside the eight columns it is splitting.  The block is launched with kLaunchRegs for each thread;
@@ -1116,7 +1120,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                         nml::tmem_ld_32x32(from + c * 16, r);
                         nml::tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) acc[c + e / 16][e % 16] += __uint_as_float(r[e]);
+                        for (int e = 0; e < 32; e += 2) add2(acc[c + e / 16][e % 16], acc[c + e / 16][e % 16 + 1], r[e], r[e + 1]);
                     }
                 }
                 nml::tc_fence_before();
