@@ -530,7 +530,7 @@ struct ForwardParams {
 
 // A row to a block, or to a cluster of blocks that take equal runs of its units and meet in the first one's shared memory.
 // kFlight units of a thread are in flight: four where there are few rows, and latency counts (1 x 131072 fp32 9.4 -> 7.3 us); with two, of many rows more
-// warps fit an SM (16384 x 32768 fp16 212 -> 189 us).
+// warps fit an SM (16384 x 32768 fp16 with eight alternatives 215 us, with four 231).
 template <typename T, int kThreads, int kFlight>
 __global__ void __launch_bounds__(kThreads == 32 ? 32 * kWarpRows : kThreads, kThreads == 32 ? 5 : 0) token_log_probs_kernel(const ForwardParams P) {
     pdl_enter();
@@ -713,7 +713,8 @@ static ForwardPlan forward_plan(long long rows, int vocab, int dtype, int top) {
     const int n = dtype == NML_F16 ? Elements<__half>::N : Elements<float>::N;
     const int units = static_cast<int>((static_cast<long long>(vocab) + 2 * n - 2) / n);  // at the worst start of a row
     ForwardPlan p;
-    // A warp to a short row, four to others, eight to the longest; these over several blocks where there are few rows.
+    // A warp to a short row, four to others, eight to the longest (16384 x 32768 fp16, eight alternatives: four 215 us, eight 244; 2048 x 131072: 143 and
+    // 119); these over several blocks where there are few rows.
     p.threads = units <= 128 ? 32 : units <= 4096 ? 128 : 256;
     if (units > 1024 && rows < 74) p.threads = 256;
     while (p.cluster < kMaxCluster && p.threads == 256 && ((rows * p.cluster < 148 && units > 512 * p.cluster) || (top && (units + p.cluster - 1) / p.cluster > kMaxUnits))) p.cluster *= 2;

@@ -427,7 +427,7 @@ __device__ __forceinline__ long long load_wide(const long long* p) {
     return v;
 }
 // Pairs: the blocks as [plane][half][rows 0 to 63, 64 to 127][16][256 elements], so that one copy brings an operand's slice in both planes: both pieces of a
-// half, the same piece of both halves, or one piece.
+// half, the same piece of both halves, or one piece.  (Eight copies of 8 KB a slice and block, whose issue paced the loop: 8192 x 2048 998 us; so 962.)
 enum { MAP_HALF = 0, MAP_ACROSS = 1, MAP_PIECE = 2, kMaps = 3 };
 struct ProductParams {
     CUtensorMap map[kMaps];
@@ -628,7 +628,7 @@ __host__ __device__ __forceinline__ int symmetric_count(int mb) {
 // in 64: 1250 clocks, where the tensor core needs 768; 128 x 256 1875 for 1536), has a quarter (a third) less to deliver, and a stage is as much smaller.
 // The first block takes the tiles and passes them to the other one; each loads its own operands, whose arrival the first one's barrier counts, and
 // stores its own row.  What the accumulators' readers of the other block tell the first one is a barrier's arrival without a fence: with one, behind
-// which the stores of the last tile had to be visible, the pair was slower than two blocks (2048 x 8192 1331 us; without 970; two blocks 1197).
+// which the stores of the last tile had to be visible, the pair was slower than two blocks (2048 x 8192 1331 us; without 970; two blocks then 1197).
 template <int kPlanes, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid_constant__ ProductParams P) {
     extern __shared__ uint8_t smem_raw[];
@@ -1366,7 +1366,7 @@ static bool polynomial(const double* coefficients, int steps, bool chained, Poly
 
 // Which matrices are chained: where the long side is so much longer that products of m x m matrices are the cheaper ones, and m is so large that
 // the rounding errors, which are random, add to little in any one direction (relative to fp32 products, errors were 2.0 at m = 256, 7 at 64).  1024 x
-// 4096 510 us instead of 652, 256 x 1024 211 / 229, 1024 x 1024 385 / 347, 128 x 512 170 / 176.
+// 4096 412 us instead of 463, eight of them 1051 / 1612, 256 x 1024 190 / 201; 512 x 768 231 / 221, 1024 x 1024 would be 340 / 307, 512 x 512 223 / 203.
 static bool chained(const Source& s, int math) { return math == NML_MATH_3XF16 && s.m >= 256 && 2ll * s.n >= 3ll * s.m; }
 
 struct Plan {
@@ -1393,13 +1393,13 @@ static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
         for (int e = 0; e < 3; ++e) wide_tiles[e] += static_cast<long long>(w[k].mb) * (((w[k].s.n + 63) / 64 + (1 << e) - 1) >> e);
     }
     // Where a round has few tiles: two to a block, narrow ones of Q X, and X X^T with its long K in parts, at least eight slices each
-    // (together: 1024 x 4096 384 us instead of 484, 128 x 2048 175 / 205, 512 x 512 185 / 217).
+    // (together: 1024 x 4096 412 us instead of 491, 1024 x 1024 309 / 385, 512 x 512 203 / 264, 128 x 2048 188 / 303).
     const int fine = 2 * blocks <= sms ? 2 : 1, spare = static_cast<int>(std::max<long long>(1, sms / (blocks * fine)));
     const int wide = wide_tiles[0] <= sms ? 1 : wide_tiles[1] <= sms ? 2 : 4;
     // Pairs of blocks (see the kernel), where every round has tiles for all SMs and little of a pair's work is lost above the diagonal or for an
-    // odd row: 4096 x 4096 3.5 ms instead of 4.5, 2048 x 8192 970 us / 1197, 8 of 512 x 2048 345 / 386, 30 of 256 x 1024 261 / 278; against it 30 of
-    // 640 x 640, five rows each, 843 / 685 (pairs do 1.38 times the work), four of 512 x 2048 among 60 of 128 x 1152 425 / 378.  "f16" would
-    // gain nothing (4096 x 4096 2.5 ms / 2.35): its slices are so short that the copies' issue paces them.
+    // odd row: 4096 x 4096 3.4 ms instead of 4.3, 2048 x 8192 931 us / 1175, eight of 1024 x 4096 1109 / 1256, of 512 x 2048 345 / 390, 30 of 256 x 1024
+    // 262 / 284; against it 30 of 640 x 640, five rows each, 814 / 685 (pairs do 1.38 times the work), four of 512 x 2048 among 60 of 128 x 1152
+    // 423 / 382.  "f16" gained nothing (4096 x 4096 2.5 ms / 2.35).
     p.pair = math == NML_MATH_3XF16 && fine == 1 && spare == 1 && wide == 4 && sms >= 2 && paired <= 1.2 * single;
     std::sort(w, w + count, [](const Work& a, const Work& b) {
         if (a.chained != b.chained) return a.chained > b.chained;
