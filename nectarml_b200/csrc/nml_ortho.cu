@@ -572,6 +572,7 @@ __device__ __forceinline__ void prefetch_columns(const uint8_t* out, long long o
     const int lane = threadIdx.x & 31;
     auto fetch = [&](long long e) { asm volatile("prefetch.global.L2 [%0];" ::"l"(__cvta_generic_to_global(out + e * 4))); };
     const int end = min(n, j0 + columns);
+    if (i0 >= m) return;
     if (out_j == 1) {
         if (i0 + lane < m)
             for (int j = j0; j < end; j += 32) fetch((i0 + lane) * out_i + j);

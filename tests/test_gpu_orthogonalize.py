@@ -314,6 +314,20 @@ def test_muon_step(nesterov, scaling, mode):
             assert torch.equal(h, p.half())
 
 
+@pytest.mark.parametrize("shapes", [[(1601, 1700), (33,)], [(2000, 1537)], [(1700, 1600), (1600, 1700)], [(384, 1024)] * 8 + [(1030, 390)] * 9], ids=str)
+def test_muon_step_of_many_tiles(shapes):
+    """Pairs of blocks: parameters whose rows are aligned and not, along and across memory, an odd number of block rows."""
+    params, grads, momenta = model(shapes)
+    halves = [p.half() for p in params]
+    want = [plain_step(p, g, v, 0.03, 0.9, True, 0.1, 1.0, "spectral") for p, g, v in zip(params, grads, momenta)]
+    ops.muon_step(params, grads, momenta, halves, lr=0.03, momentum=0.9, weight_decay=0.1)
+    ops.device_status()
+    for p, v, h, (wp, wv, wu) in zip(params, momenta, halves, want):
+        assert float((p.double() - wp).norm()) <= TOL["3xf16"] * float(wu.norm()) + 2.0 ** -22 * float(wp.norm()), p.shape
+        assert float((v.double() - wv).norm()) <= 2.0 ** -22 * float(wv.norm())
+        assert torch.equal(h, p.half())
+
+
 def test_muon_step_of_small_parameters():
     """The same where all matrices have a short side up to 64."""
     shapes = [(64, 3, 7, 7), (64,), (13, 70), (500, 64), (1, 9), (9, 1), (64, 64)]
