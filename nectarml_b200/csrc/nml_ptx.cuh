@@ -130,7 +130,7 @@ __device__ __forceinline__ void abort_state_init(volatile int* abort_state, unsi
     *reinterpret_cast<volatile unsigned long long*>(abort_state + 2) = limit_ns ? limit_ns : NML_WAIT_LIMIT_NS;
 }
 
-// The same, and what the other block of a cluster has arrived with is visible.
+// mbar_try_wait by which what the other block of a cluster stored before it arrived is visible too.
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
