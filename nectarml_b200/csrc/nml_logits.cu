@@ -669,14 +669,14 @@ __global__ void __launch_bounds__(256) token_log_probs_backward_kernel(const Bac
         } else {
 #pragma unroll
             for (int j = 0; j < N / 2; ++j)
-                x[j] = pack2(fmaxf((Elements<T>::get(v, 2 * j) - m) * kLog2e, -1e5f), fmaxf((Elements<T>::get(v, 2 * j + 1) - m) * kLog2e, -1e5f));
+                x[j] = pack2(max_nan((Elements<T>::get(v, 2 * j) - m) * kLog2e, -1e5f), max_nan((Elements<T>::get(v, 2 * j + 1) - m) * kLog2e, -1e5f));
         }
 #pragma unroll
         for (int j = 0; j < N / 2; ++j) {
             uint64_t y;
             if (far) y = add2(x[j], pack2(-log_sum * kLog2e, -log_sum * kLog2e));
             else y = add2(fma2(x[j], l2, m2), k2);
-            if (sizeof(T) == 4) y = pack2(fmaxf(low(y), -1e5f), fmaxf(high(y), -1e5f));  // (times a gradient of any size)
+            if (sizeof(T) == 4) y = pack2(max_nan(low(y), -1e5f), max_nan(high(y), -1e5f));  // (times a gradient of any size; a row with NaN keeps it)
             const uint64_t e = pack2(power2(low(y)), power2(high(y)));
             x[j] = mul2(e, entropy ? fma2(y, slope2, level2) : level2);
         }
