@@ -220,10 +220,16 @@ constexpr float kFar = -1e30f;  // instead of a distance of -inf
 struct Stats {
     float m, s, t;
 };
-// How far y moves where the maximum a becomes b >= a.
+// What the reference of m lies below m log2 e.
+template <typename T>
+__device__ __forceinline__ float below(float m) { return extreme<T>(m) ? 0.f : fmaf(m, kLog2e, -reference<T>(m)); }
+// How far y moves where the maximum a becomes b >= a: from one reference to the other.  Where only one of them is rounded, by what that one
+// lacks too, which is up to a half: 2^0.5 in the sums of a row whose maxima lie on both sides of 1e7.
 template <typename T>
 __device__ __forceinline__ float moved_by(float a, float b) {
-    return extreme<T>(a) || extreme<T>(b) ? fmaxf((a - b) * kLog2e, kFar) : reference<T>(a) - reference<T>(b);
+    const bool far_a = extreme<T>(a), far_b = extreme<T>(b);
+    if (!far_a && !far_b) return reference<T>(a) - reference<T>(b);
+    return fmaxf(fmaf(a - b, kLog2e, below<T>(b) - below<T>(a)), kFar);
 }
 // The statistics of the lanes of a warp (or of its first `width`), in every lane: against the largest maximum, once, then two plain sums.  `m` is the
 // lane's maximum where a.m is another reference.
@@ -610,7 +616,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 32 * kWarpRows : kThreads, kT
     }
     if (rank == 0 && tid < 32) {
         const bool dead = a.m == -INFINITY, bad = !(a.m < INFINITY);  // nothing but -inf; a NaN or +inf
-        const float off = extreme<T>(a.m) ? 0.f : fmaf(a.m, kLog2e, -reference<T>(a.m));  // of the reference, from m log2 e
+        const float off = below<T>(a.m);
         const float log_sum = dead ? 0.f : bad ? NAN : logf(a.s) - off * kLn2;
         if (tid < P.top) {
             const uint64_t c = sh.best[tid];

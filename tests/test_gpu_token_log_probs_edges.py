@@ -1,4 +1,5 @@
-"""Token log probabilities and their gradient where a row's numbers leave the ordinary range."""
+"""Token log probabilities and their gradient where a row's numbers leave the ordinary range: NaN and infinities without an entropy
+gradient, logits on both sides of the magnitude from which distances are taken from the maximum itself."""
 import math
 
 import pytest
@@ -6,7 +7,7 @@ import torch
 
 from nectarml_b200 import ops, train
 
-from test_gpu_token_log_probs import DEV, DTYPES, logits
+from test_gpu_token_log_probs import DEV, DTYPES, U, chain, check_backward, check_forward, logits, plain, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,39 @@ def test_gradient_of_rows_with_nan_through_autograd():
     x.requires_grad_(True)
     train.token_log_probs(x, torch.tensor([1, 2, 3], device=DEV)).log_probs.sum().backward()
     assert bool(x.grad[1].isnan().all()) and bool(x.grad[0::2].isfinite().all())
+
+
+@pytest.mark.parametrize("vocab", [5, 777, 3000, 70001])
+@pytest.mark.parametrize("around", [1e7, -1e7])
+def test_logits_on_both_sides_of_far(around, vocab):
+    """Maxima of 1e7 and more (or of -1e7 and less) are references of their own, smaller ones are rounded products: both in one row, as in one
+    that a mask of -1e7 covers as a whole.  The gradient is good to what test_large_offsets derives."""
+    x = around + logits((40, vocab), torch.float32, 23, spread=2.5) - (3.0 if around < 0 else -3.0) * torch.arange(
+        -2, 3, device=DEV).repeat(8)[:, None]
+    assert bool(((x.abs() >= 1e7).any(1) & (x.abs() < 1e7).any(1)).any())
+    t = tokens((40,), vocab)
+    r = check_forward(x, t, min(3, vocab))
+    d, dh = logits((40,), torch.float32, 24), logits((40,), torch.float32, 25)
+    lp, _, h, _ = plain(x, t)
+    p = lp.exp()
+    want = -d[:, None] * p * (t >= 0)[:, None] - dh[:, None] * p * torch.where(p > 0, lp + h[:, None], 0.0)
+    want[torch.arange(40, device=DEV), t.clamp(min=0)] += torch.where(t >= 0, d, 0.0)
+    got = ops.token_log_probs_backward(x, t, r.stats, r.entropy, d, dh).double()
+    size = (d.abs().max() + dh.abs().max() * 16).item()
+    assert bool(((got - want).abs() <= 2 * size * (8 + chain(vocab, torch.float32)) * U).all())
+
+
+@pytest.mark.parametrize("vocab", [777, 70001])
+def test_half_precision_logits_on_both_sides_of_far(vocab):
+    """The same at fp16's lowest values, where maxima below -65000 are references of their own."""
+    g = torch.Generator(device=DEV).manual_seed(26)
+    x = (-65008 + 32 * torch.randint(-2, 3, (40, vocab), device=DEV, generator=g)).half()
+    assert bool((x < -65000).any()) and bool((x >= -65000).any()) and bool(x.isfinite().all())
+    t = tokens((40,), vocab)
+    check_forward(x, t, 3)
+    # every unit on one side: the maxima meet where lanes are merged
+    y = torch.full((4, vocab), -65024.0, device=DEV).half()
+    y[:, : vocab // 2] = -64992.0
+    y[2:] = y[2:].flip(1)
+    check_forward(y, t[:4].contiguous(), 3)
+    check_backward(y, t[:4].contiguous(), False)
