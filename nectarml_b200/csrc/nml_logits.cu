@@ -215,7 +215,7 @@ template <typename T>
 __device__ __forceinline__ bool extreme(float m) { return sizeof(T) == 4 ? !(fabsf(m) < 1e7f) : m < -65000.f; }
 template <typename T>
 __device__ __forceinline__ float reference(float m) { return extreme<T>(m) ? 0.f : __fmul_rn(m, kLog2e); }  // (rounded wherever it stands)
-constexpr float kFar = -1e30f;  // instead of a distance of -inf
+constexpr float kFar = -1e20f;  // instead of a distance of -inf; times the largest sums, 2^31 logits of e^kSlack, a finite number
 
 struct Stats {
     float m, s, t;

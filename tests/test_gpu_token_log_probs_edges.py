@@ -1,5 +1,5 @@
 """Token log probabilities and their gradient where a row's numbers leave the ordinary range: NaN and infinities without an entropy
-gradient, logits on both sides of the magnitude from which distances are taken from the maximum itself."""
+gradient, logits on both sides of the magnitude from which distances are taken from the maximum itself, sums under a far larger maximum."""
 import math
 
 import pytest
@@ -74,3 +74,15 @@ def test_half_precision_logits_on_both_sides_of_far(vocab):
     y[2:] = y[2:].flip(1)
     check_forward(y, t[:4].contiguous(), 3)
     check_backward(y, t[:4].contiguous(), False)
+
+
+def test_large_sums_below_a_far_larger_maximum():
+    """A thread's sums reach 5e8 before the largest logit comes; what is left of them is 0, not 0 times what times 1e30 is no finite number."""
+    vocab = 400_000_000
+    x = torch.full((1, vocab), 7.9, device=DEV)
+    x.view(8, -1)[:, :8192] = 0.0         # (sums against 0: e^7.9 a logit)
+    x[0, -1] = 3e38
+    t = torch.tensor([vocab - 1], device=DEV)
+    r = ops.token_log_probs(x, t)
+    ops.device_status()
+    assert float(r.log_probs) == 0.0 and float(r.entropy) == 0.0 and r.stats[0].tolist() == [x[0, -1].item(), 0.0]
