@@ -1317,6 +1317,7 @@ struct Polynomial {
     Step step[kMaxSteps];
     int steps = 0;
     double largest = 1.0;    // singular value at the chains' starts, hence element of X
+    double growth = 1.0;     // of an error of the Gram matrix in one chain of all steps
 };
 static int exponent_below(double bound) {  // largest e with bound * 2^e <= 2^15
     return std::max(-24, std::min(24, static_cast<int>(floor(log2(32768.0 / std::max(bound, 1e-6))))));
@@ -1327,6 +1328,7 @@ static bool polynomial(const double* coefficients, int steps, bool chained, Poly
     double l = kBetween, lambda[kPoints + 1], q[kPoints + 1], growth = 1.0;
     p->steps = steps;
     p->largest = l;
+    p->growth = 1.0;
     bool starts = true;
     for (int k = 0; k < steps; ++k) {
         Step& s = p->step[k];
@@ -1357,6 +1359,7 @@ static bool polynomial(const double* coefficients, int steps, bool chained, Poly
         s.et = exponent_below(mt * kBetween * kBetween);
         s.eq = exponent_below(mq * kBetween);
         growth *= std::max(1.0, mu * mu);
+        p->growth *= std::max(1.0, mu * mu);
         if (!(next <= 4096.0)) return false;  // singular values beyond 64
         s.ends = !chained || k == steps - 1 || growth > kGrowth;
         starts = s.ends;
@@ -1539,7 +1542,11 @@ static void launch_pack(const PackParams<kMaxRounds>& all, const Call& call, int
 }
 constexpr int kFewRounds = 22;
 
-// Whether a group goes through double precision: see nml_ortho_small.cuh.
+// Whether a group may go through double precision (see nml_ortho_small.cuh), and whether its steps do: one chain of them all amplifies what rounding leaves
+// of a Gram matrix's zero eigenvalues, 2^-53 either way, by kSmallGrowth at most.  Beyond, negative ones come near -1, where the polynomial has no bound
+// (rank 1, 64 x 147, default coefficients: 1e-10 off after 9 steps, 4e-6 after 12, 0.1 after 15, no numbers after 20); such steps are taken one by
+// one on X.  A single step is always below it.
+constexpr double kSmallGrowth = 1e10;
 static bool all_small(const Work* w, int count) {
     return std::all_of(w, w + count, [](const Work& v) { return v.s.m <= kSmall; });
 }
@@ -1602,7 +1609,7 @@ static int run_small(Work* w, int count, const Call& call, const Polynomial& pol
 
 // One group: three launches.
 static int run_group(Work* w, int count, const Call& call, const Steps& steps, void* workspace, size_t bytes, cudaStream_t st) {
-    if (all_small(w, count)) return run_small(w, count, call, steps.of[1], workspace, bytes, st);
+    if (all_small(w, count) && steps.of[1].growth <= kSmallGrowth) return run_small(w, count, call, steps.of[1], workspace, bytes, st);
     int* err;
     int sms;
     if (const int rc = nml::current_device(&err, &sms)) return rc;
@@ -1735,7 +1742,10 @@ static int workspace_of(int count, int math, int steps, F&& size, size_t* bytes)
     int sms = nml::usable_sms(), filled = 0;
     for (int k = 0; k <= count; ++k) {
         if (filled == kGroup || (k == count && filled > 0)) {
-            *bytes = std::max(*bytes, (all_small(w, filled) ? plan_small(w, filled).bytes : plan_group(w, filled, math, steps, sms).bytes) + 1024);
+            // (small matrices: room for either way, as the coefficients, which decide, are not known here)
+            const bool small = all_small(w, filled);
+            const size_t in_double = small ? plan_small(w, filled).bytes : 0, in_tiles = small && steps == 1 ? 0 : plan_group(w, filled, math, steps, sms).bytes;
+            *bytes = std::max(*bytes, std::max(in_double, in_tiles) + 1024);
             filled = 0;
         }
         if (k < count) {

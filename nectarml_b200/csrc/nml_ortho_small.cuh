@@ -4,7 +4,8 @@
 //   A = G G^T / (|G| + eps)^2;  U_k = a I + b A + c A^2,  A <- U_k A U_k,  Q <- U_k Q;  result = Q G / (|G| + eps)
 //
 // (all of them polynomials of the first A, so symmetric; |G|^2 is the trace of G G^T).  The steps square the condition number and
-// amplify the error of A by up to a^2 = 11.9 each, so this is done in double: 2^-53 a^10 = 2e-11, and the result is rounded once.
+// amplify the error of A by up to max u^2 each (a^2 = 11.9 with the default coefficients), so this is done in double and only where all steps together
+// amplify it by 1e10 at most: five default steps by 2.3e5, 2^-53 of which is 3e-11, nine by 5e9; and the result is rounded once.
 // With tiles of 128 in three products of halves a matrix of 64 x 147 took 116 us, 15 products of one tile, 7 us each: loads, flags and
 // stores.  Here it takes 59 us in three launches: partial Gram matrices of 64 columns a block; the steps, a block to a matrix; Q G, 64 columns a block.
 // Bound by the double-precision pipe: 64 FMAs a clock and SM, from registers or by mma.sync alike (both measured), so the lower blocks of a

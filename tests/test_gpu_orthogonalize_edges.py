@@ -1,0 +1,72 @@
+"""Orthogonalised matrices at the edges of their range: many steps on matrices that have not full rank."""
+import math
+
+import pytest
+import torch
+
+from nectarml_b200 import ops
+
+from test_gpu_orthogonalize import COEF, DEV, MODES, TOL, off, plain
+
+pytestmark = pytest.mark.gpu
+
+POLAR = (2.0, -1.5, 0.5)   # p(1) = 1, p'(1) = 0: singular values end at 1, from above 1.0018 at most
+
+
+def without_full_rank(rows, cols, kind, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    mk = lambda *s: torch.randn(*s, device=DEV, generator=g, dtype=torch.float64)
+    if kind == "duplicated rows":
+        a = mk(rows, cols)
+        a[rows - rows // 2:] = a[: rows // 2]
+    else:
+        rank = min(rows, cols, int(kind.split()[1]))
+        a = mk(rows, rank) @ mk(rank, cols)
+    return a.float()
+
+
+KINDS = pytest.mark.parametrize("kind", ["duplicated rows", "rank 1", "rank 8"])
+
+
+def check_steps(g, y, steps, coefficients, mode, largest):
+    """Everything finite and bounded as the polynomial is (what rounding leaves of the missing directions grows with the steps and may end as one of the
+    directions); with a polynomial that converges, the directions that the matrix has are the polar factor's.  A step is off by 8.9 u of
+    itself (u = 2^-12, or with two halves 2^-23 and as much again for the product of the low halves), and over the steps that adds up at most."""
+    y = y.double()
+    assert bool(y.isfinite().all())
+    u = 2.0 ** -12 if mode == "f16" else 2.0 ** -22
+    assert float(torch.linalg.matrix_norm(y, 2)) <= largest * (1 + steps * 8.9 * u)
+    if coefficients == POLAR:
+        left, s, right = torch.linalg.svd(g.double(), full_matrices=False)
+        n = int((s > 0.05 * s[0]).sum())
+        d = left[:, :n].T @ y @ right[:n].T
+        assert float((d - torch.eye(n, device=DEV)).norm()) <= steps * 8.9 * u * math.sqrt(n) * 2
+
+
+@MODES
+@KINDS
+@pytest.mark.parametrize("rows,cols", [(64, 147), (147, 64), (20, 33)])
+def test_many_steps_on_small_matrices(rows, cols, kind, mode):
+    """In double as long as one chain of all steps is exact (its result is off by a rounding, and by 2^-53 times the sums' 147 terms and what
+    directions that are not there take from one step to the next, 3.45^9); one by one beyond."""
+    g = without_full_rank(rows, cols, kind)
+    for steps in (1, 5, 9):
+        assert off(ops.orthogonalize(g, steps=steps, math=mode), plain(g, steps)) <= 2.0 ** -24 + 147 * 2.0 ** -53 * 3.4445 ** 9, steps
+    for steps in (10, 12, 16, 20, 32):
+        check_steps(g, ops.orthogonalize(g, steps=steps, math=mode), steps, COEF, mode, 1.21)
+    for steps in (15, 17, 20, 32):
+        check_steps(g, ops.orthogonalize(g, steps=steps, coefficients=POLAR, math=mode), steps, POLAR, mode, 1.0018)
+    ops.device_status()
+
+
+@KINDS
+def test_many_steps_of_the_optimizer_on_small_matrices(kind):
+    shapes = [(64, 147), (33, 20), (50,), (48, 4, 3, 3)]
+    grads = [without_full_rank(s[0], math.prod(s[1:]), kind, 1).reshape(s) if len(s) > 1 else torch.ones(s, device=DEV) for s in shapes]
+    for steps in (12, 20, 32):
+        params, momenta = [torch.zeros(s, device=DEV) for s in shapes], [torch.zeros(s, device=DEV) for s in shapes]
+        ops.muon_step(params, grads, momenta, lr=1.0, momentum=0.0, nesterov=False, scaling=None, steps=steps, coefficients=POLAR)
+        for p, g in zip(params, grads):
+            if p.dim() > 1:
+                check_steps(g.reshape(g.shape[0], -1), -p.reshape(p.shape[0], -1), steps, POLAR, "3xf16", 1.0018)
+    ops.device_status()
