@@ -253,7 +253,7 @@ int nml_l1_backward(const void* a, const void* b, size_t n, const float* dloss, 
  * [rows][vocab] (`pitch` elements apart, dtype NML_F32 or NML_F16, any alignment of an element), in one launch and one pass:
  *   log_probs[r] = log softmax(x_r)[targets[r]], entropy[r] = -sum p log p, stats[r] = (largest logit m, log sum e^(x - m)),
  *   top_log_probs / top_indices [rows][top], the most likely first, equal ones by index.
- * A negative target stands for padding: log probability 0, no gradient; one of vocab or more gives NaN.  A row whose logits are all
+ * A negative target stands for padding: log probability 0 without a gradient (its entropy is that of any row); one of vocab or more gives NaN.  A row whose logits are all
  * -inf has log probabilities -inf, entropy 0, stats (-inf, 0) and the alternatives 0, 1, ...; a row with a NaN or +inf has NaN
  * (and alternatives that are valid, otherwise unspecified, indices).  Sums are fp32, in a fixed order.
  * top: 0 (both pointers may be NULL) to 32, at most vocab; with alternatives vocab is at most 2,000,000 / 1,000,000 (fp16 / fp32). */

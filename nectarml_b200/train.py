@@ -582,7 +582,7 @@ class TrainStep:
     def __init__(self, net: _Net, loss: str, lr=0.1, momentum=0.9, weight_decay=1e-4, loss_scale=16384.0, entropy_weight=0.0,
                  optimizer="sgd"):
         """loss: "cross_entropy" (torch's, of logits and labels), "token_log_probs" (the same in the library's kernels, less
-        ``entropy_weight`` times the entropy of the predictions; a negative label is left out) or "l1".
+        ``entropy_weight`` times the entropy of the predictions; a row with a negative label is left out of both) or "l1".
         optimizer: "sgd" (momentum) or "muon" (orthogonalised momentum, see ParamStore.muon_step)."""
         if optimizer not in ("sgd", "muon"):
             raise ValueError(f"optimizer: 'sgd' or 'muon', got {optimizer!r}")
@@ -598,7 +598,7 @@ class TrainStep:
             r = token_log_probs(out, target)
             gain = r.log_probs.sum()
             if self.entropy_weight:
-                gain = gain + self.entropy_weight * r.entropy.sum()
+                gain = gain + self.entropy_weight * torch.where(target >= 0, r.entropy, 0.0).sum()
             return -gain / denom
         # (the kernels read pairs of values, so a view that starts on an odd one is left to torch, as is a count on the device)
         if (out.is_cuda and out.dtype == target.dtype == torch.float16 and out.shape == target.shape and out.is_contiguous()

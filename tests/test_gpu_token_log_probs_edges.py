@@ -86,3 +86,50 @@ def test_large_sums_below_a_far_larger_maximum():
     r = ops.token_log_probs(x, t)
     ops.device_status()
     assert float(r.log_probs) == 0.0 and float(r.entropy) == 0.0 and r.stats[0].tolist() == [x[0, -1].item(), 0.0]
+
+
+@DTYPES
+def test_training_loss_leaves_padding_out(dtype):
+    """Rows with a negative label count neither in the loss, the entropy's part included, nor in the gradient."""
+    x, t = logits((12, 300), dtype, 27), tokens((12,), 300)
+    kept = t >= 0
+    assert 0 < int(kept.sum()) < 12
+    step = train.TrainStep(None, "token_log_probs", entropy_weight=0.5)
+    value, grads = [], []
+    for rows in (torch.ones_like(kept), kept):
+        y = x[rows].clone().requires_grad_(True)
+        value.append(step._loss(y, t[rows], 8))
+        value[-1].backward()
+        grads.append(y.grad)
+    # (sums of the same numbers, among which the one has zeros, in whatever order: 12 roundings of a sum of 9 logs and entropies below 6 each)
+    assert abs(float(value[0].detach().double() - value[1].detach().double())) <= 24 * U * 9 * (10 + 0.5 * 6) / 8
+    assert not grads[0][~kept].any() and bool(grads[0][kept].any())
+    # (the same rows, but 300 logits are no whole number of 32-byte units, so without the padded ones they start elsewhere in them and are summed in another
+    # order: either side is good to what test_large_offsets derives, and rounded to its type)
+    size, c = (1 + 0.5 * 16) / 8, chain(300, dtype)
+    tol = 2 * 2 * size * (8 + c) * U + (2 * 2.0 ** -11 * grads[1].double().abs() + 2.0 ** -24 if dtype == torch.float16 else 0.0)
+    assert bool(((grads[0][kept].double() - grads[1].double()).abs() <= tol).all())
+
+
+def test_training_step_with_padding():
+    """Of labels that are all padding nothing is learned, with an entropy term too; of some, as much as torch's loss and entropy over the others give."""
+    n, classes = 8, 24
+    x = torch.randn(n, 64, 64, 3, device=DEV).half()
+    labels = torch.randint(0, classes, (n,), device=DEV)
+    for padded in (range(n), (1, 4, 5)):
+        t = labels.clone()
+        t[list(padded)] = -1
+        kept = t >= 0
+        net = train.ResNet50(DEV, num_classes=classes, blocks=(1, 1, 1, 1), width=16)
+        net.init(seed=3)
+        step = train.TrainStep(net, "token_log_probs", loss_scale=8192.0, entropy_weight=0.3)
+        value = float(step([(x, t)], global_count=n, optimize=False))
+        ops.device_status()
+        if not bool(kept.any()):
+            assert value == 0 and not net.store.grad.any()
+            continue
+        with torch.no_grad():
+            lp = net.forward(x).double().log_softmax(1)
+        h = -(lp * lp.exp()).sum(1)
+        want = -float((lp[kept, t[kept]] + 0.3 * h[kept]).sum()) / n
+        assert abs(value - want) <= 1e-5 * abs(want) and bool(net.store.grad.any())
