@@ -38,6 +38,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <iterator>
 #include <type_traits>
 #include <utility>
@@ -1760,13 +1761,26 @@ static int workspace_of(int count, int math, int steps, F&& size, size_t* bytes)
 
 using namespace nml_ortho;
 
+// Whether the product kernels have the registers that their split among the warps counts on; a build that gave them others would wait for registers
+// for good, so such a build refuses the calls of this file, and no others.  (Of the build, hence the same on every device.)
+static std::atomic<bool> g_split_holds{false};
+// Sets the device up.
+static int products_run() {
+    int* err;
+    int sms;
+    if (const int rc = nml::current_device(&err, &sms)) return rc;
+    return g_split_holds.load(std::memory_order_relaxed) ? NML_OK : NML_ERR_UNSUPPORTED;
+}
+
 int nml::prepare_ortho_kernels() {
     cudaFuncAttributes a;
+    bool holds = true;
     for (auto f : {ortho_product_kernel<1, false>, ortho_product_kernel<2, false>, ortho_product_kernel<2, true>}) {
         NMLO_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kProductSmem)));
         NMLO_CUDA(cudaFuncGetAttributes(&a, f));
-        if (a.numRegs != kLaunchRegs) return NML_ERR_UNSUPPORTED;  // (a build whose register split would not hold)
+        holds = holds && a.numRegs == kLaunchRegs;
     }
+    g_split_holds.store(holds, std::memory_order_relaxed);
     NMLO_CUDA(cudaFuncSetAttribute(small_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmallStepsSmem)));
     NMLO_CUDA(cudaFuncSetAttribute(small_result_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmallResultSmem)));
     NMLO_CUDA(cudaFuncSetAttribute(small_result_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmallResultSmem)));
@@ -1808,6 +1822,8 @@ int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int o
     Steps poly;
     if (!steps_of(coefficients, steps, &poly)) return NML_ERR_UNSUPPORTED;
     if (count > 0 && (!workspace || workspace_bytes < need)) return NML_ERR_WORKSPACE;
+    if (count > 0)
+        if (const int rc = products_run()) return rc;
     Call call;
     call.in_dtype = in_dtype;
     call.out_dtype = out_dtype;
@@ -1850,6 +1866,8 @@ int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, 
     Steps poly;
     if (!steps_of(coefficients, steps, &poly)) return NML_ERR_UNSUPPORTED;
     if (need > 0 && (!workspace || workspace_bytes < need)) return NML_ERR_WORKSPACE;
+    if (need > 0)
+        if (const int rc = products_run()) return rc;  // (before anything is updated)
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Call call;
     call.math = math;
