@@ -296,7 +296,8 @@ int nml_sgd_momentum_step(float* params, const float* grads, float* velocity, vo
  *                  fits fp16's range, which fp32 operands in general do not)
  *  NML_MATH_F16    operands rounded to fp16, except X where it is carried to the next step: 2 to 3e-3 of the result's norm
  * Zeros stay zeros; a matrix with a NaN or an infinity becomes NaN.  Matrices may be views: one of the strides (in elements) is 1, the other at least
- * the length of the dense run; a result may lie where its matrix does (with its strides and type) but must not overlap another one.  Coefficients under which a singular value could
+ * the length of the dense run; a result may lie where its matrix does (with its strides and type); otherwise it must not overlap it (NML_ERR_INVALID),
+ * nor another result, nor, in calls of more than 64 matrices, another matrix.  Coefficients under which a singular value could
  * grow beyond 64 are NML_ERR_UNSUPPORTED.  Results are bitwise repeatable; the
  * order of sums, and whether short sides up to 64 are taken in double, follow from the group's sizes, the polynomial (double holds a chain
  * of steps that amplifies errors by 1e10 at most: nine default ones) and the SMs in use. */

@@ -342,7 +342,6 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__
     const Source& s = w.s;
     const int half = at_half - first[k], i0 = half / (2 * w.nb) * kBlock, j0 = half % (2 * w.nb) * 64;
     uint8_t* const out = block_at(P.c.blocks, w.x[0], half / 2) + (half & 1) * kHalf;
-    if (j0 >= w.nb * kBlock) return;
     // the norm, from the partial sums in a fixed order
     double sum = 0.0;
     for (int i = tid; i < w.sums; i += 256) sum += load_double(P.c.sums + w.first_sum + i);
@@ -1523,6 +1522,7 @@ struct Call {
     float eps = 0.f;
     Momentum mo = {1.f, 0.f, false, false};
     bool apply = false;
+    bool packed = false;  // everything has to be read before anything is written
     float keep = 0.f, rate = 0.f;
     const int* skip = nullptr;
 };
@@ -1546,7 +1546,7 @@ constexpr int kFewRounds = 22;
 // Whether a group may go through double precision (see nml_ortho_small.cuh), and whether its steps do: one chain of them all amplifies what rounding leaves
 // of a Gram matrix's zero eigenvalues, 2^-53 either way, by kSmallGrowth at most.  Beyond, negative ones come near -1, where the polynomial has no bound
 // (rank 1, 64 x 147, default coefficients: 1e-10 off after 9 steps, 4e-6 after 12, 0.1 after 15, no numbers after 20); such steps are taken one by
-// one on X.  A single step is always below it.
+// one on X.
 constexpr double kSmallGrowth = 1e10;
 static bool all_small(const Work* w, int count) {
     return std::all_of(w, w + count, [](const Work& v) { return v.s.m <= kSmall; });
@@ -1610,7 +1610,7 @@ static int run_small(Work* w, int count, const Call& call, const Polynomial& pol
 
 // One group: three launches.
 static int run_group(Work* w, int count, const Call& call, const Steps& steps, void* workspace, size_t bytes, cudaStream_t st) {
-    if (all_small(w, count) && steps.of[1].growth <= kSmallGrowth) return run_small(w, count, call, steps.of[1], workspace, bytes, st);
+    if (all_small(w, count) && !call.packed && steps.of[1].growth <= kSmallGrowth) return run_small(w, count, call, steps.of[1], workspace, bytes, st);
     int* err;
     int sms;
     if (const int rc = nml::current_device(&err, &sms)) return rc;
@@ -1722,16 +1722,49 @@ static bool apart(const nml_muon_param* params, int count) {
         return false;
     }
 }
-// Whether every result has a place of its own.
-static bool apart(const nml_matrix* matrices, int count) {
+// The memory of a matrix (one of its strides is 1).
+static nml::Runs runs_of(const void* p, int rows, int cols, long long row, long long col, long long size) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    if (col == 1 && (row >= cols || rows == 1)) return {at, rows, cols * size, row * size};
+    return {at, cols, rows * size, col * size};
+}
+enum Places { APART, OVER_INPUTS, CLASH };
+// Where results lie: apart from one another, and each apart from its own matrix or where that one does (CLASH otherwise); OVER_INPUTS: some lie over other
+// matrices that are read.
+static Places places(const nml_matrix* matrices, int count, long long in_size, long long out_size) {
+    auto in = [&](int k) { return runs_of(matrices[k].in, matrices[k].rows, matrices[k].cols, matrices[k].in_row, matrices[k].in_col, in_size); };
+    auto out = [&](int k) { return runs_of(matrices[k].out, matrices[k].rows, matrices[k].cols, matrices[k].out_row, matrices[k].out_col, out_size); };
+    for (int k = 0; k < count; ++k)
+        if (matrices[k].in != matrices[k].out && overlap(in(k), out(k))) return CLASH;
+    if (count < 2) return APART;
+    struct Piece {
+        nml::Runs runs;
+        int k;
+    };
     try {
-        std::vector<const void*> out;
-        out.reserve(count);
-        for (int k = 0; k < count; ++k) out.push_back(matrices[k].out);
-        std::sort(out.begin(), out.end());
-        return std::adjacent_find(out.begin(), out.end()) == out.end();
+        std::vector<Piece> ins, outs;
+        std::vector<uintptr_t> reach;  // the furthest end of the first ones of `ins`
+        ins.reserve(count), outs.reserve(count), reach.reserve(count);
+        for (int k = 0; k < count; ++k) ins.push_back({in(k), k}), outs.push_back({out(k), k});
+        auto by_place = [](const Piece& a, const Piece& b) { return a.runs.at < b.runs.at; };
+        std::sort(ins.begin(), ins.end(), by_place);
+        std::sort(outs.begin(), outs.end(), by_place);
+        for (const Piece& p : ins) reach.push_back(std::max(p.runs.end(), reach.empty() ? 0 : reach.back()));
+        Places found = APART;
+        for (int o = 0; o < count; ++o) {
+            const Piece& p = outs[o];
+            for (int e = o + 1; e < count && outs[e].runs.at < p.runs.end(); ++e)
+                if (overlap(p.runs, outs[e].runs)) return CLASH;
+            if (found == OVER_INPUTS) continue;
+            for (size_t e = std::upper_bound(reach.begin(), reach.end(), p.runs.at) - reach.begin(); e < ins.size() && ins[e].runs.at < p.runs.end(); ++e)
+                if (ins[e].k != p.k && overlap(p.runs, ins[e].runs)) {
+                    found = OVER_INPUTS;
+                    break;
+                }
+        }
+        return found;
     } catch (...) {
-        return false;
+        return CLASH;
     }
 }
 
@@ -1744,9 +1777,8 @@ static int workspace_of(int count, int math, int steps, F&& size, size_t* bytes)
     for (int k = 0; k <= count; ++k) {
         if (filled == kGroup || (k == count && filled > 0)) {
             // (small matrices: room for either way, as the coefficients, which decide, are not known here)
-            const bool small = all_small(w, filled);
-            const size_t in_double = small ? plan_small(w, filled).bytes : 0, in_tiles = small && steps == 1 ? 0 : plan_group(w, filled, math, steps, sms).bytes;
-            *bytes = std::max(*bytes, std::max(in_double, in_tiles) + 1024);
+            const size_t in_double = all_small(w, filled) ? plan_small(w, filled).bytes : 0;
+            *bytes = std::max(*bytes, std::max(in_double, plan_group(w, filled, math, steps, sms).bytes) + 1024);
             filled = 0;
         }
         if (k < count) {
@@ -1818,7 +1850,10 @@ int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int o
         // in place: element by element
         if (x.in == x.out && (in_dtype != out_dtype || x.in_row != x.out_row || x.in_col != x.out_col)) return NML_ERR_INVALID;
     }
-    if (!apart(matrices, count)) return NML_ERR_INVALID;
+    // Tiles are packed from all matrices of a group before the first result is written; from double precision, and from one group to the next, results are
+    // written while others' matrices are still to be read.
+    const Places where = places(matrices, count, in_dtype == NML_F16 ? 2 : 4, out_dtype == NML_F16 ? 2 : 4);
+    if (where == CLASH || (where == OVER_INPUTS && count > kGroup)) return NML_ERR_INVALID;
     Steps poly;
     if (!steps_of(coefficients, steps, &poly)) return NML_ERR_UNSUPPORTED;
     if (count > 0 && (!workspace || workspace_bytes < need)) return NML_ERR_WORKSPACE;
@@ -1829,6 +1864,7 @@ int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int o
     call.out_dtype = out_dtype;
     call.math = math;
     call.eps = eps;
+    call.packed = where == OVER_INPUTS;
     Work w[kGroup];
     for (int at = 0; at < count; at += kGroup) {
         const int n = std::min(kGroup, count - at);

@@ -1,12 +1,12 @@
-"""Orthogonalised matrices at the edges of their range: many steps on matrices that have not full rank."""
+"""Orthogonalised matrices at the edges of their range: many steps on matrices that have not full rank, results over matrices."""
 import math
 
 import pytest
 import torch
 
-from nectarml_b200 import ops
+from nectarml_b200 import _lib, ops
 
-from test_gpu_orthogonalize import COEF, DEV, MODES, TOL, off, plain
+from test_gpu_orthogonalize import COEF, DEV, MODES, TOL, gradient, off, plain
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,37 @@ def test_many_steps_of_the_optimizer_on_small_matrices(kind):
             if p.dim() > 1:
                 check_steps(g.reshape(g.shape[0], -1), -p.reshape(p.shape[0], -1), steps, POLAR, "3xf16", 1.0018)
     ops.device_status()
+
+
+@MODES
+@pytest.mark.parametrize("rows,cols", [(20, 40), (64, 2000), (300, 200)])
+def test_results_over_other_matrices(rows, cols, mode):
+    """Every matrix of a call is read before a result is written: two that trade places, one that is read in place and elsewhere."""
+    a, b = gradient(rows, cols, seed=31), gradient(rows, cols, seed=32)
+    want = plain(a), plain(b)
+    x, y = a.clone(), b.clone()
+    ops.orthogonalize([x, y], out=[y, x], math=mode)
+    assert off(y, want[0]) <= TOL[mode] and off(x, want[1]) <= TOL[mode]
+    x, y = a.clone(), torch.empty_like(a)
+    ops.orthogonalize([x, x], out=[x, y], math=mode)
+    assert off(x, want[0]) <= TOL[mode] and torch.equal(x, y)
+    ops.device_status()
+
+
+def test_results_in_one_buffer():
+    """Side by side in the rows of one buffer, and refused where they meet."""
+    a, b = gradient(90, 70, seed=33), gradient(90, 50, seed=34)
+    room = torch.full((90, 130), 5.0, device=DEV)
+    ops.orthogonalize([a, b], out=[room[:, 3:73], room[:, 73:123]])
+    assert off(room[:, 3:73], plain(a)) <= TOL["3xf16"] and off(room[:, 73:123], plain(b)) <= TOL["3xf16"]
+    assert room[:, :3].eq(5).all() and room[:, 123:].eq(5).all()
+    kept = room.clone()
+    batch = torch.empty(3 * 90 * 70, device=DEV)
+    for mats, outs in (([a, b], [room[:, 3:73], room[:, 72:122]]), ([a[:40], a[:40].clone()], [room[:40, :70], room[39:79, :70]])):
+        with pytest.raises(_lib.NectarB200Error, match="status 1"):
+            ops.orthogonalize(mats, out=outs)
+    with pytest.raises(_lib.NectarB200Error, match="status 1"):   # a batch whose results lie half a matrix apart
+        ops.orthogonalize(torch.stack([a, a]), out=batch.as_strided((2, 90, 70), (90 * 35, 70, 1)))
+    with pytest.raises(_lib.NectarB200Error, match="status 1"):
+        ops.orthogonalize(room[:89, :70], out=room[1:, :70])
+    assert torch.equal(room, kept)
