@@ -260,7 +260,8 @@ int nml_l1_backward(const void* a, const void* b, size_t n, const float* dloss, 
 int nml_token_log_probs(const void* logits, int dtype, long long rows, int vocab, long long pitch, const long long* targets, int top,
                         float* log_probs, float* entropy, float* stats, float* top_log_probs, long long* top_indices, void* stream);
 /* d_logits = d_log_probs (1[j = target] - p_j) - d_entropy p_j (log p_j + entropy), in the logits' type; d_entropy may be NULL (then
- * entropy may be too).  Rows of -inf alone get zeros.  d_logits may be the logits' own memory (with their pitch). */
+ * entropy may be too).  Rows of -inf alone get zeros.  d_logits may be the logits' own memory (with their pitch); otherwise
+ * it must not overlap what is read (NML_ERR_INVALID). */
 int nml_token_log_probs_backward(const void* logits, int dtype, long long rows, int vocab, long long pitch, const long long* targets,
                                  const float* stats, const float* entropy, const float* d_log_probs, const float* d_entropy, void* d_logits,
                                  long long d_pitch, void* stream);

@@ -799,12 +799,21 @@ int nml_token_log_probs_backward(const void* logits, int dtype, long long rows, 
                                  long long d_pitch, void* stream) {
     if (!shape_ok(logits, dtype, rows, vocab, pitch) || !shape_ok(d_logits, dtype, rows, vocab, d_pitch)) return NML_ERR_INVALID;
     if (!targets || !stats || !d_log_probs || (d_entropy && !entropy)) return NML_ERR_INVALID;
-    if (d_logits == logits && d_pitch != pitch && rows > 1) return NML_ERR_INVALID;
     if (!aligned(4, stats, entropy, d_log_probs, d_entropy) || !aligned(8, targets)) return NML_ERR_INVALID;
+    const int size = dtype == NML_F16 ? 2 : 4, n = kUnitBytes / size;
+    {  // the result: element for element where the logits are, or apart from them; and from what its row's blocks read first
+        auto runs = [&](const void* p, long long count, long long length, long long step) {
+            return nml::Runs{reinterpret_cast<uintptr_t>(p), count, length, step};
+        };
+        const nml::Runs out = runs(d_logits, rows, static_cast<long long>(vocab) * size, d_pitch * size);
+        const bool in_place = d_logits == logits && (d_pitch == pitch || rows == 1);
+        if (!in_place && overlap(out, runs(logits, rows, static_cast<long long>(vocab) * size, pitch * size))) return NML_ERR_INVALID;
+        auto meets = [&](const void* p, long long each) { return p && overlap(out, runs(p, 1, rows * each, rows * each)); };
+        if (meets(targets, 8) || meets(stats, 8) || meets(d_log_probs, 4) || meets(d_entropy, 4) || (d_entropy && meets(entropy, 4))) return NML_ERR_INVALID;
+    }
     int* status;
     int sms;
     if (const int rc = nml::current_device(&status, &sms)) return rc;
-    const int size = dtype == NML_F16 ? 2 : 4, n = kUnitBytes / size;
     const long long units = (static_cast<long long>(vocab) + 2 * n - 2) / n;
     long long per_row = (units + 2047) / 2048;  // eight units a thread
     if (rows * per_row > 0x7fffffff) per_row = 1;

@@ -291,7 +291,8 @@ def token_log_probs_backward(logits: torch.Tensor, targets: torch.Tensor, stats:
                              d_log_probs: torch.Tensor, d_entropy: Optional[torch.Tensor] = None, *,
                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of the logits, in their dtype, from those of the log probabilities and (optional) the entropies; ``stats`` and
-    ``entropy`` are the forward's.  Padding takes no gradient of its log probability, a row of -inf alone none at all.  ``out`` may be the logits themselves."""
+    ``entropy`` are the forward's.  Padding takes no gradient of its log probability, a row of -inf alone none at all.  ``out`` may be the logits themselves,
+    or lies apart from what is read."""
     return _native.token_log_probs_backward(logits, targets, stats, entropy, d_log_probs, d_entropy, out)
 
 

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from nectarml_b200 import ops, train
+from nectarml_b200 import _lib, ops, train
 
 from test_gpu_token_log_probs import DEV, DTYPES, U, chain, check_backward, check_forward, logits, plain, tokens
 
@@ -133,3 +133,29 @@ def test_training_step_with_padding():
         h = -(lp * lp.exp()).sum(1)
         want = -float((lp[kept, t[kept]] + 0.3 * h[kept]).sum()) / n
         assert abs(value - want) <= 1e-5 * abs(want) and bool(net.store.grad.any())
+
+
+@DTYPES
+def test_gradient_beside_the_logits(dtype):
+    """Between the logits' rows, in the columns beside them, in place in a view; and refused where it would lie over other elements."""
+    x = logits((6, 501), dtype, 28)
+    t = tokens((6,), 501)
+    room = torch.empty(12, 501, dtype=dtype, device=DEV)
+    room[0::2] = x
+    check_backward(room[0::2], t, True, out=room[1::2])
+    assert torch.equal(room[0::2], x)
+    wide = torch.empty(6, 1010, dtype=dtype, device=DEV)
+    wide[:, :501] = x
+    check_backward(wide[:, :501], t, True, out=wide[:, 501:1002])
+    assert torch.equal(wide[:, :501], x)
+    r = ops.token_log_probs(x, t)
+    ones = torch.ones(6, device=DEV)
+    for a, b in ((wide[:, :501], wide[:, 500:1001]), (wide[:, 1:502], wide[:, :501]), (wide[:5, :501], wide[1:, :501])):
+        n = a.shape[0]
+        with pytest.raises(_lib.NectarB200Error, match="status 1"):
+            ops.token_log_probs_backward(a, t[:n], r.stats[:n], None, ones[:n], out=b)
+    one = wide[:1, 3:504]
+    one.copy_(x[:1])
+    first = ops.token_log_probs(one, t[:1])
+    got = ops.token_log_probs_backward(one, t[:1], first.stats, None, ones[:1], out=wide.view(-1)[3:504].view(1, 501))   # one row, in place, another pitch
+    assert got.data_ptr() == one.data_ptr() and bool(got.isfinite().all())
