@@ -28,6 +28,7 @@
 #include <initializer_list>
 #include <memory>
 #include <mutex>
+#include <optional>
 #include <string>
 #include <utility>
 #include <vector>
@@ -1128,6 +1129,11 @@ PyObject* py_orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!arity(n, 7)) return nullptr;
     return guarded([&]() -> PyObject* {
         const Items in(a[0], "matrices: a sequence of tensors");
+        std::optional<Items> outs;  // (until the results are wrapped: the items of what is no list or tuple belong to it)
+        if (a[1] != Py_None) {
+            outs.emplace(a[1], "out: a sequence of tensors");
+            require(outs->size() == in.size(), "out: one tensor for each matrix");
+        }
         const long out_code = as_int(a[2]);
         const int math = static_cast<int>(as_int(a[3]));
         const std::vector<double> c = coefficients_of(a[4]);
@@ -1147,13 +1153,7 @@ PyObject* py_orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 in_dtype = dtype;
             }
             require(dtype == in_dtype && x.device() == first->device(), "matrices of one dtype on one device");
-            PyObject* given = Py_None;
-            if (a[1] != Py_None) {
-                const Items outs(a[1], "out: a sequence of tensors");
-                require(outs.size() == in.size(), "out: one tensor for each matrix");
-                given = outs[k];
-            }
-            results.push_back(output(given, x.sizes(), out_code, x));
+            results.push_back(output(outs ? (*outs)[k] : Py_None, x.sizes(), out_code, x));
             const at::Tensor& y = results.back();
             require(y.sizes() == x.sizes() && y.device() == x.device(), "out: shape and device of its matrix");
             if (k == 0) out_dtype = dtype_of(y);

@@ -104,3 +104,24 @@ def test_results_in_one_buffer():
     with pytest.raises(_lib.NectarB200Error, match="status 1"):
         ops.orthogonalize(room[:89, :70], out=room[1:, :70])
     assert torch.equal(room, kept)
+
+
+def test_results_given_as_any_sequence():
+    """A list, a tuple, the matrices of one tensor, or what is run through once."""
+    gs = [gradient(30 + k, 50, seed=40 + k) for k in range(2)] + [gradient(30, 50, seed=42)]
+    want = ops.orthogonalize(gs)
+    mk = lambda: [torch.empty_like(g) for g in gs]
+    for wrap in (list, tuple, iter, lambda o: (x for x in o)):
+        outs = mk()
+        got = ops.orthogonalize(gs, out=wrap(outs))
+        assert all(y.data_ptr() == o.data_ptr() and torch.equal(o, w) for y, o, w in zip(got, outs, want))
+    same = [gs[2], gs[2].neg()]
+    out = torch.zeros(2, 30, 50, device=DEV)
+    got = ops.orthogonalize(same, out=out)
+    assert torch.equal(out[0], want[2]) and torch.equal(out[1], -want[2]) and got[1].data_ptr() == out[1].data_ptr()
+    got = ops.orthogonalize(torch.stack(same), out=out)   # (a batch with its batch)
+    assert got is out or got.data_ptr() == out.data_ptr()
+    with pytest.raises(AssertionError, match="one tensor for each"):
+        ops.orthogonalize(gs, out=iter(mk()[:2]))
+    with pytest.raises(TypeError):
+        ops.orthogonalize(gs, out=3)

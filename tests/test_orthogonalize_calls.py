@@ -2,8 +2,9 @@
 import ctypes as C
 
 import pytest
+import torch
 
-from nectarml_b200 import _lib
+from nectarml_b200 import _lib, ops
 
 P = 4096
 
@@ -116,3 +117,12 @@ def test_overlaps_against_sets_of_bytes(lib):
 def test_one_input_many_times(lib):
     """A matrix that is read as often as one likes costs no more than the others."""
     assert _call(lib, [_rows(A, OUT + 0x1000 * k, 8, 8) for k in range(20000)]) == WORKSPACE
+
+
+def test_results_have_to_match_in_number():
+    x = torch.zeros(4, 6)
+    for outs in ([], [x, x], iter([]), torch.zeros(2, 4, 6)):
+        with pytest.raises(AssertionError, match="one tensor for each"):
+            ops.orthogonalize([x], out=outs)
+    with pytest.raises(TypeError, match="sequence"):
+        ops.orthogonalize([x], out=3)
