@@ -1267,7 +1267,8 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
 namespace nml_ortho {
 
 // ---------------------------------------------------------------- parameters that are no matrices --
-constexpr int kVectors = 128;
+constexpr int kVectors = 128;          // pieces of one launch
+constexpr int kVectorPiece = 16384;    // values of a piece: a longer vector is several
 struct Vector {
     float* param;
     const float* grad;
@@ -1281,7 +1282,7 @@ struct VectorParams {
     float keep, rate;
     const int* skip;
 };
-// Plain momentum: p = p keep - rate u, a block to a vector.
+// Plain momentum: p = p keep - rate u, a block to a piece of a vector.
 __global__ void __launch_bounds__(256) momentum_vectors_kernel(const __grid_constant__ VectorParams P) {
     pdl_enter();
     if (skipped(P.skip)) return;
@@ -1920,24 +1921,31 @@ int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, 
     vectors.skip = found_inf;
     Work w[kGroup];
     int matrices = 0, others = 0;
+    auto run_vectors = [&]() -> int {
+        int* err;
+        int sms;
+        if (const int rc = nml::current_device(&err, &sms)) return rc;
+        nml::launch(momentum_vectors_kernel, others, 256, 0, st, vectors);
+        NMLO_CUDA(cudaGetLastError());
+        nml::count_launches(1);
+        others = 0;
+        return NML_OK;
+    };
     for (int k = 0; k <= count; ++k) {
         if (matrices == kGroup || (k == count && matrices > 0)) {
             if (const int rc = run_group(w, matrices, call, poly, workspace, workspace_bytes, st)) return rc;
             matrices = 0;
         }
-        if (others == kVectors || (k == count && others > 0)) {
-            int* err;
-            int sms;
-            if (const int rc = nml::current_device(&err, &sms)) return rc;
-            nml::launch(momentum_vectors_kernel, others, 256, 0, st, vectors);
-            NMLO_CUDA(cudaGetLastError());
-            nml::count_launches(1);
-            others = 0;
-        }
         if (k == count) break;
         const nml_muon_param& p = params[k];
         if (p.rows == 0) {
-            vectors.v[others++] = {p.param, p.grad, p.momentum, static_cast<__half*>(p.param_f16), p.cols};
+            for (long long from = 0; from < p.cols; from += kVectorPiece) {
+                __half* const half = static_cast<__half*>(p.param_f16);
+                vectors.v[others++] = {p.param + from, p.grad + from, p.momentum + from, half ? half + from : nullptr,
+                                       static_cast<int>(std::min<long long>(kVectorPiece, p.cols - from))};
+                if (others == kVectors)
+                    if (const int rc = run_vectors()) return rc;
+            }
             continue;
         }
         const long long row = p.cols, col = 1;
@@ -1948,7 +1956,7 @@ int nml_muon_step(const nml_muon_param* params, int count, int math, int steps, 
         set_sizes(w[matrices].s, p.rows, p.cols);
         ++matrices;
     }
-    return NML_OK;
+    return others > 0 ? run_vectors() : NML_OK;
 }
 
 }  // extern "C"

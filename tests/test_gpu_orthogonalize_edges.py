@@ -125,3 +125,32 @@ def test_results_given_as_any_sequence():
         ops.orthogonalize(gs, out=iter(mk()[:2]))
     with pytest.raises(TypeError):
         ops.orthogonalize(gs, out=3)
+
+
+@pytest.mark.parametrize("n", [16383, 16384, 16385, 2_100_003])
+def test_long_vectors(n):
+    """Vectors of any length, beside short ones: 2^-22 is four roundings of fp32."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    mk = lambda: [torch.randn(k, device=DEV, generator=g) for k in (n, 5, n, 1)]
+    params, grads, momenta = mk(), mk(), mk()
+    halves = [p.half() for p in params]
+    want = []
+    for p, q, v in zip(params, grads, momenta):
+        v = 0.9 * v.double() + q.double()
+        want.append((p.double() * (1 - 0.02 * 0.1) - 0.02 * (q.double() + 0.9 * v), v))
+    ops.muon_step(params, grads, momenta, halves, lr=0.02, momentum=0.9, weight_decay=0.1)
+    ops.device_status()
+    for p, v, h, (wp, wv) in zip(params, momenta, halves, want):
+        assert bool(((p.double() - wp).abs() <= 2.0 ** -22 * (1 + wp.abs())).all())
+        assert bool(((v.double() - wv).abs() <= 2.0 ** -22 * (4 + wv.abs())).all()) and torch.equal(h, p.half())
+
+
+def test_the_longest_vector():
+    """2^31 - 1 values: an index that goes on by a block's threads must not pass 2^31 (25 GB; powers of two, so exact)."""
+    n = 2 ** 31 - 1
+    p, q, v = (torch.full((n,), value, device=DEV) for value in (1.0, 0.5, 0.25))
+    ops.muon_step([p], [q], [v], lr=0.5, momentum=0.5, nesterov=False)
+    ops.device_status()
+    for part in (slice(0, 100000), slice(2 ** 30 - 100, 2 ** 30 + 100), slice(n - 100000, n)):
+        assert bool((v[part] == 0.625).all()) and bool((p[part] == 1 - 0.3125).all())
+    assert float(p.min()) == float(p.max()) == 0.6875
