@@ -18,7 +18,7 @@
 // being worked on.
 //
 // Operands are fp16.  |X| <= 1 bounds every element of every matrix here, so powers of two chosen on the host put all of them
-// into fp16's range, which needs no look at the data.
+// into fp16's range; of the data only |G| next to eps matters to that (see lift_of).
 //   "3xf16" (fp32 results): every operand is a high and a low half, 22 bits, and a product is the three that matter, in fp32
 //           accumulators: an error of about 2^-22 of the largest element a product, below that of fp32 products by FMA.
 //   "f16"   one product.  What may not be rounded to 11 bits is X itself where it is carried from step to step: noise in directions whose singular
@@ -88,6 +88,7 @@ struct Symmetric {  // buffers of one symmetric product
 struct Op {
     int kind, jobs;            // of symmetric products: the tiles of a second one follow those of the first
     int gram, from;            // POLY: of X X^T; which copy of X is read
+    int grown;                 // log2 of what the steps may have multiplied that X by, and in higher bits, of what they may have the one that is written
     Symmetric job[2];
     float f1, d1;
     int left;                  // ITERATE, RESULT: the symmetric factor
@@ -122,7 +123,7 @@ struct alignas(16) Work {
     int first_gram, first_symmetric, first_update, first_parts;  // its tiles: of X X^T, symmetric products, Q X, SUM
     int wide;                           // 64-column groups to a tile of Q X: 1, 2 or 4
     int fine, parts;                    // tiles to a block of a symmetric product, 1 or 2; parts of K of X X^T
-    float sx;                           // X is stored times this
+    int sx;                             // X is stored times 2^sx, and more where it is small (see lift)
     int chained;
 };
 template <int N>
@@ -135,6 +136,7 @@ struct Common {
     double* sums;
     Round* rounds;
     int* done;        // the tile counter, and behind it every matrix's finished eighths of tiles
+    int* lifts;       // every matrix's lift
     uint8_t* blocks;
     const int* skip;  // the optimizer step's: do nothing where this is set
     int count;
@@ -171,6 +173,19 @@ __device__ __forceinline__ int owner_of(const int (&first)[N], int count, int k)
     }
     return lo;
 }
+
+// Where |G| is far below eps, X starts at a norm far below 1, and the halves of its elements would be too few bits of fp16's range (64 bits off by 2e-2 at
+// |G| = 1e-6 eps, where fp32 is by 1e-7).  So it is stored times 2^lift more, lift = floor(log2 (|G| + eps) / |G|), less what the steps so far may have
+// multiplied it by, as long as that is positive.
+constexpr int kMostLift = 100;
+__device__ __forceinline__ int lift_of(double own, double norm) {
+    const double over = norm / own;  // (NaN and infinities: none)
+    return over > 1.0 ? min(kMostLift, ilogb(over)) : 0;
+}
+__device__ __forceinline__ int lifted(int lift, int grown) { return max(0, lift - grown); }
+constexpr int kGrownBits = 8;
+// 2^e, 0 below fp32's normal range.
+__device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.f : __int_as_float((e + 127) << 23); }
 
 template <typename T>
 __device__ __forceinline__ float load_as_float(const T* p) { return static_cast<float>(load_global(p)); }
@@ -352,8 +367,10 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__
     sum = part[0];
 #pragma unroll
     for (int q = 1; q < 8; ++q) sum += part[q];
-    const double norm = sqrt(sum) + static_cast<double>(P.eps);
-    const double inv = norm == 0.0 ? 0.0 : static_cast<double>(w.sx) / norm;  // (zeros stay zeros without an eps too)
+    const double own = sqrt(sum), norm = own + static_cast<double>(P.eps);
+    const int lift = lift_of(own, norm);
+    const double inv = norm == 0.0 ? 0.0 : ldexp(1.0, w.sx + lift) / norm;  // (zeros stay zeros without an eps too)
+    if (half == 0 && tid == 0) P.c.lifts[k] = lift;
     const T* const in = static_cast<const T*>(s.in);
     auto update = [&](float v, float momentum) {  // of the element's gradient and new momentum
         if (P.mo.on) {
@@ -507,7 +524,7 @@ constexpr int kQueue = 4;            // tiles that the producer may be ahead
 struct Info {        // of a matrix
     int m, n, nb, wide, fine, parts;
     uint32_t x[2], sym, partial;
-    float sx;
+    float factor;    // of the accumulators, a power of two: from X's scale to that of what is written
 };
 // Thirty-two rows and columns of a result, from a warp's room in shared memory.
 __device__ __forceinline__ void write_columns(const ProductParams& P, const uint8_t* staging, uint8_t* out, uint8_t* half, float rate, long long out_i,
@@ -728,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                         const int* const words = reinterpret_cast<const int*>(&rounds[round].op[cls]);
                         const int word = lane < kOpWords ? load_global(words + lane) : 0;
                         const int kind = __shfl_sync(0xffffffffu, word, offsetof(Op, kind) / 4), jobs = __shfl_sync(0xffffffffu, word, offsetof(Op, jobs) / 4);
-                        const int gram = __shfl_sync(0xffffffffu, word, offsetof(Op, gram) / 4);
+                        const int gram = __shfl_sync(0xffffffffu, word, offsetof(Op, gram) / 4), grown = __shfl_sync(0xffffffffu, word, offsetof(Op, grown) / 4);
                         is_wide = kind == ITERATE || kind == RESULT;
                         whole = kind == POLY && gram;
                         // (matrices of the first class come first, and their tiles count from 0; those of the second behind all of the first)
@@ -747,7 +764,11 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                             const Work* const from = P.c.table + a;
                             auto word = [](const uint32_t* p) { return static_cast<uint32_t>(load_global(reinterpret_cast<const int*>(p))); };
                             w = {load_global(&from->s.m), load_global(&from->s.n), load_global(&from->nb), load_global(&from->wide), load_global(&from->fine),
-                                 load_global(&from->parts), {word(&from->x[0]), word(&from->x[1])}, word(&from->sym), word(&from->partial), load_global(&from->sx)};
+                                 load_global(&from->parts), {word(&from->x[0]), word(&from->x[1])}, word(&from->sym), word(&from->partial), 1.f};
+                            const int lift = load_global(P.c.lifts + a), scale = load_global(&from->sx) + lifted(lift, grown & ((1 << kGrownBits) - 1));
+                            if (gram) w.factor = power_of_two(-2 * scale);
+                            if (kind == RESULT) w.factor = power_of_two(-scale);
+                            if (kind == ITERATE) w.factor = power_of_two(lifted(lift, grown >> kGrownBits) - lifted(lift, grown & ((1 << kGrownBits) - 1)));
                         }
                         mb = (w.m + kBlock - 1) / kBlock;
                         symmetric_tiles = symmetric_count<kPair>(mb) * w.fine;
@@ -1140,7 +1161,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 const long long out_i = load_wide(&src->out_i), out_j = load_wide(&src->out_j);
                 uint8_t* const out = reinterpret_cast<uint8_t*>(load_wide(reinterpret_cast<const long long*>(&src->out)));
                 uint8_t* const half = reinterpret_cast<uint8_t*>(load_wide(reinterpret_cast<const long long*>(&src->half)));
-                const float f0 = op_f1 / w.sx, rate = P.rate * load_global(&src->scale);  // (a power of two)
+                const float f0 = op_f1 * w.factor, rate = P.rate * load_global(&src->scale);  // (a power of two)
                 const int i0 = tile_i * kBlock + quarter * 32, j0 = tile_j * kBlock + g0 * 16;
                 // Thirty-two columns at a time go through shared memory: where rows lie densely, eight lanes write a row's 128 bytes; else the lanes
                 // of a warp lie beside one another along a column.
@@ -1161,7 +1182,6 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 const bool iterate = kind == ITERATE;
                 const uint32_t to = iterate ? (from_x ? w.x[0] : w.x[1]) : symmetric_first(w, job.out);
                 const int block = iterate ? tile_i * w.nb + tile_j : lower(tile_i, tile_j);
-                const float over = gram ? 1.f / (w.sx * w.sx) : 1.f;  // (a power of two)
                 // Thirty-two columns of both planes at a time go through shared memory, so that four lanes write 64 contiguous bytes of a row (a thread's
                 // own 32 bytes, in 32 lines a store, took 1.1 us a matrix and tile; bulk copies of 4 KB out of shared memory, whose room
                 // has to be waited for, 3).
@@ -1238,7 +1258,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                 const int matrices = !in_use || above || partial || groups == 0 ? 0 : kind == POLY || kind == SUM ? 2 : 1;
 #pragma unroll 1
                 for (int e = 0; e < matrices; ++e) {  // (A and P: f0 is a power of two)
-                    scale(e ? op_f1 / job.f0 : (iterate ? op_f1 : job.f0) * over);
+                    scale(e ? op_f1 / job.f0 : (iterate ? op_f1 : job.f0) * w.factor);
                     if (e || kind == PLAIN) add_diagonal(e ? op_d1 : job.d1);
                     store(e ? symmetric_first(w, kPoly) : to, iterate || kPlanes == 2);
                 }
@@ -1313,6 +1333,7 @@ struct Step {
     double a, b, c;
     int ea, ep, eu, et, eq;  // A, P, U, T and Q are stored times 2^e
     bool starts, ends;       // a chain
+    int grown;               // where it ends: log2 of what X may have been multiplied by, at least 0
 };
 struct Polynomial {
     Step step[kMaxSteps];
@@ -1326,7 +1347,7 @@ static int exponent_below(double bound) {  // largest e with bound * 2^e <= 2^15
 static bool polynomial(const double* coefficients, int steps, bool chained, Polynomial* p) {
     constexpr int kPoints = 128;        // singular values, at which the matrices' eigenvalues are followed
     constexpr double kBetween = 1.01;   // and what lies between two of them
-    double l = kBetween, lambda[kPoints + 1], q[kPoints + 1], growth = 1.0;
+    double l = kBetween, lambda[kPoints + 1], q[kPoints + 1], growth = 1.0, multiplied = 0.0;  // (log2)
     p->steps = steps;
     p->largest = l;
     p->growth = 1.0;
@@ -1364,7 +1385,11 @@ static bool polynomial(const double* coefficients, int steps, bool chained, Poly
         if (!(next <= 4096.0)) return false;  // singular values beyond 64
         s.ends = !chained || k == steps - 1 || growth > kGrowth;
         starts = s.ends;
-        if (s.ends) l = std::max(sqrt(next) * kBetween, 1e-3), p->largest = std::max(p->largest, l);
+        if (s.ends) {
+            l = std::max(sqrt(next) * kBetween, 1e-3), p->largest = std::max(p->largest, l);
+            multiplied += log2(std::max(mq * kBetween, 1e-30));
+            s.grown = std::max(0, std::min(kMostLift, static_cast<int>(ceil(multiplied))));
+        }
     }
     return true;
 }
@@ -1445,7 +1470,7 @@ static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
     p.sums_at = round_up(sizeof(Work) * kGroup, 256);
     p.rounds_at = p.sums_at + round_up(sizeof(double) * p.sums, 256);
     p.done_at = p.rounds_at + round_up(sizeof(Round) * kMaxRounds, 256);
-    p.blocks_at = p.done_at + round_up(sizeof(int) * (kGroup + 1), 1024);
+    p.blocks_at = p.done_at + round_up(sizeof(int) * (2 * kGroup + 1), 1024);
     p.blocks_at = round_up(p.blocks_at, 1024);
     p.bytes = p.blocks_at + static_cast<size_t>(p.blocks) * 2 * kPlane;
     return p;
@@ -1453,6 +1478,7 @@ static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
 
 // The products of a class, in order; their number.
 static int build_ops(const Polynomial& poly, uint32_t identity, bool in_parts, Op* ops) {
+    int grown = 0;             // of the present X
     int n = 0, from = 0, gram_before = 0, symmetric_before = 0, wide_before = 0, sum_before = 0;
     auto add = [&](Op op) {
         op.jobs = std::max(op.jobs, 1);
@@ -1478,6 +1504,7 @@ static int build_ops(const Polynomial& poly, uint32_t identity, bool in_parts, O
         a.kind = POLY;
         a.gram = s.starts;
         a.from = from;
+        a.grown = grown;
         if (s.starts) a.job[0] = {0, 0, kGram, static_cast<float>(ldexp(1.0, s.ea)), 0.f};
         else a.job[0] = symmetric(u, eu_last, kT, poly.step[k - 1].et, kGram, s.ea, 0.0);
         a.f1 = static_cast<float>(ldexp(s.c, s.ep - (s.starts ? 0 : eu_last + poly.step[k - 1].et)));
@@ -1511,6 +1538,8 @@ static int build_ops(const Polynomial& poly, uint32_t identity, bool in_parts, O
             x.left = q;
             x.f1 = static_cast<float>(ldexp(1.0, -eq));
             x.identity = identity + k;
+            x.grown = grown | s.grown << kGrownBits;
+            grown = s.grown;
             add(x);
             from ^= 1;
         }
@@ -1588,7 +1617,7 @@ static int run_small(Work* w, int count, const Call& call, const Polynomial& pol
     const SmallPlan p = plan_small(w, count);
     uint8_t* const base = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<uintptr_t>(workspace), 1024));
     if (!workspace || base + p.bytes > static_cast<uint8_t*>(workspace) + bytes) return NML_ERR_WORKSPACE;
-    const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), nullptr, nullptr, nullptr, call.skip, count};
+    const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), nullptr, nullptr, nullptr, nullptr, call.skip, count};
     double* const q = reinterpret_cast<double*>(base + p.q_at);
     const bool half = call.in_dtype == NML_F16;
     auto gram = [&](auto n) {
@@ -1621,10 +1650,10 @@ static int run_group(Work* w, int count, const Call& call, const Steps& steps, v
     for (int k = 0; k < count; ++k) {
         const double elements = static_cast<double>(w[k].s.m) * w[k].s.n;
         const int e = std::min(exponent_below(steps.of[w[k].chained ? 0 : 1].largest), static_cast<int>(lround(0.5 * log2(elements))));
-        w[k].sx = static_cast<float>(ldexp(1.0, e));
+        w[k].sx = e;
     }
     const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), reinterpret_cast<Round*>(base + p.rounds_at),
-                      reinterpret_cast<int*>(base + p.done_at), base + p.blocks_at, call.skip, count};
+                      reinterpret_cast<int*>(base + p.done_at), reinterpret_cast<int*>(base + p.done_at) + kGroup + 1, base + p.blocks_at, call.skip, count};
 
     // rounds: a product of each class, with as many tiles as its matrices have
     PackParams<kMaxRounds> pack = {c, call.mo, call.eps, p.halves, 0, p.identity, call.math == NML_MATH_F16 ? steps.of[1].steps : 0, {}, {}};

@@ -1,4 +1,5 @@
-"""Orthogonalised matrices at the edges of their range: many steps on matrices that have not full rank, results over matrices."""
+"""Orthogonalised matrices at the edges of their range: many steps on matrices that have not full rank, norms far below eps,
+results over matrices, long vectors."""
 import math
 
 import pytest
@@ -154,3 +155,33 @@ def test_the_longest_vector():
     for part in (slice(0, 100000), slice(2 ** 30 - 100, 2 ** 30 + 100), slice(n - 100000, n)):
         assert bool((v[part] == 0.625).all()) and bool((p[part] == 1 - 0.3125).all())
     assert float(p.min()) == float(p.max()) == 0.6875
+
+
+@MODES
+@pytest.mark.parametrize("shapes", [[(200, 300)], [(300, 700), (90, 80)], [(700, 300)], [(512, 1100)] * 2 + [(1601, 1700)], [(40, 90), (64, 64)]], ids=str)
+def test_norms_below_eps(shapes, mode):
+    """X starts at |G| / (|G| + eps), however small: fp32 keeps such numbers as well as any.  While X is small a step multiplies it by a, rounded once in U, and
+    rounds it once: with two halves 2^-22 each and as much for the product of the low ones, in five steps 15 x 2^-22 = 3.6e-6 beyond what
+    the module's tolerance holds for norms of 1."""
+    gs = [gradient(r, c, seed=50 + r) for r, c in shapes]
+    for ratio in (0.3, 0.03, 1e-3, 1e-5, 1e-8, 1e-15):
+        eps = float(torch.tensor(float(gs[0].norm()) * (1 / ratio - 1)))
+        ys = ops.orthogonalize(gs, eps=eps, math=mode)
+        for g, y in zip(gs, ys):
+            want = plain(g, eps=eps)
+            assert off(y, want) <= (3.6e-6 if mode == "3xf16" and ratio <= 1e-3 else TOL[mode]), (ratio, g.shape)
+            assert off(ops.orthogonalize(g * 2.0 ** -60, eps=eps * 2.0 ** -60, math=mode), want) <= TOL[mode], (ratio, g.shape)   # (only their ratio counts)
+    for steps, c in ((1, COEF), (3, ((3.9, -4.0, 1.2), (0.3, -0.1, 0.0), (2.0, -1.5, 0.5))), (20, POLAR)):
+        for g in gs:
+            eps = float(torch.tensor(float(g.norm()) * 1e5))
+            assert off(ops.orthogonalize(g, steps=steps, coefficients=c, eps=eps, math=mode), plain(g, steps, c, eps)) <= TOL[mode], steps
+    ops.device_status()
+
+
+def test_optimizer_step_with_norms_below_eps():
+    shapes = [(130, 70), (300, 700), (64, 3, 7, 7)]
+    grads = [1e-13 * gradient(s[0], math.prod(s[1:]), seed=60 + k).reshape(s) for k, s in enumerate(shapes)]
+    params, momenta = [torch.zeros(s, device=DEV) for s in shapes], [torch.zeros(s, device=DEV) for s in shapes]
+    ops.muon_step(params, grads, momenta, lr=1.0, momentum=0.0, scaling=None)
+    for p, g in zip(params, grads):
+        assert off(-p.reshape(p.shape[0], -1), plain(g.reshape(p.shape[0], -1))) <= 3.6e-6
