@@ -125,6 +125,7 @@ struct alignas(16) Work {
     int fine, parts;                    // tiles to a block of a symmetric product, 1 or 2; parts of K of X X^T
     int sx;                             // X is stored times 2^sx, and more where it is small (see lift)
     int chained;
+    int lift;                           // written by the pass that finds the norm (see lift_of), for those behind it
 };
 template <int N>
 struct Group {
@@ -136,7 +137,6 @@ struct Common {
     double* sums;
     Round* rounds;
     int* done;        // the tile counter, and behind it every matrix's finished eighths of tiles
-    int* lifts;       // every matrix's lift
     uint8_t* blocks;
     const int* skip;  // the optimizer step's: do nothing where this is set
     int count;
@@ -179,8 +179,9 @@ __device__ __forceinline__ int owner_of(const int (&first)[N], int count, int k)
 // multiplied it by, as long as that is positive.
 constexpr int kMostLift = 100;
 __device__ __forceinline__ int lift_of(double own, double norm) {
-    const double over = norm / own;  // (NaN and infinities: none)
-    return over > 1.0 ? min(kMostLift, ilogb(over)) : 0;
+    if (!(norm >= 2.0 * own) || own == 0.0) return 0;
+    const double over = norm / own;
+    return over > 1.0 ? min(kMostLift, ilogb(over)) : 0;  // (infinities: none)
 }
 __device__ __forceinline__ int lifted(int lift, int grown) { return max(0, lift - grown); }
 constexpr int kGrownBits = 8;
@@ -324,8 +325,9 @@ struct PackParams {
     float diagonal[kMaxSteps];
     Round round[N];
 };
+// (five blocks an SM: 48 registers, hence more loads in flight than the 40 that fit six.  MLP step's 34 million elements 84 -> 75 us)
 template <int N, typename T>
-__global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__ PackParams<N> P) {
+__global__ void __launch_bounds__(256, 5) ortho_pack_kernel(const __grid_constant__ PackParams<N> P) {
     pdl_enter();
     if (skipped(P.c.skip)) return;
     __shared__ float tile[64][129];
@@ -369,8 +371,8 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const __grid_constant__
     for (int q = 1; q < 8; ++q) sum += part[q];
     const double own = sqrt(sum), norm = own + static_cast<double>(P.eps);
     const int lift = lift_of(own, norm);
-    const double inv = norm == 0.0 ? 0.0 : ldexp(1.0, w.sx + lift) / norm;  // (zeros stay zeros without an eps too)
-    if (half == 0 && tid == 0) P.c.lifts[k] = lift;
+    const double inv = norm == 0.0 ? 0.0 : __hiloint2double((1023 + w.sx + lift) << 20, 0) / norm;  // (zeros stay zeros without an eps too)
+    if (half == 0 && tid == 0) P.c.table[k].lift = lift;  // (no block of this pass uses what it reads there)
     const T* const in = static_cast<const T*>(s.in);
     auto update = [&](float v, float momentum) {  // of the element's gradient and new momentum
         if (P.mo.on) {
@@ -765,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_product_kernel(const __grid
                             auto word = [](const uint32_t* p) { return static_cast<uint32_t>(load_global(reinterpret_cast<const int*>(p))); };
                             w = {load_global(&from->s.m), load_global(&from->s.n), load_global(&from->nb), load_global(&from->wide), load_global(&from->fine),
                                  load_global(&from->parts), {word(&from->x[0]), word(&from->x[1])}, word(&from->sym), word(&from->partial), 1.f};
-                            const int lift = load_global(P.c.lifts + a), scale = load_global(&from->sx) + lifted(lift, grown & ((1 << kGrownBits) - 1));
+                            const int lift = load_global(&from->lift), scale = load_global(&from->sx) + lifted(lift, grown & ((1 << kGrownBits) - 1));
                             if (gram) w.factor = power_of_two(-2 * scale);
                             if (kind == RESULT) w.factor = power_of_two(-scale);
                             if (kind == ITERATE) w.factor = power_of_two(lifted(lift, grown >> kGrownBits) - lifted(lift, grown & ((1 << kGrownBits) - 1)));
@@ -1470,7 +1472,7 @@ static Plan plan_group(Work* w, int count, int math, int steps, int sms) {
     p.sums_at = round_up(sizeof(Work) * kGroup, 256);
     p.rounds_at = p.sums_at + round_up(sizeof(double) * p.sums, 256);
     p.done_at = p.rounds_at + round_up(sizeof(Round) * kMaxRounds, 256);
-    p.blocks_at = p.done_at + round_up(sizeof(int) * (2 * kGroup + 1), 1024);
+    p.blocks_at = p.done_at + round_up(sizeof(int) * (kGroup + 1), 1024);
     p.blocks_at = round_up(p.blocks_at, 1024);
     p.bytes = p.blocks_at + static_cast<size_t>(p.blocks) * 2 * kPlane;
     return p;
@@ -1617,7 +1619,7 @@ static int run_small(Work* w, int count, const Call& call, const Polynomial& pol
     const SmallPlan p = plan_small(w, count);
     uint8_t* const base = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<uintptr_t>(workspace), 1024));
     if (!workspace || base + p.bytes > static_cast<uint8_t*>(workspace) + bytes) return NML_ERR_WORKSPACE;
-    const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), nullptr, nullptr, nullptr, nullptr, call.skip, count};
+    const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), nullptr, nullptr, nullptr, call.skip, count};
     double* const q = reinterpret_cast<double*>(base + p.q_at);
     const bool half = call.in_dtype == NML_F16;
     auto gram = [&](auto n) {
@@ -1653,7 +1655,7 @@ static int run_group(Work* w, int count, const Call& call, const Steps& steps, v
         w[k].sx = e;
     }
     const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), reinterpret_cast<Round*>(base + p.rounds_at),
-                      reinterpret_cast<int*>(base + p.done_at), reinterpret_cast<int*>(base + p.done_at) + kGroup + 1, base + p.blocks_at, call.skip, count};
+                      reinterpret_cast<int*>(base + p.done_at), base + p.blocks_at, call.skip, count};
 
     // rounds: a product of each class, with as many tiles as its matrices have
     PackParams<kMaxRounds> pack = {c, call.mo, call.eps, p.halves, 0, p.identity, call.math == NML_MATH_F16 ? steps.of[1].steps : 0, {}, {}};
