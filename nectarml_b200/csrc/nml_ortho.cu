@@ -20,7 +20,8 @@
 // Operands are fp16.  |X| <= 1 bounds every element of every matrix here, so powers of two chosen on the host put all of them
 // into fp16's range; of the data only |G| next to eps matters to that (see lift_of).
 //   "3xf16" (fp32 results): every operand is a high and a low half, 22 bits, and a product is the three that matter, in fp32
-//           accumulators: an error of about 2^-22 of the largest element a product, below that of fp32 products by FMA.
+//           accumulators: an error of about 2^-22 of the largest element a product.  Five single steps are 1.0e-6 to 2.4e-6 off, fp32's 1.0e-6 to
+//           3.5e-6 (65 x 65 to 1600 x 1700); chained ones (see Polynomial) a third to four times as much as fp32's.
 //   "f16"   one product.  What may not be rounded to 11 bits is X itself where it is carried from step to step: noise in directions whose singular
 //           value is small grows by `a` a step (3.4^5 = 490), the signal in the others does not.  So X keeps its low half, and the
 //           update adds a I times it: one more K block a tile.  (Errors of the result against 64 bits at gradients of 32 strong
@@ -446,7 +447,8 @@ __device__ __forceinline__ long long load_wide(const long long* p) {
     return v;
 }
 // Pairs: the blocks as [plane][half][rows 0 to 63, 64 to 127][16][256 elements], so that one copy brings an operand's slice in both planes: both pieces of a
-// half, the same piece of both halves, or one piece.  (Eight copies of 8 KB a slice and block, whose issue paced the loop: 8192 x 2048 998 us; so 962.)
+// half, the same piece of both halves, or one piece.  (Eight copies of 8 KB a slice and block, whose issue paced the loop: 8192 x 2048 998 us; so 962.
+// Figures beside this kernel are of single passes; where passes follow one another, the power cap takes 1.1 to 1.2 times as long.)
 enum { MAP_HALF = 0, MAP_ACROSS = 1, MAP_PIECE = 2, kMaps = 3 };
 struct ProductParams {
     CUtensorMap map[kMaps];
@@ -1328,8 +1330,8 @@ static inline size_t round_up(size_t v, size_t m) { return (v + m - 1) / m * m; 
 // X_(k+t) = Q X_k with Q = U_(k+t-1) ... U_k.  So t steps need one product X X^T and one Q X over the long side, and products of
 // m x m matrices, half of each, in between: for 5 steps as 3 + 2 and n = r m it is 6 r + 14 instead of 15 r + 5 products of m^3.
 // What limits t is that the error of A_k, 2^-24 of its elements, grows by U^2 a step; kGrowth holds the chain's to that of one step from
-// a matrix 150 times as large.  (fp32 accuracy, against 64 bits: 3 + 2 as exact as five single steps over gradients of five kinds, 1e-6 to 8e-6;
-// all five in one chain 1e-6 to 4e-4.)  "f16" has no such reserve and takes single steps.
+// a matrix 150 times as large.  (Against 64 bits: 3 + 2 over gradients of five kinds 1e-6 to 8e-6; random 256 x 513 8.0e-6, 400 x 5000 1.4e-5 and 2048 x 8192 1.8e-6, the same
+// steps in fp32 2.1e-6, 5.3e-6 and 5.3e-6; all five in one chain 1e-6 to 4e-4.)  "f16" has no such reserve and takes single steps.
 constexpr double kGrowth = 150.0;
 struct Step {
     double a, b, c;

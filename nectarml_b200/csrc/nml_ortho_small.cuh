@@ -7,9 +7,11 @@
 // amplify the error of A by up to max u^2 each (a^2 = 11.9 with the default coefficients), so this is done in double and only where all steps together
 // amplify it by 1e10 at most: five default steps by 2.3e5, 2^-53 of which is 3e-11, nine by 5e9; and the result is rounded once.
 // With tiles of 128 in three products of halves a matrix of 64 x 147 took 116 us, 15 products of one tile, 7 us each: loads, flags and
-// stores.  Here it takes 59 us in three launches: partial Gram matrices of 64 columns a block; the steps, a block to a matrix; Q G, 64 columns a block.
-// Bound by the double-precision pipe: 64 FMAs a clock and SM, from registers or by mma.sync alike (both measured), so the lower blocks of a
-// product of 64 x 64 matrices take 2304 clocks; mma.sync needs a quarter of the shared-memory reads.
+// stores.  Here it takes 59 us in three launches: partial Gram matrices of 64 columns a block; the steps, a block to a matrix; Q G, 64 columns a block
+// (8, 52 and 11 us where each is timed alone, launch included).
+// The steps are bound by one block's double-precision pipe and by the barriers between its products: 64 FMAs a clock and SM, from registers or by mma.sync
+// alike (both measured), so the lower blocks of a product of 64 x 64 matrices take 2304 clocks and the 17 of five steps 39 thousand; the launch takes 99
+// thousand, of which the pipe is busy for 53 % (with what is done to the elements).  mma.sync needs a quarter of the shared-memory reads.
 #pragma once
 
 namespace nml_ortho {
