@@ -300,8 +300,7 @@ int nml_sgd_momentum_step(float* params, const float* grads, float* velocity, vo
  * the length of the dense run; a result may lie where its matrix does (with its strides and type); otherwise it must not overlap it (NML_ERR_INVALID),
  * nor another result, nor, in calls of more than 64 matrices, another matrix.  Coefficients under which a singular value could
  * grow beyond 64 are NML_ERR_UNSUPPORTED.  Results are bitwise repeatable; the
- * order of sums, and whether short sides up to 64 are taken in double, follow from the group's sizes, the polynomial (double holds a chain
- * of steps that amplifies errors by 1e10 at most: nine default ones) and the SMs in use. */
+ * order of sums, and whether a short side up to 64 is taken in double, follow from the group's sizes and the SMs in use. */
 typedef struct nml_matrix {
     const void* in;
     void* out;

@@ -1338,12 +1338,12 @@ struct Step {
     int ea, ep, eu, et, eq;  // A, P, U, T and Q are stored times 2^e
     bool starts, ends;       // a chain
     int grown;               // where it ends: log2 of what X may have been multiplied by, at least 0
+    double amplified;        // an error of the Gram matrix by this step, at most
 };
 struct Polynomial {
     Step step[kMaxSteps];
     int steps = 0;
     double largest = 1.0;    // singular value at the chains' starts, hence element of X
-    double growth = 1.0;     // of an error of the Gram matrix in one chain of all steps
 };
 static int exponent_below(double bound) {  // largest e with bound * 2^e <= 2^15
     return std::max(-24, std::min(24, static_cast<int>(floor(log2(32768.0 / std::max(bound, 1e-6))))));
@@ -1354,7 +1354,6 @@ static bool polynomial(const double* coefficients, int steps, bool chained, Poly
     double l = kBetween, lambda[kPoints + 1], q[kPoints + 1], growth = 1.0, multiplied = 0.0;  // (log2)
     p->steps = steps;
     p->largest = l;
-    p->growth = 1.0;
     bool starts = true;
     for (int k = 0; k < steps; ++k) {
         Step& s = p->step[k];
@@ -1384,8 +1383,8 @@ static bool polynomial(const double* coefficients, int steps, bool chained, Poly
         s.eu = exponent_below(mu * kBetween);
         s.et = exponent_below(mt * kBetween * kBetween);
         s.eq = exponent_below(mq * kBetween);
-        growth *= std::max(1.0, mu * mu);
-        p->growth *= std::max(1.0, mu * mu);
+        s.amplified = std::max(1.0, mu * mu);
+        growth *= s.amplified;
         if (!(next <= 4096.0)) return false;  // singular values beyond 64
         s.ends = !chained || k == steps - 1 || growth > kGrowth;
         starts = s.ends;
@@ -1577,17 +1576,18 @@ static void launch_pack(const PackParams<kMaxRounds>& all, const Call& call, int
 }
 constexpr int kFewRounds = 22;
 
-// Whether a group may go through double precision (see nml_ortho_small.cuh), and whether its steps do: one chain of them all amplifies what rounding leaves
-// of a Gram matrix's zero eigenvalues, 2^-53 either way, by kSmallGrowth at most.  Beyond, negative ones come near -1, where the polynomial has no bound
-// (rank 1, 64 x 147, default coefficients: 1e-10 off after 9 steps, 4e-6 after 12, 0.1 after 15, no numbers after 20); such steps are taken one by
-// one on X.
-constexpr double kSmallGrowth = 1e10;
+// Whether a group goes through double precision: see nml_ortho_small.cuh.
 static bool all_small(const Work* w, int count) {
     return std::all_of(w, w + count, [](const Work& v) { return v.s.m <= kSmall; });
 }
+// A chain of steps there amplifies what rounding leaves of a Gram matrix's zero eigenvalues, 2^-53 either way, by kSmallGrowth at most: beyond, negative ones
+// come near -1, where the polynomial has no bound (rank 1, 64 x 147, default coefficients: 1e-10 off after 9 steps in one chain, 4e-6 after 12, 0.1 after
+// 15, no numbers after 20).  Then X is formed, in fp32, and the next chain starts at its Gram matrix.
+constexpr double kSmallGrowth = 1e10;
 struct SmallPlan {
     int partials = 0, chunks = 0;
-    size_t sums_at = 0, q_at = 0, bytes = 0;
+    size_t sums_at = 0, q_at = 0, x_at = 0, bytes = 0;
+    size_t x[kGroup];  // where each matrix's X begins behind that
 };
 static SmallPlan plan_small(Work* w, int count) {
     SmallPlan p;
@@ -1601,7 +1601,12 @@ static SmallPlan plan_small(Work* w, int count) {
     }
     p.sums_at = round_up(sizeof(Work) * kGroup, 256);
     p.q_at = p.sums_at + sizeof(double) * kSmall * kSmall * p.partials;
-    p.bytes = p.q_at + sizeof(double) * kSmall * kSmall * count;
+    p.x_at = round_up(p.q_at + sizeof(double) * kSmall * kSmall * count, 256);
+    p.bytes = p.x_at;
+    for (int k = 0; k < count; ++k) {
+        p.x[k] = p.bytes - p.x_at;
+        p.bytes += round_up(sizeof(float) * w[k].s.m * w[k].s.n, 256);
+    }
     return p;
 }
 constexpr size_t kSmallStepsSmem = 5 * sizeof(double) * kSmall * kSmallPitch, kSmallResultSmem = 2 * sizeof(double) * kSmall * kSmallPitch;
@@ -1623,28 +1628,44 @@ static int run_small(Work* w, int count, const Call& call, const Polynomial& pol
     if (!workspace || base + p.bytes > static_cast<uint8_t*>(workspace) + bytes) return NML_ERR_WORKSPACE;
     const Common c = {reinterpret_cast<Work*>(base), reinterpret_cast<double*>(base + p.sums_at), nullptr, nullptr, nullptr, call.skip, count};
     double* const q = reinterpret_cast<double*>(base + p.q_at);
-    const bool half = call.in_dtype == NML_F16;
-    auto gram = [&](auto n) {
-        constexpr int N = decltype(n)::value;
-        Group<N> g;
-        std::copy(w, w + count, g.w);
-        nml::launch(half ? small_gram_kernel<N, __half> : small_gram_kernel<N, float>, p.partials, 256, 0, st, g, c, call.mo);
-    };
-    if (count <= 8) gram(std::integral_constant<int, 8>());
-    else gram(std::integral_constant<int, kGroup>());
-    SmallSteps s = {c, q, call.eps, poly.steps, {}, {}, {}};
-    for (int k = 0; k < poly.steps; ++k) s.a[k] = poly.step[k].a, s.b[k] = poly.step[k].b, s.k[k] = poly.step[k].c;
-    nml::launch(small_steps_kernel, count, 32 * kStepsWarps, kSmallStepsSmem, st, s);
-    const SmallResult r = {c, q, call.mo, call.out_dtype == NML_F16, call.apply, call.keep, call.rate};
-    nml::launch(half ? small_result_kernel<__half> : small_result_kernel<float>, p.chunks, 256, kSmallResultSmem, st, r);
-    NMLO_CUDA(cudaGetLastError());
-    nml::count_launches(3);
+    // Three launches a chain.  Where everything has to be read before a result is written, the last chain has no steps, and takes X to its place.
+    for (int first = 0, chains = 0; first < poly.steps || call.packed; ++chains) {
+        const bool starts = chains == 0;
+        int end = first;
+        for (double growth = 1.0; end < poly.steps && (end == first || growth * poly.step[end].amplified <= kSmallGrowth); ++end) growth *= poly.step[end].amplified;
+        const bool last = end == poly.steps && (!call.packed || first == end);
+        const bool half = starts && call.in_dtype == NML_F16;
+        const Momentum mo = starts ? call.mo : Call().mo;
+        auto gram = [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            Group<N> g;
+            std::copy(w, w + count, g.w);
+            for (int k = 0; k < count; ++k) {
+                Source& s = g.w[k].s;
+                float* const x = reinterpret_cast<float*>(base + p.x_at + p.x[k]);
+                if (!starts) s.in = x, s.in_i = s.n, s.in_j = 1;
+                if (!last) s.out = x, s.out_i = s.n, s.out_j = 1;
+            }
+            nml::launch(half ? small_gram_kernel<N, __half> : small_gram_kernel<N, float>, p.partials, 256, 0, st, g, c, mo);
+        };
+        if (count <= 8) gram(std::integral_constant<int, 8>());
+        else gram(std::integral_constant<int, kGroup>());
+        SmallSteps s = {c, q, call.eps, starts, end - first, {}, {}, {}};
+        for (int k = first; k < end; ++k) s.a[k - first] = poly.step[k].a, s.b[k - first] = poly.step[k].b, s.k[k - first] = poly.step[k].c;
+        nml::launch(small_steps_kernel, count, 32 * kStepsWarps, kSmallStepsSmem, st, s);
+        const SmallResult r = {c, q, mo, last && call.out_dtype == NML_F16, last && call.apply, call.keep, call.rate};
+        nml::launch(half ? small_result_kernel<__half> : small_result_kernel<float>, p.chunks, 256, kSmallResultSmem, st, r);
+        NMLO_CUDA(cudaGetLastError());
+        nml::count_launches(3);
+        if (last) break;
+        first = end;
+    }
     return NML_OK;
 }
 
-// One group: three launches.
+// One group: three launches (a chain).
 static int run_group(Work* w, int count, const Call& call, const Steps& steps, void* workspace, size_t bytes, cudaStream_t st) {
-    if (all_small(w, count) && !call.packed && steps.of[1].growth <= kSmallGrowth) return run_small(w, count, call, steps.of[1], workspace, bytes, st);
+    if (all_small(w, count)) return run_small(w, count, call, steps.of[1], workspace, bytes, st);
     int* err;
     int sms;
     if (const int rc = nml::current_device(&err, &sms)) return rc;
@@ -1810,9 +1831,7 @@ static int workspace_of(int count, int math, int steps, F&& size, size_t* bytes)
     int sms = nml::usable_sms(), filled = 0;
     for (int k = 0; k <= count; ++k) {
         if (filled == kGroup || (k == count && filled > 0)) {
-            // (small matrices: room for either way, as the coefficients, which decide, are not known here)
-            const size_t in_double = all_small(w, filled) ? plan_small(w, filled).bytes : 0;
-            *bytes = std::max(*bytes, std::max(in_double, plan_group(w, filled, math, steps, sms).bytes) + 1024);
+            *bytes = std::max(*bytes, (all_small(w, filled) ? plan_small(w, filled).bytes : plan_group(w, filled, math, steps, sms).bytes) + 1024);
             filled = 0;
         }
         if (k < count) {
@@ -1884,8 +1903,8 @@ int nml_orthogonalize(const nml_matrix* matrices, int count, int in_dtype, int o
         // in place: element by element
         if (x.in == x.out && (in_dtype != out_dtype || x.in_row != x.out_row || x.in_col != x.out_col)) return NML_ERR_INVALID;
     }
-    // Tiles are packed from all matrices of a group before the first result is written; from double precision, and from one group to the next, results are
-    // written while others' matrices are still to be read.
+    // Tiles are packed from all matrices of a group before the first result is written, and small matrices' X can be formed elsewhere first; but from one group
+    // to the next, results are written while others' matrices are still to be read.
     const Places where = places(matrices, count, in_dtype == NML_F16 ? 2 : 4, out_dtype == NML_F16 ? 2 : 4);
     if (where == CLASH || (where == OVER_INPUTS && count > kGroup)) return NML_ERR_INVALID;
     Steps poly;

@@ -4,8 +4,8 @@
 //   A = G G^T / (|G| + eps)^2;  U_k = a I + b A + c A^2,  A <- U_k A U_k,  Q <- U_k Q;  result = Q G / (|G| + eps)
 //
 // (all of them polynomials of the first A, so symmetric; |G|^2 is the trace of G G^T).  The steps square the condition number and
-// amplify the error of A by up to max u^2 each (a^2 = 11.9 with the default coefficients), so this is done in double and only where all steps together
-// amplify it by 1e10 at most: five default steps by 2.3e5, 2^-53 of which is 3e-11, nine by 5e9; and the result is rounded once.
+// amplify the error of A by up to max u^2 each (a^2 = 11.9 with the default coefficients), so this is done in double, and in one chain only as far as
+// its steps together amplify it by 1e10: five default steps do by 2.3e5, 2^-53 of which is 3e-11, nine by 5e9; and the result is rounded once.
 // With tiles of 128 in three products of halves a matrix of 64 x 147 took 116 us, 15 products of one tile, 7 us each: loads, flags and
 // stores.  Here it takes 59 us in three launches: partial Gram matrices of 64 columns a block; the steps, a block to a matrix; Q G, 64 columns a block
 // (8, 52 and 11 us where each is timed alone, launch included).
@@ -123,7 +123,8 @@ struct SmallSteps {
     Common c;
     double* q;       // results, kSmall x kSmall to a matrix
     double eps;
-    int steps;
+    bool starts;     // at G, which is normalised
+    int steps;       // none: Q is 1
     double a[kMaxSteps], b[kMaxSteps], k[kMaxSteps];  // coefficients
 };
 // The steps, a block to a matrix.
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(32 * kStepsWarps) small_steps_kernel(const __g
 #pragma unroll
         for (int o = 16; o > 0; o /= 2) trace += __shfl_xor_sync(0xffffffffu, trace, o);
         const double norm = sqrt(trace) + P.eps;
-        if (tid == 0) inverse = norm == 0.0 ? 0.0 : 1.0 / norm;  // (zeros stay zeros without an eps too)
+        if (tid == 0) inverse = !P.starts ? 1.0 : norm == 0.0 ? 0.0 : 1.0 / norm;  // (zeros stay zeros without an eps too)
     }
     __syncthreads();
     const double inv = inverse;
@@ -174,6 +175,7 @@ __global__ void __launch_bounds__(32 * kStepsWarps) small_steps_kernel(const __g
         });
     };
     const auto plain = [](double d, int, int) { return d; };
+    if (P.steps == 0) each([&](int i, int j) { Q[i][j] = i == j ? 1.0 : 0.0; });
     for (int k = 0; k < P.steps; ++k) {
         const bool last = k + 1 == P.steps;
         product(A, A, U, [&](double d, int i, int j) { return P.k[k] * d + P.b[k] * A[i][j] + (i == j ? P.a[k] : 0.0); });

@@ -48,8 +48,8 @@ def check_steps(g, y, steps, coefficients, mode, largest):
 @KINDS
 @pytest.mark.parametrize("rows,cols", [(64, 147), (147, 64), (20, 33)])
 def test_many_steps_on_small_matrices(rows, cols, kind, mode):
-    """In double as long as one chain of all steps is exact (its result is off by a rounding, and by 2^-53 times the sums' 147 terms and what
-    directions that are not there take from one step to the next, 3.45^9); one by one beyond."""
+    """In one chain as long as that is exact (its result is off by a rounding, and by 2^-53 times the sums' 147 terms and what directions
+    that are not there take from one step to the next, 3.45^9); in several beyond."""
     g = without_full_rank(rows, cols, kind)
     for steps in (1, 5, 9):
         assert off(ops.orthogonalize(g, steps=steps, math=mode), plain(g, steps)) <= 2.0 ** -24 + 147 * 2.0 ** -53 * 3.4445 ** 9, steps
@@ -57,6 +57,16 @@ def test_many_steps_on_small_matrices(rows, cols, kind, mode):
         check_steps(g, ops.orthogonalize(g, steps=steps, math=mode), steps, COEF, mode, 1.21)
     for steps in (15, 17, 20, 32):
         check_steps(g, ops.orthogonalize(g, steps=steps, coefficients=POLAR, math=mode), steps, POLAR, mode, 1.0018)
+    steep = ((60.0, 0.0, 0.0), (0.015, 0.0, 0.0), (50.0, 0.0, 0.0), (0.015, 0.0, 0.0), (60.0, 0.0, 0.0))   # two chains of steps that scale: X is rounded twice
+    y = ops.orthogonalize(g * 1e-3, steps=5, coefficients=steep, eps=float(torch.tensor(float(g.norm()) * 100)), math=mode)
+    assert off(y, plain(g * 1e-3, 5, steep, float(torch.tensor(float(g.norm()) * 100)))) <= 2.0 ** -22
+    half = g.half()
+    for steps in (5, 12):
+        y = ops.orthogonalize(half, steps=steps, coefficients=POLAR, math=mode)
+        assert y.dtype == torch.float16 and off(y, ops.orthogonalize(half.float(), steps=steps, coefficients=POLAR, math=mode)) <= 2.0 ** -11 + 2.0 ** -24
+    many = [without_full_rank(1 + k % 64, 1 + 7 * k, kind, k) for k in range(20)]
+    for x, y in zip(many, ops.orthogonalize(many, steps=25, coefficients=POLAR, math=mode)):
+        check_steps(x, y, 25, POLAR, mode, 1.0018)
     ops.device_status()
 
 
@@ -82,9 +92,17 @@ def test_results_over_other_matrices(rows, cols, mode):
     x, y = a.clone(), b.clone()
     ops.orthogonalize([x, y], out=[y, x], math=mode)
     assert off(y, want[0]) <= TOL[mode] and off(x, want[1]) <= TOL[mode]
+    if rows <= 64:   # (formed elsewhere, and taken to their places as they are)
+        assert all(torch.equal(p, q) for p, q in zip((y, x), ops.orthogonalize([a, b], math=mode)))
     x, y = a.clone(), torch.empty_like(a)
     ops.orthogonalize([x, x], out=[x, y], math=mode)
     assert off(x, want[0]) <= TOL[mode] and torch.equal(x, y)
+    for steps in (1, 2, 20):
+        x, y = a.half(), b.half()
+        u, v = x.clone(), y.clone()
+        ops.orthogonalize([u, v], out=[v, u], math=mode, steps=steps, coefficients=POLAR)
+        for got, z in ((v, x), (u, y)):   # (a rounding to fp16 more than in its own place)
+            assert off(got, plain(z, steps, POLAR)) <= TOL[mode] + 2 * 2.0 ** -11
     ops.device_status()
 
 

@@ -14,16 +14,19 @@ def _built(lib):
     pass
 
 
-def test_workspace_of_small_matrices_has_room_for_either_way(lib):
-    """Many steps are taken one by one on tiles, as those of larger matrices are; the coefficients, which decide, come with the call."""
+def test_workspace_of_small_matrices(lib):
+    """Partial products and results in double, and room for X in fp32, whatever the length: not for tiles of 128 rows."""
     def need(shapes, steps):
         m = (_lib.Matrix * len(shapes))(*[_lib.Matrix(P, P, r, c, c, 1, c, 1) for r, c in shapes])
         n = C.c_size_t()
         assert lib.nml_orthogonalize_workspace_size(m, len(shapes), _lib.NML_MATH_3XF16, steps, C.byref(n)) == 0
         return n.value
-    block = 65536
-    for steps in (1, 2, 5, 32):   # two iterates of two blocks, three symmetric matrices of one
-        assert need([(64, 147)], steps) >= 7 * block and need([(147, 64)] * 3, steps) >= 21 * block
+    one, tables = 64 * 64 * 8, 65536
+    for rows, cols in ((64, 147), (147, 64), (1, 1 << 24), (1 << 20, 3), (64, 1 << 20)):
+        for steps in (1, 5, 32):
+            x = 4 * rows * cols
+            assert x <= need([(rows, cols)], steps) <= x + 25 * one + tables, (rows, cols)
+            assert 3 * x <= need([(rows, cols)] * 3, steps) <= 3 * x + 75 * one + tables
 
 
 INVALID, WORKSPACE = 1, 2
