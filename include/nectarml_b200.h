@@ -293,9 +293,10 @@ int nml_sgd_momentum_step(float* params, const float* grads, float* velocity, vo
 /* Orthogonalised matrices: `steps` (1 to 32) steps of X <- (a I + b A + c A^2) X with A = X X^T, starting at G / (|G| + eps) (Frobenius
  * norm), (a, b, c) = coefficients[3 k ...] of step k (a host array).  With coefficients like 3.4445, -4.7750, 2.0315 five steps bring the
  * singular values near 1 and keep the singular vectors.  A group of matrices of any sizes goes through the launches together.
- *  NML_MATH_3XF16  fp32-accurate (errors 0.3 to 4 times those of the same steps in fp32): operands as high and low fp16 halves, three products, fp32 accumulators (the normalised iterate
- *                  fits fp16's range, which fp32 operands in general do not)
- *  NML_MATH_F16    operands rounded to fp16, except X where it is carried to the next step: 2 to 3e-3 of the result's norm
+ *  NML_MATH_3XF16  fp32-accurate (errors 0.3 to 4 times those of the same steps in fp32): operands as high and low fp16 halves, three products,
+ *                  fp32 accumulators (the normalised iterate fits fp16's range, which fp32 operands in general do not)
+ *  NML_MATH_F16    operands rounded to fp16, except X where it is carried to the next step: 2 to 3e-3 of the result's norm (to 1.5e-2
+ *                  where a matrix has a handful of singular values, over which errors do not average)
  * Zeros stay zeros; a matrix with a NaN or an infinity becomes NaN.  Matrices may be views: one of the strides (in elements) is 1, the other at least
  * the length of the dense run; a result may lie where its matrix does (with its strides and type); otherwise it must not overlap it (NML_ERR_INVALID),
  * nor another result, nor, in calls of more than 64 matrices, another matrix.  Coefficients under which a singular value could

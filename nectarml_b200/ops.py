@@ -236,7 +236,8 @@ def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], *, steps: int 
 
     ``g``: a matrix, a batch [n, rows, cols], or a sequence of such of any sizes, float32 or float16 (all of one), which go through
     the kernels together.  One dimension of a matrix is dense; transposed ones and slices of rows or columns are read in place.  ``math``: "3xf16"
-    (errors of 0.3 to 4 times those of the same steps in float32) or "f16" (faster, good to 2 to 3e-3 of the result's norm).  ``out`` may be ``g``
+    (errors of 0.3 to 4 times those of the same steps in float32) or "f16" (faster, good to 2 to 3e-3 of the result's norm, to 1.5e-2
+    where a matrix has few rows or columns).  ``out`` may be ``g``
     itself; results must not overlap one another.  ``coefficients``: (a, b, c), or a row for each step."""
     single = isinstance(g, torch.Tensor)
     items = [g] if single else g
